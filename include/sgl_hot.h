@@ -8,6 +8,9 @@
  *   (3) feature / TGN-memory row gather through a cache index
  *       (HBM-resident hot rows, pinned-host cold rows),
  *   (4) the cos(w*dt + b) time encoding.
+ * Next to them stand the operators of an attention layer over what was sampled:
+ * the rotary encoding of rows by their event times, the per-head norm of queries
+ * and keys with that rotation, and differential attention over ragged segments.
  *
  * Conventions
  *   - every pointer named in a "device" role must be dereferenceable from the
@@ -35,7 +38,7 @@
 extern "C" {
 #endif
 
-#define SGL_ABI_VERSION 8
+#define SGL_ABI_VERSION 9
 
 /* ------------------------------------------------------------------ status */
 #define SGL_OK        0
@@ -53,7 +56,8 @@ int32_t     sgl_abi_version(void);
 /* sizeof of the ABI's structs as this library was compiled, so that a binding
  * which mirrors them field by field (ctypes, cgo, JNI) can check its layout at
  * load time: which = 0 sgl_tcsr, 1 sgl_sample_params, 2 sgl_hop_out,
- * 3 sgl_cache, 4 sgl_gather_seg, 5 sgl_seed_query, 6 sgl_window_params;
+ * 3 sgl_cache, 4 sgl_gather_seg, 5 sgl_seed_query, 6 sgl_window_params,
+ * 7 sgl_rows, 8 sgl_rotary_params, 9 sgl_norm_side, 10 sgl_diff_attn_args;
  * 0 for any other index. */
 size_t      sgl_struct_bytes(int32_t which);
 
@@ -721,6 +725,105 @@ int32_t sgl_segment_max_ts(const int64_t* local, const int64_t* ts,
 int32_t sgl_time_encode(const void* dt, int32_t dt_dtype, int64_t N_max,
                         const int64_t* N_dev, const float* w, const float* b,
                         int32_t dim, float* out, void* stream);
+
+/* ------------------------------------------- operators of attention layers */
+#define SGL_DT_BF16 2
+#define SGL_DT_F16  3
+/* Rows of heads: element (n, h, d) is data[n * row_stride + h * head_stride + d]
+ * (strides in elements, the last axis contiguous). */
+typedef struct {
+    void*   data;
+    int64_t row_stride, head_stride;
+} sgl_rows;
+
+/* Rotation of the first rot_dim of a head's `dim` values by the angles
+ * pos * freq[i], i < rot_dim / 2, formed in 64 bits.  Pair i is (i, i + rot_dim/2),
+ * or (2i, 2i + 1) when interleaved; its values (a, b) become
+ * amplitude * (a cos - b sin, a sin + b cos), with `inverse` the transpose of
+ * that map (the gradient).  The other values are copied.  1 <= dim <= 1024,
+ * rot_dim even, 0 <= rot_dim <= dim. */
+typedef struct {
+    int32_t       dtype;               /* SGL_DT_F32 / _BF16 / _F16                */
+    int32_t       dim, rot_dim, interleaved, inverse, reserved;
+    double        amplitude;
+    const double* freq;                /* device [rot_dim / 2]; NULL iff rot_dim = 0 */
+} sgl_rotary_params;
+
+/* out = rotated x; out may be x itself (same strides), but may not overlap it
+ * otherwise.  Rows from *N_dev on (when given) are left as they were. */
+int32_t sgl_rotary(const sgl_rotary_params* p, int32_t heads, const sgl_rows* x,
+                   const int64_t* pos, int64_t N_max, const int64_t* N_dev,
+                   const sgl_rows* out, void* stream);
+
+/* One side (queries or keys) of a norm call: y = rotate(x * r * w) with
+ * r = (mean of x^2 over the head + eps)^-1/2 in 32 bits, w = weight[h *
+ * weight_stride + d] (weight_stride 0: shared by the heads; NULL: ones).
+ * Backward: y holds the gradient of y (read), dx and dweight (NULL: not wanted)
+ * are written; dweight has the shape of weight.  pos may be NULL iff rot_dim = 0. */
+typedef struct {
+    sgl_rows       x, y, dx;
+    const int64_t* pos;
+    int64_t        N_max;
+    const int64_t* N_dev;
+    const float*   weight;
+    int64_t        weight_stride;      /* 0 or dim */
+    float*         dweight;
+    int32_t        heads, reserved;
+} sgl_norm_side;
+
+/* One launch for `num` sides (1 or 2); p->inverse must be 0.  Backward sums the
+ * weights' gradients in a fixed order (workspace: one row per block). */
+int32_t sgl_qk_norm_rotary(const sgl_rotary_params* p, double eps, int32_t num,
+                           const sgl_norm_side* sides, void* stream);
+size_t  sgl_qk_norm_rotary_backward_workspace_bytes(const sgl_rotary_params* p,
+                                                    int32_t num, const sgl_norm_side* sides);
+int32_t sgl_qk_norm_rotary_backward(const sgl_rotary_params* p, double eps, int32_t num,
+                                    const sgl_norm_side* sides, void* workspace,
+                                    size_t workspace_bytes, void* stream);
+
+/* Differential attention over ragged sequences.  Query head h (of Hq) reads key
+ * head h / (Hq / Hk); with S_m = scale * q_m k_m^T for the two halves m = 1, 2
+ * of every head,   out = softmax(S_1) v - lam[h] * softmax(S_2) v.
+ *   q   (row, 2 * Hq, D) : head 2h + m     k   (key, 2 * Hk, D)
+ *   v   (key, Hk, Dv)                      out (row, Hq, Dv)
+ * Sequence b has the queries [q_ptr[b], q_ptr[b+1]) (q_ptr NULL: the one query
+ * b, Tq = B) and the keys [k_ptr[b], k_ptr[b+1]) (root_start_ptr of a sampled
+ * hop, for one); both pointer arrays ascend.  Query i of nq sees key j of nk when
+ *   !causal, or i + nk - nq - window < j <= i + nk - nq  (window 0: no lower end),
+ * and key_mask (NULL: all) is not 0 there.  A query that sees no key, or only keys
+ * whose score is -inf, gives zeros and passes no gradient.  Values of keys that a
+ * query does not see never reach its result, NaN and infinities included.
+ * Rows of no sequence: zeros with SGL_ATTN_ZERO_REST, else left as they were.
+ * B_dev (when given) is the live number of sequences, <= B.
+ * 1 <= D <= 128, 1 <= Dv <= 256, Tq and Tk below 2^31. */
+#define SGL_ATTN_ZERO_REST 1
+typedef struct {
+    int32_t        dtype, Hq, Hk, D, Dv, causal;
+    int64_t        window;
+    double         scale;
+    int64_t        B, Tq, Tk;
+    const int64_t* B_dev;
+    const int64_t* q_ptr;
+    const int64_t* k_ptr;
+    const uint8_t* key_mask;           /* device [Tk] */
+    const float*   lam;                /* device [Hq] */
+    sgl_rows       q, k, v, out;
+    float*         lse;                /* device [Tq, Hq, 2]: log-sum-exp of each map; NULL in a
+                                        * forward call that no backward follows */
+    sgl_rows       o2;                 /* softmax(S_2) v, kept for the backward; data NULL likewise */
+    sgl_rows       d_out, d_q, d_k, d_v;  /* backward */
+    float*         d_lam;              /* device [Hq] */
+    int32_t        flags, reserved;
+} sgl_diff_attn_args;
+
+size_t  sgl_diff_attn_workspace_bytes(const sgl_diff_attn_args* a);
+int32_t sgl_diff_attn(const sgl_diff_attn_args* a, void* workspace,
+                      size_t workspace_bytes, void* stream);
+/* Reads q, k, v, lam, out, lse, o2, d_out; writes d_q, d_k, d_v, d_lam.  No
+ * atomics: the same inputs give the same bits. */
+size_t  sgl_diff_attn_backward_workspace_bytes(const sgl_diff_attn_args* a);
+int32_t sgl_diff_attn_backward(const sgl_diff_attn_args* a, void* workspace,
+                               size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

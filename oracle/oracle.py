@@ -77,7 +77,7 @@ def load():
     if _cached is None:
         build()
         cdll = C.CDLL(LIB_PATH)
-        lib = _abi.bind(cdll, "sglo_")
+        lib = _abi.bind(cdll, "sglo_", without=_abi.MODEL_OPS)
         cdll.sglo_set_num_threads.argtypes = [C.c_int32]
         cdll.sglo_get_max_threads.restype = C.c_int32
         cdll.sglo_philox4x32_10.argtypes = [C.c_void_p] * 3

@@ -58,6 +58,10 @@ size_t      sglo_struct_bytes(int32_t which) {
         case 4: return sizeof(sgl_gather_seg);
         case 5: return sizeof(sgl_seed_query);
         case 6: return sizeof(sgl_window_params);
+        case 7: return sizeof(sgl_rows);
+        case 8: return sizeof(sgl_rotary_params);
+        case 9: return sizeof(sgl_norm_side);
+        case 10: return sizeof(sgl_diff_attn_args);
         default: return 0;
     }
 }

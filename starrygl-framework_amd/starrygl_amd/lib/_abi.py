@@ -5,7 +5,7 @@ header declares.  The product library exports them as ``sgl_*``.
 """
 import ctypes as C
 
-ABI_VERSION = 8
+ABI_VERSION = 9
 
 SGL_OK, SGL_EINVAL, SGL_ERANGE, SGL_ENOTSUP, SGL_EHIP, SGL_ENOMEM = 0, -1, -2, -3, -4, -5
 SAMPLE_RECENT, SAMPLE_UNIFORM = 0, 1
@@ -15,11 +15,13 @@ STATIC_HOP_MAX_SLOTS = 65536
 BATCH_MAX = 64
 UNIQUE_SORTED, UNIQUE_GROUPED, UNIQUE_PREMARKED, UNIQUE_MULTI_LAUNCH = 0, 1, 0x100, 0x200
 SAMPLE_MULTI_LAUNCH = 1
-DT_I64, DT_F32 = 0, 1
+DT_I64, DT_F32, DT_BF16, DT_F16 = 0, 1, 2, 3
+ATTN_ZERO_REST = 1
 
 SAMPLE_TYPES = {"recent": SAMPLE_RECENT, "uniform": SAMPLE_UNIFORM}
 
 i32, i64, u64, vp, sz = C.c_int32, C.c_int64, C.c_uint64, C.c_void_p, C.c_size_t
+f64 = C.c_double
 
 
 class TCSR(C.Structure):
@@ -63,8 +65,30 @@ class WindowParams(C.Structure):
                 ("first_k", i64), ("edge_tag", vp), ("tag_value", i64)]
 
 
+class Rows(C.Structure):
+    _fields_ = [("data", vp), ("row_stride", i64), ("head_stride", i64)]
+
+
+class RotaryParams(C.Structure):
+    _fields_ = [("dtype", i32), ("dim", i32), ("rot_dim", i32), ("interleaved", i32), ("inverse", i32), ("reserved", i32),
+                ("amplitude", f64), ("freq", vp)]
+
+
+class NormSide(C.Structure):
+    _fields_ = [("x", Rows), ("y", Rows), ("dx", Rows), ("pos", vp), ("N_max", i64), ("N_dev", vp), ("weight", vp),
+                ("weight_stride", i64), ("dweight", vp), ("heads", i32), ("reserved", i32)]
+
+
+class DiffAttnArgs(C.Structure):
+    _fields_ = [("dtype", i32), ("Hq", i32), ("Hk", i32), ("D", i32), ("Dv", i32), ("causal", i32), ("window", i64),
+                ("scale", f64), ("B", i64), ("Tq", i64), ("Tk", i64), ("B_dev", vp), ("q_ptr", vp), ("k_ptr", vp),
+                ("key_mask", vp), ("lam", vp), ("q", Rows), ("k", Rows), ("v", Rows), ("out", Rows), ("lse", vp),
+                ("o2", Rows), ("d_out", Rows), ("d_q", Rows), ("d_k", Rows), ("d_v", Rows), ("d_lam", vp),
+                ("flags", i32), ("reserved", i32)]
+
+
 # in the order of sgl_struct_bytes(which)
-STRUCTS = (TCSR, SampleParams, HopOut, Cache, GatherSeg, SeedQuery, WindowParams)
+STRUCTS = (TCSR, SampleParams, HopOut, Cache, GatherSeg, SeedQuery, WindowParams, Rows, RotaryParams, NormSide, DiffAttnArgs)
 
 
 P = C.POINTER
@@ -128,15 +152,28 @@ PROTOTYPES = {
     "block_build": (i32, [vp, vp, i64, i64, i64, i64, vp, vp, vp, vp]),
     "segment_max_ts": (i32, [vp, vp, i64, vp, i64, vp, vp, vp, vp]),
     "time_encode": (i32, [vp, i32, i64, vp, vp, vp, i32, vp, vp]),
+    "rotary": (i32, [P(RotaryParams), i32, P(Rows), vp, i64, vp, P(Rows), vp]),
+    "qk_norm_rotary": (i32, [P(RotaryParams), f64, i32, P(NormSide), vp]),
+    "qk_norm_rotary_backward_workspace_bytes": (sz, [P(RotaryParams), i32, P(NormSide)]),
+    "qk_norm_rotary_backward": (i32, [P(RotaryParams), f64, i32, P(NormSide), vp, sz, vp]),
+    "diff_attn_workspace_bytes": (sz, [P(DiffAttnArgs)]),
+    "diff_attn": (i32, [P(DiffAttnArgs), vp, sz, vp]),
+    "diff_attn_backward_workspace_bytes": (sz, [P(DiffAttnArgs)]),
+    "diff_attn_backward": (i32, [P(DiffAttnArgs), vp, sz, vp]),
 }
+# operators of attention layers: no counterpart among the sampling algorithms that the CPU oracle restates (the tests
+# hold them to plain 64-bit forms)
+MODEL_OPS = frozenset(n for n in PROTOTYPES if n.startswith(("rotary", "qk_norm_rotary", "diff_attn")))
 
 
 class BoundLib:
     """Entry points of one shared library, addressed without their prefix."""
 
-    def __init__(self, cdll, prefix):
+    def __init__(self, cdll, prefix, without=()):
         self._cdll, self._prefix = cdll, prefix
         for name, (res, args) in PROTOTYPES.items():
+            if name in without:
+                continue
             fn = getattr(cdll, prefix + name)  # AttributeError if a symbol is missing
             fn.restype, fn.argtypes = res, args
             setattr(self, name, fn)
@@ -146,8 +183,8 @@ class BoundLib:
         return msg.decode() if msg else ""
 
 
-def bind(cdll, prefix="sgl_"):
-    return BoundLib(cdll, prefix)
+def bind(cdll, prefix="sgl_", without=()):
+    return BoundLib(cdll, prefix, without)
 
 
 class SglError(RuntimeError):

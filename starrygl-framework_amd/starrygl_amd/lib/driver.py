@@ -12,6 +12,7 @@ import gc
 import os
 
 from . import _abi
+from .model_ops import ModelOps
 from ._abi import (TCSR, Cache, GatherSeg, HopOut, SampleParams, SeedQuery, WindowParams, check, i64, vp)
 
 
@@ -155,7 +156,7 @@ def check_unique_total(u_total):
                            "capacity was exceeded); re-initialise the remap state (HotPath.remap_reinit)")
 
 
-class HotPath:
+class HotPath(ModelOps):
     def __init__(self, lib, backend):
         self.lib, self.be = lib, backend
         if lib.abi_version() != _abi.ABI_VERSION:
