@@ -808,7 +808,7 @@ typedef struct {
     const uint8_t* key_mask;           /* device [Tk] */
     const float*   lam;                /* device [Hq] */
     sgl_rows       q, k, v, out;
-    float*         lse;                /* device [Tq, Hq, 2]: log-sum-exp of each map; NULL in a
+    float*         lse;                /* device [Tq, Hq, 2]: log2 of the sum of exp(S_m); NULL in a
                                         * forward call that no backward follows */
     sgl_rows       o2;                 /* softmax(S_2) v, kept for the backward; data NULL likewise */
     sgl_rows       d_out, d_q, d_k, d_v;  /* backward */

@@ -1,0 +1,4 @@
+// Backward matrix kernels of differential attention for fp32: a file of its own, so that the types compile side by side.
+#include "diff_attn_bwd.hpp"
+
+template void sgl::attn::backward_type<float>(const AttnArgs&, hipStream_t);

@@ -1,0 +1,4 @@
+// Forward matrix kernels of differential attention for fp32: a file of its own, so that the types compile side by side.
+#include "diff_attn_fwd.hpp"
+
+template void sgl::attn::forward_type<float>(const AttnArgs&, hipStream_t);

@@ -153,8 +153,6 @@ def test_what_is_not_finite_stays_with_those_who_see_it(hot, dtype):
         part = {name: ref[name][ok], name + "_tol": ref[name + "_tol"][ok]}
         _within(got.detach().cpu()[ok], part, name)
     assert y[100:135].isnan().any() and y[50].isnan().all()
-    # and without a later event's infinities being seen by an earlier row, exactly the same bits
-    assert torch.equal(y[65:100], diff_attention(*base[:3], lam, kp, kp, causal=True)[65:100])
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16, F16])
