@@ -21,14 +21,15 @@ FwdWork forward_work(const sgl_diff_attn_args& a) {
         units = a.Tq * a.Hk * w.groups;
         keys = a.B > 0 ? a.Tk / a.B : 0;
     } else {
-        const int rows = a.dtype != SGL_DT_F32 && heads_width(a) <= 64 ? 128 : 64;      // rows of a block
+        const int rows = 128;                   // of a block
         w.tiles = (int32_t)ceil_div<int64_t>(a.Tq, rows);
         w.groups = 1;
         units = (int64_t)w.tiles * a.Hq;
         keys = a.Tk / (a.B > 0 && a.B < w.tiles ? a.B : (w.tiles > 0 ? w.tiles : 1));
     }
-    // a call of fewer blocks than the chip holds side by side splits its key ranges, down to 256 keys a block
-    int64_t splits = units > 0 ? 1024 / units : 1;
+    // a call of fewer blocks than the chip holds side by side splits its key ranges, down to 256 keys a block (row tiles, whose
+    // partial results are as large as 2 x 128 rows of fp32, only when they would leave half of it idle)
+    int64_t splits = units > 0 ? (a.q_ptr ? 256 : 1024) / units : 1;
     if (splits > keys / 256) splits = keys / 256;
     w.splits = (int32_t)(splits < 1 ? 1 : splits > 64 ? 64 : splits);
     w.items = units * w.splits;
@@ -91,10 +92,10 @@ size_t forward_need(const sgl_diff_attn_args& a, int32_t parts) {
 }
 
 // query rows of a block of the backward kernels
-int64_t backward_row_tiles(const sgl_diff_attn_args& a) { return ceil_div<int64_t>(a.Tq, a.dtype == SGL_DT_F32 && heads_width(a) > 64 ? 32 : 128); }
+int64_t backward_row_tiles(const sgl_diff_attn_args& a) { return ceil_div<int64_t>(a.Tq, a.dtype == SGL_DT_F32 && heads_width(a) <= 64 ? 64 : 128); }
 size_t backward_need(const sgl_diff_attn_args& a) {
     if (!a.q_ptr) return align_up((size_t)seg_blocks(a) * (size_t)a.Hq * sizeof(float));
-    return align_up((size_t)a.Tq * (size_t)a.Hq * 2 * sizeof(float)) + align_up((size_t)a.Tq * 2 * sizeof(int32_t)) +
+    return align_up((size_t)a.Tq * (size_t)a.Hq * 2 * sizeof(float)) +
            align_up((size_t)backward_row_tiles(a) * (size_t)a.Hq * sizeof(float)) + 256;
 }
 
@@ -147,7 +148,6 @@ extern "C" int32_t sgl_diff_attn_backward(const sgl_diff_attn_args* a, void* wor
         seg_backward(g, as_stream(stream));
     } else {
         g.delta = ws.take<float>((size_t)a->Tq * (size_t)a->Hq * 2);
-        g.spans = ws.take<int32_t>((size_t)a->Tq * 2);
         g.lam_part = ws.take<float>((size_t)backward_row_tiles(*a) * (size_t)a->Hq);
         if (a->dtype == SGL_DT_F32) backward_type<float>(g, as_stream(stream));
         else if (a->dtype == SGL_DT_BF16) backward_type<__bf16>(g, as_stream(stream));

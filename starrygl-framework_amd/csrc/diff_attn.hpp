@@ -23,7 +23,6 @@ struct AttnArgs {
     float* part_ml;             // [parts, Tq * Hq, 2, 2]: running maximum (in powers of two) and sum
     float* part_o;              // [parts, Tq * Hq, 2, Dv]
     float* delta;               // backward [Tq, Hq, 2]: t_1, t_2
-    int32_t* spans;             // backward [Tq, 2]: the keys that a row sees, before key_mask
     float* lam_part;            // backward [row tiles, Hq]: sums of t_2
 };
 
@@ -49,6 +48,47 @@ __device__ __forceinline__ int32_t find_seq(const int64_t* __restrict__ ptr, int
         if (ptr[mid] <= i) lo = mid; else hi = mid;
     }
     return lo;
+}
+
+// The sequences of N elements per lane, first + at[0 .. N), 0 <= at < 64, of one wave (`first` the same in all lanes).  A search
+// by halves waits for one load after the other; here the wave looks at 64 entries at a time (one load up to 63 sequences,
+// three up to 250000) and the lanes find their own among the 64 that follow.
+template <int N>
+__device__ __forceinline__ void find_seqs(const int64_t* __restrict__ ptr, int32_t B, int64_t first, const int32_t (&at)[N], int32_t (&seq)[N]) {
+    const int lane = threadIdx.x & 63;
+    int32_t lo = 0, len = B + 1;                  // the entries at hand: [lo, lo + len)
+    while (len > 64) {
+        const int32_t step = (len + 63) / 64;
+        const int c = __popcll(__ballot(lane * step < len && ptr[lo + min(lane * step, len - 1)] <= first));
+        if (c == 0) {
+            len = 1;                              // all behind `first`
+            break;
+        }
+        lo += (c - 1) * step;
+        len = min(step, B + 1 - lo);
+    }
+    const int c = __popcll(__ballot(lane < len && ptr[lo + min(lane, len - 1)] <= first));
+    const int32_t s0 = lo + c - 1;                // the last entry <= first, -1: none
+    // how far the next 64 entries lie behind `first`
+    const int32_t k = s0 + 1 + lane;
+    const int64_t far = k <= B ? ptr[k] - first : 64;
+    const int32_t next = (int32_t)min(far, (int64_t)64);
+#pragma unroll
+    for (int n = 0; n < N; ++n) seq[n] = s0;
+    if (__builtin_amdgcn_readfirstlane(next) < 64) {
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            int32_t pos = 0;                      // entries <= first + at
+#pragma unroll
+            for (int w = 32; w > 0; w >>= 1)
+                if (__shfl(next, pos + w - 1) <= at[n]) pos += w;
+            if (__shfl(next, pos) <= at[n]) ++pos;
+            seq[n] = pos < 64 ? s0 + pos : find_seq(ptr, B, first + at[n]);      // (64 empty sequences in a row)
+        }
+    }
+#pragma unroll
+    for (int n = 0; n < N; ++n)
+        if (seq[n] >= B) seq[n] = -1;
 }
 
 __device__ __forceinline__ int32_t clamp_to(int64_t x, int64_t n) { return (int32_t)(x < 0 ? 0 : (x > n ? n : x)); }
@@ -149,48 +189,84 @@ __device__ __forceinline__ int row_of(int s, int j, int half) {
     return 2 * Mat<T>::EP * s + 8 * (j / 4) + 4 * half + j % 4;
 }
 
-// LDS image of rows of RB bytes: pieces of 8 rows x 8 chunks (16 bytes each), 1 KB, the pieces of 8 rows side by side; chunk c
-// of row r lies in its piece's row r % 8 at place (c ^ r) % 8.  Eight lanes that read one chunk column, and the sixteen that
-// read two columns of four rows (the transposed reads), then meet different banks; a piece is what one wave brings in at a time
-// (8 whole lines of 128 bytes); and an address is a lane's part plus a constant but for the two bits of the exchange.
+// LDS image of rows of RB bytes: pieces of 8 rows x 8 chunks (16 bytes each), 1 KB, the pieces of 8 rows side by side.  Row r is
+// line r & 7 of its pieces, its chunk c lies at place (c ^ mix(r)) & 7 of the line.  A 128-bit read serves 16 lanes a cycle, of
+// 32 consecutive rows those with an even (then those with an odd) number of ones in bits 2-4: bits 0-3 tell them apart, and
+// one chunk column meets all 64 banks once.  So do the transposed reads (4 columns of 4 rows, whose bit 1 moves the place
+// by 4).  A piece is what one wave brings in at a time (8 whole lines of memory); an address is a lane's part plus a
+// constant but for the bits of the exchange.
+__device__ __forceinline__ constexpr int mix(int r) { return ((r & 2) << 1) | ((r >> 2) & 1) | ((r >> 2) & 2); }
 template <int RB>
 __device__ __forceinline__ int at(int r, int chunk) {
-    return ((r >> 3) * (RB / 128) + (chunk >> 3)) * 1024 + (r & 7) * 128 + (((chunk ^ r) & 7) << 4);
+    return ((r >> 3) * (RB / 128) + (chunk >> 3)) * 1024 + ((r & 7) << 7) + (((chunk ^ mix(r)) & 7) << 4);
 }
 
-// row fragment: row r, chunk 2 i + half
+// row fragment: row row0 + col (row0 a multiple of 16), chunk 2 i + half
 template <typename T, int RB>
 __device__ __forceinline__ typename Mat<T>::Frag row_frag(const char* tile, int row0, int col, int i, int half) {
     return *reinterpret_cast<const typename Mat<T>::Frag*>(tile + (row0 >> 3) * (RB / 128) * 1024 + (i >> 2) * 1024 + (col >> 3) * (RB / 128) * 1024 +
-                                                           (col & 7) * 128 + ((((2 * i) & 7) ^ (half ^ (col & 7))) << 4));
+                                                           ((col & 7) << 7) + ((((2 * i) & 7) ^ (half ^ mix(col))) << 4));
 }
 
-// column fragment: elements (row0 + row_of(s, j, half), 32 t + lane column): the transposed left operand whose 32 rows are
-// the 32 elements from 32 t of the tile's rows
+// row fragment of half `map` of a head: RB / 32 chunks, whole pieces of 8 or (64-byte halves) half a piece
+template <typename T, int RB>
+__device__ __forceinline__ typename Mat<T>::Frag map_frag(const char* tile, int row0, int col, int map, int i, int half) {
+    if constexpr (RB >= 256) return row_frag<T, RB>(tile + map * (RB / 256) * 1024, row0, col, i, half);
+    else return map ? row_frag<T, RB>(tile, row0, col, i + 2, half) : row_frag<T, RB>(tile, row0, col, i, half);
+}
+
+// column fragment: elements (row0 + row_of(s, j, half), 32 t + lane column), row0 a multiple of 16: the transposed left operand
+// whose 32 rows are the 32 elements from 32 t of the tile's rows
 template <typename T, int RB>
 __device__ __forceinline__ typename Mat<T>::Frag col_frag(const char* tile, int row0, int s, int t, int lane) {
     const int half = lane >> 5;
     if constexpr (sizeof(T) == 2) {
-        const int r = 4 * half + ((lane & 15) >> 2), c = ((lane >> 4) & 1) * 2 + ((lane & 3) >> 1);       // chunk 4 t + c
-        const int base = (row0 / 8 + 2 * s) * (RB / 128) * 1024 + (t >> 1) * 1024 + r * 128 + ((((4 * t) & 7) ^ (c ^ r)) << 4) + (lane & 1) * 8;
+        const int r = 4 * half + ((lane & 15) >> 2), c = ((lane >> 4) & 1) * 2 + ((lane & 3) >> 1);       // row of a piece, chunk 4 t + c
+        const int place = ((((4 * t) & 7) ^ (c ^ mix(r))) << 4) + (lane & 1) * 8;
+        const char* base = tile + ((row0 / 8 + 2 * s) * (RB / 128) + (t >> 1)) * 1024;
         typedef SGL_LDS s16x4 lds4;
         union {
             s16x8 v;
             typename Mat<T>::Frag f;
         } u;
-        const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(tile + base));
-        const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(tile + base + (RB / 128) * 1024));
+        const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(base + (r * 128 + place)));
+        const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(base + (RB / 128) * 1024 + (r * 128 + (place ^ 32))));
         u.v = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
         return u.f;
     } else {
         typename Mat<T>::Frag f;
         const int c = (lane & 31) >> 2;                                                                      // chunk 8 t + c
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-            f[j] = *reinterpret_cast<const float*>(tile + ((row0 / 8 + s) * (RB / 128) + t) * 1024 + (4 * half + j) * 128 + ((c ^ (4 * half + j)) << 4) + (lane & 3) * 4);
+        for (int j = 0; j < 4; ++j) {
+            const int r = 4 * half + j;
+            f[j] = *reinterpret_cast<const float*>(tile + ((row0 / 8 + s) * (RB / 128) + t) * 1024 + (r << 7) + ((c ^ mix(r + 8 * (s & 1))) << 4) + (lane & 3) * 4);
+        }
         return f;
     }
 }
+
+// Fragments 0 .. N - 1 from LDS, `use`d in turn with the next DEPTH on their way.  The order is fixed: left to itself the
+// compiler, short of registers, reads each fragment into the same four and waits for it (a read takes as long as four
+// products).
+template <typename T, int N, int DEPTH>
+struct Pipe {
+    typename Mat<T>::Frag f[DEPTH];
+    template <typename Load>
+    __device__ __forceinline__ void fill(Load load) {
+#pragma unroll
+        for (int n = 0; n < DEPTH && n < N; ++n) f[n] = load(n);
+        __builtin_amdgcn_sched_barrier(0);
+    }
+    template <typename Load, typename Use>
+    __device__ __forceinline__ void drain(Load load, Use use) {
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            use(n, f[n % DEPTH]);
+            if (n + DEPTH < N) f[n % DEPTH] = load(n + DEPTH);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    }
+};
 
 // where chunk c of a staged row comes from: the two halves of a head ([2][D], D <= DP each), or one head of Dv <= 2 DP
 struct Source {
@@ -209,40 +285,148 @@ __device__ __forceinline__ Source run(const sgl_rows& r, int head, int Dv) {
     return Source{static_cast<const T*>(r.data) + (int64_t)head * r.head_stride, r.row_stride, 0, Dv};
 }
 
-// Stage ROWS rows from row0 (rows beyond `last` repeat it: their columns are hidden) into the image of RB-byte rows, by
-// NT threads.  DMA: every chunk is whole and aligned, and goes from memory to LDS without passing through registers (a
-// wave's 64 chunks land side by side, so the swizzle is applied to what each lane fetches); complete after
+// whether bit `bits` of register r's row is set, bits shifted by 4 half before
+__device__ __forceinline__ bool row_bit(uint32_t bits, int r) { return (bits >> (8 * (r / 4) + r % 4)) & 1; }
+
+// Staging of ROWS rows from row0 (rows beyond `last` repeat it: their columns are hidden) into the image of RB-byte rows by NT
+// threads.  DMA: every chunk is whole and aligned, and goes from memory to LDS without passing through registers (a
+// wave's 64 chunks land side by side, a piece, so the exchange is applied to what each lane fetches); complete after
 // staged().  Otherwise through registers, with zeros behind a row's valid elements.
-template <typename T, int DP, int ROWS, int NT, bool DMA>
-__device__ __forceinline__ void stage(char* tile, const Source& s, bool two, int32_t row0, int32_t last, int aligned) {
+template <typename T, int DP, int ROWS, int NT, bool DMA, bool TWO>
+struct Stager {
+    static constexpr int RB = 2 * DP * (int)sizeof(T), CH = RB / 16, EP = 16 / (int)sizeof(T);
+    static constexpr int NW = NT / 64, PG = CH / 8;             // waves; pieces side by side
+    static_assert(NW % PG == 0 || PG % NW == 0, "a wave covers whole columns or walks whole rows of pieces");
+    // the thread's own part of an address (fits 32 bits: dma_rows); the rest is the same for all lanes
+    static constexpr int COLS = PG > NW ? PG / NW : 1;          // columns of pieces that a wave walks through
+    static constexpr int KINDS = PG >= NW ? 2 : 1;              // rows of pieces of both parities, or of the wave's own
+    int32_t off[COLS][KINDS];
+
+    // row in its tile and chunk of what lane `lane` of piece `piece` brings
+    static __device__ __forceinline__ void of_piece(int piece, int lane, int& r, int& c) {
+        const int rows8 = piece / PG;
+        r = rows8 * 8 + (lane >> 3);
+        c = piece % PG * 8 + ((lane ^ mix(r)) & 7);
+    }
+    static __device__ __forceinline__ int64_t element(const Source& s, int r, int c) {
+        return r * s.row_stride + (TWO ? c / (CH / 2) * s.half_stride + c % (CH / 2) * EP : c * EP);
+    }
+    __device__ __forceinline__ void plan(const Source& s) {
+        if constexpr (DMA) {
+            const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+#pragma unroll
+            for (int p = 0; p < COLS; ++p)
+#pragma unroll
+                for (int q = 0; q < KINDS; ++q) {
+                    int r, c;
+                    of_piece(q * PG + p * NW + wave, lane, r, c);           // (PG > NW: wave < NW; else p = 0)
+                    off[p][q] = (int32_t)((element(s, r, c) - q * 8 * s.row_stride) * (int64_t)sizeof(T));
+                }
+        }
+    }
+    __device__ __forceinline__ void load(char* tile, const Source& s, int32_t row0, int32_t last, int aligned) const {
+        if constexpr (DMA) {
+            const int wave = threadIdx.x >> 6;
+            if (row0 + ROWS - 1 <= last) {
+                // a descriptor for the tile's rows: the thread's part of an address is one register, the rest is scalar (the
+                // descriptor's type exists in the device pass only)
+#if defined(__HIP_DEVICE_COMPILE__)
+                const auto rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(static_cast<const T*>(s.data) + (int64_t)row0 * s.row_stride), 0, 0x7FFFFFFF, 0x00027000);
+                const int32_t step = (int32_t)s.row_stride * (int32_t)sizeof(T) * (PG > NW ? 8 : NW / PG * 8);
+#pragma unroll
+                for (int k = 0; k < ROWS * CH / NT; ++k) {
+                    const int at0 = __builtin_amdgcn_readfirstlane((k * NW + wave) * 1024);
+                    __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (SGL_LDS void*)(tile + at0), 16, off[k % COLS][KINDS == 2 ? k / COLS & 1 : 0], k / COLS * step, 0, 0);
+                }
+#endif
+            } else {
+                const int lane = threadIdx.x & 63;
+#pragma unroll 1
+                for (int k = 0; k < ROWS * CH / NT; ++k) {
+                    const int piece = k * NW + wave;
+                    int r, c;
+                    of_piece(piece, lane, r, c);
+                    const int32_t n = row0 + r < last ? row0 + r : last;
+                    const T* src = static_cast<const T*>(s.data) + (int64_t)n * s.row_stride + element(s, 0, c);
+                    const int at0 = __builtin_amdgcn_readfirstlane(piece * 1024);
+                    __builtin_amdgcn_global_load_lds((SGL_GLOBAL void*)src, (SGL_LDS void*)(tile + at0), 16, 0, 0);
+                }
+            }
+        } else {
+            typedef typename Mat<T>::Frag Frag;
+            const T* __restrict__ base = static_cast<const T*>(s.data);
+            for (int i = threadIdx.x; i < ROWS * CH; i += NT) {
+                const int r = i / CH, c = i % CH;
+                const int32_t n = row0 + r < last ? row0 + r : last;
+                const int e = TWO ? (c % (CH / 2)) * EP : c * EP;
+                const T* src = base + (int64_t)n * s.row_stride + (TWO ? (c / (CH / 2)) * s.half_stride : 0) + e;
+                Frag f;
+                if (aligned && e + EP <= s.len) {
+                    f = *reinterpret_cast<const Frag*>(src);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < EP; ++j) f[j] = e + j < s.len ? src[j] : (T)0.0f;
+                }
+                *reinterpret_cast<Frag*>(tile + at<RB>(r, c)) = f;
+            }
+        }
+    }
+};
+
+// Staging for a pass in which something that is not finite has turned up: such elements become zero, and byte (row, chunk) of
+// `marks` has their bits.  What a column does not see then no longer reaches it as 0 * NaN; what it sees is put back as NaN
+// by the caller from the marks.
+template <typename T, int DP, int ROWS, int NT>
+__device__ __forceinline__ void stage_finite(char* tile, uint8_t* marks, const Source& s, bool two, int32_t row0, int32_t last) {
     constexpr int RB = 2 * DP * (int)sizeof(T), CH = RB / 16, EP = 16 / (int)sizeof(T);
     const T* __restrict__ base = static_cast<const T*>(s.data);
-    if constexpr (DMA) {
-#pragma unroll
-        for (int i0 = 0; i0 < ROWS * CH; i0 += NT) {
-            const int i = i0 + threadIdx.x, piece = i >> 6;
-            const int r = piece / (CH / 8) * 8 + ((i >> 3) & 7), c = piece % (CH / 8) * 8 + ((i ^ (i >> 3)) & 7);
-            const int32_t n = row0 + r < last ? row0 + r : last;
-            const T* src = base + (int64_t)n * s.row_stride + (two ? (c / (CH / 2)) * s.half_stride + (c % (CH / 2)) * EP : c * EP);
-            const int wave0 = __builtin_amdgcn_readfirstlane(i0 + ((int)threadIdx.x & ~63));
-            __builtin_amdgcn_global_load_lds((SGL_GLOBAL void*)src, (SGL_LDS void*)(tile + wave0 * 16), 16, 0, 0);
+#pragma unroll 1
+    for (int i = threadIdx.x; i < ROWS * CH; i += NT) {
+        const int r = i / CH, c = i % CH;
+        const int32_t n = row0 + r < last ? row0 + r : last;
+        const int e = two ? (c % (CH / 2)) * EP : c * EP;
+        const T* src = base + (int64_t)n * s.row_stride + (two ? (c / (CH / 2)) * s.half_stride : 0) + e;
+        T* to = reinterpret_cast<T*>(tile + at<RB>(r, c));
+        uint32_t bits = 0;
+#pragma unroll 1
+        for (int j = 0; j < EP; ++j) {
+            const T x = e + j < s.len ? src[j] : (T)0.0f;
+            const float y = (float)x;
+            const bool bad = !(y - y == 0.f);
+            to[j] = bad ? (T)0.0f : x;
+            bits |= bad ? 1u << j : 0u;
         }
+        marks[i] = (uint8_t)bits;
+    }
+}
+
+// marks of the elements 32 t .. 32 t + 31 of staged row r, a bit each
+template <typename T, int RB>
+__device__ __forceinline__ uint32_t marked(const uint8_t* marks, int r, int t) {
+    if constexpr (sizeof(T) == 2) {
+        return *reinterpret_cast<const uint32_t*>(marks + r * (RB / 16) + 4 * t);
     } else {
-        typedef typename Mat<T>::Frag Frag;
-        for (int i = threadIdx.x; i < ROWS * CH; i += NT) {
-            const int r = i / CH, c = i % CH;
-            const int32_t n = row0 + r < last ? row0 + r : last;
-            const int e = two ? (c % (CH / 2)) * EP : c * EP;
-            const T* src = base + (int64_t)n * s.row_stride + (two ? (c / (CH / 2)) * s.half_stride : 0) + e;
-            Frag f;
-            if (aligned && e + EP <= s.len) {
-                f = *reinterpret_cast<const Frag*>(src);
-            } else {
+        const uint2 w = *reinterpret_cast<const uint2*>(marks + r * (RB / 16) + 8 * t);
+        auto pack = [](uint32_t x) { return (x & 0xF) | (x >> 4 & 0xF0) | (x >> 8 & 0xF00) | (x >> 12 & 0xF000); };
+        return pack(w.x) | pack(w.y) << 16;
+    }
+}
+// any of chunks [c0, c1)
+template <int RB>
+__device__ __forceinline__ bool marked_any(const uint8_t* marks, int r, int c0, int c1) {
+    uint32_t x = 0;
+#pragma unroll 1
+    for (int c = c0; c < c1; ++c) x |= marks[r * (RB / 16) + c];
+    return x != 0;
+}
+// the results of a column at the marked elements become NaN
+template <typename T, int RB, int N>
+__device__ __forceinline__ void spoil(f32x16 (&x)[N], const uint8_t* marks, int r, int half) {
 #pragma unroll
-                for (int j = 0; j < EP; ++j) f[j] = e + j < s.len ? src[j] : (T)0.0f;
-            }
-            *reinterpret_cast<Frag*>(tile + at<RB>(r, c)) = f;
-        }
+    for (int t = 0; t < N; ++t) {
+        const uint32_t bits = marked<T, RB>(marks, r, t) >> (4 * half);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) x[t][e] = row_bit(bits, e) ? NAN : x[t][e];
     }
 }
 
@@ -252,20 +436,16 @@ __device__ __forceinline__ void staged() {
     __syncthreads();
 }
 
-// fragment `chunk` (of EP elements) of a row kept in registers; zero where the row is not live or beyond len
-template <typename T>
-__device__ __forceinline__ typename Mat<T>::Frag global_frag(const T* src, int e, int len, bool live, int aligned, bool negate) {
+// EP elements from element e of a row, kept in registers; zero beyond len.  WHOLE: every chunk is whole and aligned.
+template <typename T, bool WHOLE>
+__device__ __forceinline__ typename Mat<T>::Frag global_frag(const T* src, int e, int len, int aligned) {
     typename Mat<T>::Frag f;
     constexpr int EP = Mat<T>::EP;
-    if (live && aligned && e + EP <= len) {
+    if (WHOLE || (aligned && e + EP <= len)) {
         f = *reinterpret_cast<const typename Mat<T>::Frag*>(src + e);
     } else {
 #pragma unroll
-        for (int j = 0; j < EP; ++j) f[j] = live && e + j < len ? src[e + j] : (T)0.0f;
-    }
-    if (negate) {
-#pragma unroll
-        for (int j = 0; j < EP; ++j) f[j] = -f[j];
+        for (int j = 0; j < EP; ++j) f[j] = e + j < len ? src[e + j] : (T)0.0f;
     }
     return f;
 }
@@ -277,31 +457,88 @@ __device__ __forceinline__ f32x16 zero16() {
     return z;
 }
 
-// Work item of a block: consecutive items of one XCD (blocks go to the 8 of them in turn) are neighbours, so that what they
-// share lies in one L2.  The grid is a multiple of 8; items >= n do nothing.
-__device__ __forceinline__ int64_t xcd_item(int64_t n) {
-    const int64_t per = ceil_div<int64_t>(n, 8), b = blockIdx.x;
-    return (b % 8) * per + b / 8;
-}
-
-// smallest and largest over a wave
-__device__ __forceinline__ int wave_min(int x) {
+// 32 rows of results, one a lane of either half (the layout of the products), to memory through the wave's own piece of LDS
+// (32 rows of RB bytes): a row's elements lie in 2 x 16 registers of two lanes, eight bytes here and there; from LDS they go
+// out as whole 16-byte chunks side by side.  x[t]: 32 elements from 32 t; row r of them goes to dst(r) where keep(r) holds.
+template <typename T, int RB, int N, bool WHOLE, typename Dst, typename Keep>
+__device__ __forceinline__ void store_rows(const f32x16 (&x)[N], float scale, char* box, int lane, int len, int aligned, Dst dst, Keep keep) {
+    constexpr int BYTES = N * 32 * (int)sizeof(T), CH = BYTES / 16, EP = 16 / (int)sizeof(T);
+    static_assert(BYTES <= RB, "a row fits");
+    struct alignas(4 * sizeof(T)) Four {
+        T e[4];
+    };
+    const int half = lane >> 5, col = lane & 31;
 #pragma unroll
-    for (int m = 1; m < 64; m <<= 1) x = min(x, __shfl_xor(x, m));
-    return __builtin_amdgcn_readfirstlane(x);
-}
-__device__ __forceinline__ int wave_max(int x) { return -wave_min(-x); }
-
-// 32 keys [j0, j0 + 32) of a lane's column that it does not see become -inf: column span [lo, hi), key mask
-__device__ __forceinline__ void hide(f32x16& s, int32_t j0, int half, Span span, const uint8_t* __restrict__ mask, int32_t last) {
+    for (int t = 0; t < N; ++t)
 #pragma unroll
-    for (int r = 0; r < 16; ++r) {
-        const int32_t j = j0 + 8 * (r / 4) + 4 * half + r % 4;
-        bool see = j >= span.lo && j < span.hi;
-        if (mask != nullptr) see = see && mask[j < last ? j : last];
-        s[r] = see ? s[r] : NEG_INF;
+        for (int r4 = 0; r4 < 4; ++r4) {
+            Four y;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) y.e[e] = (T)(x[t][4 * r4 + e] * scale);
+            const int b = (t * 32 + 8 * r4 + 4 * half) * (int)sizeof(T);
+            *reinterpret_cast<Four*>(box + col * BYTES + ((((b >> 4) ^ col) & (CH - 1)) << 4) + (b & 15)) = y;
+        }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < 32 * CH / 64; ++i) {
+        const int r = i * (64 / CH) + lane / CH, c = lane % CH;
+        const typename Mat<T>::Frag f = *reinterpret_cast<const typename Mat<T>::Frag*>(box + r * BYTES + (((c ^ r) & (CH - 1)) << 4));
+        if (!keep(r)) continue;
+        T* to = dst(r) + c * EP;
+        if (WHOLE || (aligned && (c + 1) * EP <= len)) {
+            *reinterpret_cast<typename Mat<T>::Frag*>(to) = f;
+        } else {
+#pragma unroll
+            for (int e = 0; e < EP; ++e)
+                if (c * EP + e < len) to[e] = f[e];
+        }
     }
 }
+
+// store_rows of as many 32-element pieces at a time as PIECE bytes a row hold
+template <typename T, int PIECE, int N, bool WHOLE, typename Dst, typename Keep>
+__device__ __forceinline__ void store_pieces(const f32x16 (&x)[N], float scale, char* box, int lane, int len, int aligned, Dst dst, Keep keep) {
+    constexpr int FIT = PIECE / (32 * (int)sizeof(T)), AT = FIT >= N ? N : FIT >= 2 ? 2 : 1;
+    static_assert(FIT >= 1, "one piece fits");
+#pragma unroll
+    for (int t = 0; t < N; t += AT) {
+        f32x16 part[AT];
+#pragma unroll
+        for (int u = 0; u < AT; ++u) part[u] = x[t + u];
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        store_rows<T, AT * 32 * (int)sizeof(T), AT, WHOLE>(part, scale, box, lane, len - t * 32, aligned, [&](int r) { return dst(r) + t * 32; }, keep);
+    }
+}
+
+// Work item of a block: consecutive items of one XCD (blocks go to the 8 of them in turn) are neighbours, so that what they
+// share lies in one L2.  The grid is a multiple of 8; items >= n do nothing.
+__device__ __forceinline__ uint32_t xcd_item(uint32_t n) { return (blockIdx.x % 8) * ((n + 7) / 8) + blockIdx.x / 8; }
+
+// The spans of 32 columns (lanes l and l + 32 hold the same one): their union, and what all of them see.  Spans of ascending rows
+// ascend, so the first and the last that are not empty say it.
+struct Reach {
+    int32_t lo, hi;             // the union
+    int32_t from, to;           // seen by all
+};
+__device__ __forceinline__ Reach reach_of(Span span) {
+    const uint32_t live = (uint32_t)__ballot(span.lo < span.hi);
+    if (live == 0) return Reach{0x7FFFFFFF, 0, 0, 0};
+    const int first = __builtin_ctz(live), last = 31 - __builtin_clz(live);
+    return Reach{__builtin_amdgcn_readlane(span.lo, first), __builtin_amdgcn_readlane(span.hi, last), __builtin_amdgcn_readlane(span.lo, last),
+                 __builtin_amdgcn_readlane(span.hi, first)};
+}
+
+// bit k: element base + k lies in [lo, hi)
+__device__ __forceinline__ uint32_t span_bits(int32_t base, Span span) {
+    const int32_t from = min(max(span.lo - base, 0), 32), to = min(max(span.hi - base, 0), 32);
+    return (uint32_t)((1ull << to) - 1) & ~(uint32_t)((1ull << from) - 1);
+}
+// the key mask of the keys [j0, j0 + 32), the same in all lanes; keys beyond `last` repeat it
+__device__ __forceinline__ uint32_t mask_bits(const uint8_t* __restrict__ mask, int32_t j0, int lane, int32_t last) {
+    if (mask == nullptr) return ~0u;
+    return (uint32_t)__ballot(mask[min(j0 + (lane & 31), last)] != 0);
+}
+// whether a column sees key j
 __device__ __forceinline__ bool sees(int32_t j, Span span, const uint8_t* __restrict__ mask) {
     return j >= span.lo && j < span.hi && (mask == nullptr || mask[j]);
 }
@@ -326,6 +563,8 @@ struct Int {
 int64_t seg_blocks(const sgl_diff_attn_args& a);
 void seg_forward(const AttnArgs& g, hipStream_t st);
 void seg_backward(const AttnArgs& g, hipStream_t st);
+// rows whose offsets inside a tile of 64 fit 31 bits: up to 2^21 elements from row to row, 2^24 from half to half
+inline bool dma_rows(const sgl_rows& r) { return r.row_stride >= 0 && r.row_stride <= (1 << 21) && r.head_stride >= 0 && r.head_stride <= (1 << 24); }
 template <typename T>
 void forward_type(const AttnArgs& g, hipStream_t st);
 template <typename T>

@@ -1,13 +1,15 @@
 // Forward kernels of differential attention on the matrix units.
 //
-// A wave takes query rows of one head and ONE of the two maps, the queries as the COLUMNS of its products: S^T = K_m Q_m^T has
-// its keys in registers and one query per lane, so the softmax's running maximum and sum are one number per lane, and P^T is
-// already laid out as the right operand of O^T += V^T P^T.  The two waves of a row group share the staged keys and values
-// and join their maps at the end.  Rows of different sequences share a tile: every column has its own span of keys, and
+// A wave takes 32 query rows of one head as the COLUMNS of its products: S_m^T = K_m Q_m^T has its keys in registers and one
+// query per lane, so the softmax's running maximum and sum are one number per lane and map, and P^T is already laid out as
+// the right operand of O^T += V^T P^T.  Rows of different sequences share a tile: every column has its own span of keys, and
 // the tile walks the union (which for ascending pointers is one run).
 //
-// One query per sequence over a long history (no q_ptr): the query heads of a group are the columns, and the two row groups take
-// every other sub-tile of keys.
+// Heads up to 64 wide (16-bit; fp32 up to 32) keep both maps in one wave, and a fragment of the values feeds both.  Wider ones have no registers for
+// that: two waves take a map each and join at the end.
+//
+// One query per sequence over a long history (no q_ptr): the query heads of a group are the columns, a map to a wave, and two
+// groups of waves take every other sub-tile of keys.
 #pragma once
 
 #include "diff_attn.hpp"
@@ -16,84 +18,84 @@ namespace sgl {
 namespace attn {
 namespace {
 
-template <typename T, int DP>
+template <typename T, int DP, bool HEADS>
 struct Shape {
     static constexpr int RB = 2 * DP * (int)sizeof(T);          // bytes of a staged row, of keys and of values
-    static constexpr int BN = 32768 / (2 * RB) >= 64 ? 64 : 32; // keys of a tile
+    static constexpr int MAPS = !HEADS && RB <= 256 ? 2 : 1;    // of a wave
+    static constexpr int WAVES = HEADS || MAPS == 2 ? 4 : 8, GROUPS = WAVES * MAPS / 2, NT = WAVES * 64;
+    static constexpr int BN = RB <= (HEADS ? 256 : 128) ? 64 : 32;      // keys of a tile
     static constexpr int TILE = 2 * BN * RB;
     static constexpr int EP = Mat<T>::EP;
     static constexpr int QS = DP / (2 * EP);                    // steps over a half of a head
     static constexpr int PS = 32 / (2 * EP);                    // steps over 32 keys
     static constexpr int VT = 2 * DP / 32;                      // 32-wide tiles of the values
-    // column tiles of a wave: with two, every fragment read from LDS feeds two products (16-bit types are bound by LDS reads
-    // with one); the 128-wide heads have no registers for them, and fp32's products are slow enough without
-    static constexpr int RT = sizeof(T) == 2 && DP <= 64 ? 2 : 1;
-    static constexpr int ROWS = 2 * 32 * RT;                    // rows of a block
+    static constexpr int ROWS = GROUPS * 32;                    // query rows of a block
 };
 
 // A maximum may grow by this much (powers of two) before the sums and results are rescaled to it: probabilities stay below
 // 2^8, and most tiles leave the 2 DP / 32 x 16 multiplications of every column tile out.
 constexpr float SLACK = 8.f;
 
-template <typename T, int DP, int RT>
+template <typename T, int DP, int MAPS>
 struct State {
-    f32x16 o[RT][Shape<T, DP>::VT];
-    float m[RT], l[RT];
+    static constexpr int VT = 2 * DP / 32;
+    f32x16 o[MAPS][VT];
+    float m[MAPS], l[MAPS];
     __device__ __forceinline__ void reset() {
 #pragma unroll
-        for (int c = 0; c < RT; ++c) {
+        for (int c = 0; c < MAPS; ++c) {
             m[c] = NEG_INF;
             l[c] = 0.f;
 #pragma unroll
-            for (int t = 0; t < Shape<T, DP>::VT; ++t) o[c][t] = zero16();
+            for (int t = 0; t < VT; ++t) o[c][t] = zero16();
         }
     }
-    // whether something that is not a number got into a column that sees any key.  A value that is not finite, in a key that
-    // the column does not see, enters as 0 * NaN or 0 * inf; the pass is then done again key by key.
-    __device__ __forceinline__ bool spoilt(const Span (&span)[RT]) const {
+    // whether something that is not a number got in: a value that is not finite, in a key that the column does not see, enters as
+    // 0 * NaN or 0 * inf.  The keys are then gone through again without such values.
+    __device__ __forceinline__ bool spoilt() const {
         bool bad = false;
 #pragma unroll
-        for (int c = 0; c < RT; ++c) {
-            bool b = false;
+        for (int c = 0; c < MAPS; ++c)
 #pragma unroll
-            for (int t = 0; t < Shape<T, DP>::VT; ++t)
+            for (int t = 0; t < VT; ++t)
 #pragma unroll
-                for (int r = 0; r < 16; ++r) b = b || o[c][t][r] != o[c][t][r];
-            bad = bad || (b && span[c].lo < span[c].hi);
-        }
+                for (int r = 0; r < 16; ++r) bad = bad || o[c][t][r] != o[c][t][r];
         return bad;
     }
 };
 
-// one sub-tile of 32 keys
-template <typename T, int DP, int RT, bool CAREFUL>
-__device__ __forceinline__ void step(State<T, DP, RT>& st, const typename Mat<T>::Frag (&q)[RT][Shape<T, DP>::QS], const char* ktile, const char* vtile, int sub,
-                                     int map, int32_t j0, bool all, const Span (&span)[RT], const AttnArgs& g, int lane) {
-    typedef Shape<T, DP> S;
+// one sub-tile of 32 keys; map0: the first of the wave's maps
+template <typename T, int DP, int MAPS>
+__device__ __forceinline__ void step(State<T, DP, MAPS>& st, const typename Mat<T>::Frag (&q)[MAPS][Shape<T, DP, false>::QS], const char* ktile, const char* vtile, int sub,
+                                     int map0, int32_t j0, bool all, Span span, const AttnArgs& g, int lane) {
+    typedef Shape<T, DP, false> S;
     typedef Mat<T> M;
     constexpr int RB = S::RB;
     const int half = lane >> 5, col = lane & 31;
-    f32x16 s[RT];
+    constexpr int AHEAD = MAPS == 2 ? 2 : 4;                    // (each feeds MAPS products of the values)
+    f32x16 s[MAPS];
 #pragma unroll
-    for (int c = 0; c < RT; ++c) s[c] = zero16();
-    // a half of a head is RB / 2 bytes: RB / 32 chunks, whole pieces of 8 or (64-byte halves) half a piece
-    const char* kmap = RB >= 256 ? ktile + map * (RB / 256) * 1024 : ktile;
-#pragma unroll
-    for (int i = 0; i < S::QS; ++i) {
-        typename M::Frag k;
-        if constexpr (RB >= 256) k = row_frag<T, RB>(kmap, sub * 32, col, i, half);
-        else k = map ? row_frag<T, RB>(kmap, sub * 32, col, i + 2, half) : row_frag<T, RB>(kmap, sub * 32, col, i, half);
-#pragma unroll
-        for (int c = 0; c < RT; ++c) s[c] = M::mma(k, q[c][i], s[c]);
-    }
+    for (int c = 0; c < MAPS; ++c) s[c] = zero16();
+    // (the maps take turns: products into one sum follow each other at a distance)
+    auto load_k = [&](int n) { return map_frag<T, RB>(ktile, sub * 32, col, MAPS == 2 ? n & 1 : map0, n / MAPS, half); };
+    auto load_v = [&](int n) { return col_frag<T, RB>(vtile, sub * 32, n / S::VT, n % S::VT, lane); };
+    Pipe<T, MAPS * S::QS, AHEAD> keys_ahead;
+    keys_ahead.fill(load_k);
+    keys_ahead.drain(load_k, [&](int n, const typename M::Frag& k) { s[n % MAPS] = M::mma(k, q[n % MAPS][n / MAPS], s[n % MAPS]); });
+    // the first values are on their way while the probabilities are formed
+    Pipe<T, S::PS * S::VT, AHEAD> values_ahead;
+    values_ahead.fill(load_v);
     if (!all) {
+        const uint32_t see = (span_bits(j0, span) & mask_bits(g.a.key_mask, j0, lane, (int32_t)g.a.Tk - 1)) >> (4 * half);
 #pragma unroll
-        for (int c = 0; c < RT; ++c) hide(s[c], j0, half, span[c], g.a.key_mask, (int32_t)g.a.Tk - 1);
+        for (int c = 0; c < MAPS; ++c)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s[c][r] = row_bit(see, r) ? s[c][r] : NEG_INF;
     }
-    float top[RT];
+    float top[MAPS];
     bool grows = false;
 #pragma unroll
-    for (int c = 0; c < RT; ++c) {
+    for (int c = 0; c < MAPS; ++c) {
         float t = s[c][0];
 #pragma unroll
         for (int r = 1; r < 16; ++r) t = fmaxf(t, s[c][r]);
@@ -102,7 +104,7 @@ __device__ __forceinline__ void step(State<T, DP, RT>& st, const typename Mat<T>
     }
     if (__any(grows)) {
 #pragma unroll
-        for (int c = 0; c < RT; ++c) {
+        for (int c = 0; c < MAPS; ++c) {
             const float mn = fmaxf(st.m[c], top[c]);
             const float f = mn == NEG_INF ? 1.f : exp2_hw(st.m[c] - mn);
             st.m[c] = mn;
@@ -114,7 +116,7 @@ __device__ __forceinline__ void step(State<T, DP, RT>& st, const typename Mat<T>
         }
     }
 #pragma unroll
-    for (int c = 0; c < RT; ++c) {
+    for (int c = 0; c < MAPS; ++c) {
         const float ms = st.m[c] == NEG_INF ? 0.f : st.m[c];
         float sum = 0.f;
 #pragma unroll
@@ -124,319 +126,349 @@ __device__ __forceinline__ void step(State<T, DP, RT>& st, const typename Mat<T>
         }
         st.l[c] += sum;
     }
-    if constexpr (!CAREFUL) {
+    typename M::Frag p[MAPS];
+    values_ahead.drain(load_v, [&](int n, const typename M::Frag& v) {
 #pragma unroll
-        for (int i = 0; i < S::PS; ++i) {
-            typename M::Frag p[RT];
-#pragma unroll
-            for (int c = 0; c < RT; ++c) p[c] = to_frag<T>(s[c], i);
-#pragma unroll
-            for (int t = 0; t < S::VT; ++t) {
-                const typename M::Frag v = col_frag<T, RB>(vtile, sub * 32, i, t, lane);
-#pragma unroll
-                for (int c = 0; c < RT; ++c) st.o[c][t] = M::mma(v, p[c], st.o[c][t]);
-            }
+        for (int c = 0; c < MAPS; ++c) {
+            if (n % S::VT == 0) p[c] = to_frag<T>(s[c], n / S::VT);
+            st.o[c][n % S::VT] = M::mma(v, p[c], st.o[c][n % S::VT]);
         }
-    } else {
-        // one key at a time, taken over by the columns that see it
-        for (int i = 0; i < S::PS; ++i)
-            for (int jj = 0; jj < 2 * S::EP; ++jj) {
-                const int hh = jj / S::EP, j = jj % S::EP;
-                const int32_t key = j0 + row_of<T>(i, j, hh);
-#pragma unroll
-                for (int c = 0; c < RT; ++c) {
-                    const bool on = sees(key, span[c], g.a.key_mask);
-                    typename M::Frag p;
-                    float x = 0.f;
-#pragma unroll
-                    for (int r = 0; r < 16; ++r)
-                        if (r == i * S::EP + j) x = s[c][r];
-#pragma unroll
-                    for (int e = 0; e < S::EP; ++e) p[e] = e == j && half == hh ? (T)x : (T)0.f;
-#pragma unroll
-                    for (int t = 0; t < S::VT; ++t) {
-                        typename M::Frag v = col_frag<T, RB>(vtile, sub * 32, i, t, lane);
-#pragma unroll
-                        for (int e = 0; e < S::EP; ++e) v[e] = e == j && half == hh ? v[e] : (T)0.f;
-                        const f32x16 n = M::mma(v, p, st.o[c][t]);
-#pragma unroll
-                        for (int r = 0; r < 16; ++r) st.o[c][t][r] = on ? n[r] : st.o[c][t][r];
-                    }
-                }
-            }
-    }
+    });
 }
 
-// HEADS: the columns are the query heads of one key head, all at query `seq`; otherwise 32 RT query rows of one head
+// HEADS: the columns are the query heads of one key head, all at query `seq`; otherwise 32 query rows of one head
 template <typename T, int DP, bool HEADS, bool DMA>
-__global__ __launch_bounds__(BLOCK, 2) void fwd_kernel(AttnArgs g, FwdWork w) {
-    typedef Shape<T, DP> S;
+__global__ __launch_bounds__((Shape<T, DP, HEADS>::NT), 2) void fwd_kernel(AttnArgs g, FwdWork w) {
+    typedef Shape<T, DP, HEADS> S;
     typedef Mat<T> M;
-    constexpr int RB = S::RB, BN = S::BN, RT = HEADS ? 1 : S::RT;
+    constexpr int RB = S::RB, BN = S::BN, MAPS = S::MAPS, VT = S::VT;
     __shared__ __align__(16) char s_a[S::TILE];
     __shared__ __align__(16) char s_b[S::TILE];
-    __shared__ int s_lo[2], s_hi[2], s_bad;
+    __shared__ __align__(8) uint8_t s_marks[BN * (RB / 16)];
+    __shared__ int s_lo[S::GROUPS], s_hi[S::GROUPS], s_bad;
     const sgl_diff_attn_args& a = g.a;
     const int G = a.Hq / a.Hk;
-    const int64_t item = xcd_item(w.items);
+    const uint32_t item = xcd_item((uint32_t)w.items);
     if (item >= w.items) return;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5, col = lane & 31;
-    const int map = wave & 1, group = wave >> 1;
+    const int map0 = MAPS == 2 ? 0 : wave & 1, group = MAPS == 2 ? wave : wave >> 1;
     const int32_t B = (int32_t)live_count(a.B_dev, a.B);
-    const int split = (int)(item % w.splits);
-    int64_t rest = item / w.splits;
+    const int split = (int)(item % (uint32_t)w.splits);
+    uint32_t rest = item / (uint32_t)w.splits;
 
-    int hk, h[RT];
-    int64_t i[RT];
-    Span span[RT];
-    bool mine[RT];              // the column is a row of the result
-#pragma unroll
-    for (int c = 0; c < RT; ++c) span[c] = Span{0, 0};
+    int hk, h;
+    int32_t i, i0 = 0, seq;     // the lane's query row, the wave's first
+    bool mine;                  // the column is a row of the result
     if constexpr (HEADS) {
-        const int cg = (int)(rest % w.groups);
-        rest /= w.groups;
-        hk = (int)(rest % a.Hk);
-        i[0] = rest / a.Hk;
-        const int32_t seq = i[0] < B ? (int32_t)i[0] : -1;
-        mine[0] = cg * 32 + col < G && (seq >= 0 || (a.flags & SGL_ATTN_ZERO_REST));
-        h[0] = hk * G + (cg * 32 + col < G ? cg * 32 + col : 0);
-        if (cg * 32 + col < G) span[0] = keys_of(a, seq, i[0]);
+        const int cg = (int)(rest % (uint32_t)w.groups);
+        rest /= (uint32_t)w.groups;
+        hk = (int)(rest % (uint32_t)a.Hk);
+        i = (int32_t)(rest / (uint32_t)a.Hk);
+        seq = i < B ? i : -1;
+        mine = cg * 32 + col < G;
+        h = hk * G + (mine ? cg * 32 + col : 0);
     } else {
         // the heads of a group next to each other (they read the same keys); of a causal call the long rows first
-        const int hg = (int)(rest % G);
-        rest /= G;
-        hk = (int)(rest / w.tiles);
-        int32_t tile = (int32_t)(rest % w.tiles);
+        const int hg = (int)(rest % (uint32_t)G);
+        rest /= (uint32_t)G;
+        hk = (int)(rest / (uint32_t)w.tiles);
+        int32_t tile = (int32_t)(rest % (uint32_t)w.tiles);
         if (a.causal) tile = w.tiles - 1 - tile;
-#pragma unroll
-        for (int c = 0; c < RT; ++c) {
-            h[c] = hk * G + hg;
-            i[c] = (int64_t)tile * S::ROWS + group * 32 * RT + c * 32 + col;
-            const int32_t seq = i[c] >= a.Tq ? -1 : a.q_ptr ? find_seq(a.q_ptr, B, i[c]) : (i[c] < B ? (int32_t)i[c] : -1);
-            span[c] = keys_of(a, seq, i[c]);
-            mine[c] = i[c] < a.Tq && (seq >= 0 || (a.flags & SGL_ATTN_ZERO_REST));
-        }
+        h = hk * G + hg;
+        i0 = tile * S::ROWS + group * 32;
+        i = i0 + col;
+        mine = i < a.Tq;
+        const int32_t at[1] = {col};
+        int32_t found[1];
+        find_seqs<1>(a.q_ptr, B, i0, at, found);
+        seq = found[0];
     }
-    // the wave's union of spans, and the run that all its columns see
-    int32_t ulo = 0x7FFFFFFF, uhi = 0, alo = 0, ahi = 0x7FFFFFFF;
+    Span span = keys_of(a, mine ? seq : -1, i);
+    // (in flight until the first tile is there)
+    typename M::Frag q[MAPS][S::QS];
 #pragma unroll
-    for (int c = 0; c < RT; ++c)
-        if (span[c].lo < span[c].hi) ulo = min(ulo, span[c].lo), uhi = max(uhi, span[c].hi), alo = max(alo, span[c].lo), ahi = min(ahi, span[c].hi);
-    ulo = wave_min(ulo), uhi = wave_max(uhi), alo = wave_max(alo), ahi = a.key_mask ? 0 : wave_min(ahi);
-    if (lane == 0 && map == 0) s_lo[group] = ulo, s_hi[group] = uhi;
+    for (int c = 0; c < MAPS; ++c)
+#pragma unroll
+        for (int k = 0; k < S::QS; ++k)
+            q[c][k] = global_frag<T, DMA>(row<T>(a.q, mine ? i : 0, 2 * h + map0 + c), (2 * k + half) * S::EP, a.D, g.aligned);
+    mine = mine && (seq >= 0 || (a.flags & SGL_ATTN_ZERO_REST));
+    Reach reach = reach_of(span);
+    if (a.key_mask) reach.to = 0;
+    if (lane == 0 && (MAPS == 2 || map0 == 0)) s_lo[group] = reach.lo, s_hi[group] = reach.hi;
     if (threadIdx.x == 0) s_bad = 0;
     __syncthreads();
-    int32_t lo = min(s_lo[0], s_lo[1]), hi = max(s_hi[0], s_hi[1]);
+    int32_t lo = s_lo[0], hi = s_hi[0];
+#pragma unroll
+    for (int k = 1; k < S::GROUPS; ++k) lo = min(lo, s_lo[k]), hi = max(hi, s_hi[k]);
     if (w.splits > 1 && lo < hi) {
         const int32_t chunk = (int32_t)ceil_div<int64_t>(ceil_div<int64_t>((int64_t)hi - lo, w.splits), BN) * BN;
         const int64_t from = (int64_t)lo + (int64_t)chunk * split;
         lo = (int32_t)min(from, (int64_t)hi);
         hi = (int32_t)min(from + chunk, (int64_t)hi);
-        uhi = min(uhi, hi), ulo = max(ulo, lo);
-#pragma unroll
-        for (int c = 0; c < RT; ++c) span[c].lo = max(span[c].lo, lo), span[c].hi = min(span[c].hi, hi);
-    }
-
-    typename M::Frag q[RT][S::QS];
-#pragma unroll
-    for (int c = 0; c < RT; ++c) {
-        const bool live = span[c].lo < span[c].hi;
-#pragma unroll
-        for (int k = 0; k < S::QS; ++k)
-            q[c][k] = global_frag<T>(row<T>(a.q, live ? i[c] : 0, 2 * h[c] + map), (2 * k + half) * S::EP, a.D, live, g.aligned, g.negate);
+        reach.hi = min(reach.hi, hi), reach.lo = max(reach.lo, lo);
+        span.lo = max(span.lo, lo), span.hi = min(span.hi, hi);
     }
     const Source ks = halves<T>(a.k, hk, a.D), vs = run<T>(a.v, hk, a.Dv);
     const int32_t last = (int32_t)a.Tk - 1;
-    State<T, DP, RT> st;
+    State<T, DP, MAPS> st;
     st.reset();
+    Stager<T, DP, BN, S::NT, DMA, true> stage_k;
+    Stager<T, DP, BN, S::NT, DMA, false> stage_v;
+    stage_k.plan(ks);
+    stage_v.plan(vs);
+    bool finite = false;        // the pass without what is not finite
     auto load = [&](char* buf, int32_t j) {
-        stage<T, DP, BN, BLOCK, DMA>(buf, ks, true, j, last, g.aligned);
-        stage<T, DP, BN, BLOCK, DMA>(buf + BN * RB, vs, false, j, last, g.aligned);
+        stage_k.load(buf, ks, j, last, g.aligned);
+        if (finite) stage_finite<T, DP, BN, S::NT>(buf + BN * RB, s_marks, vs, false, j, last);
+        else stage_v.load(buf + BN * RB, vs, j, last, g.aligned);
     };
     auto work = [&](const char* buf, int32_t j) {
 #pragma unroll
         for (int sub = 0; sub < BN / 32; ++sub) {
             const int32_t j0 = j + sub * 32;
-            if (j0 >= uhi || j0 + 32 <= ulo) continue;
-            if (HEADS && (((j0 - lo) >> 5) & 1) != group) continue;
-            step<T, DP, RT, false>(st, q, buf, buf + BN * RB, sub, map, j0, j0 >= alo && j0 + 32 <= ahi, span, g, lane);
+            if (j0 >= reach.hi || j0 + 32 <= reach.lo) continue;
+            if (HEADS && (((j0 - lo) >> 5) & (S::GROUPS - 1)) != group) continue;
+            step<T, DP, MAPS>(st, q, buf, buf + BN * RB, sub, map0, j0, j0 >= reach.from && j0 + 32 <= reach.to, span, g, lane);
         }
     };
     if (lo < hi) {
         load(s_a, lo);
-        staged();
-        for (int32_t j = lo; j < hi; j += 2 * BN) {
-            if (j + BN < hi) load(s_b, j + BN);
-            work(s_a, j);
-            staged();
-            if (j + BN >= hi) break;
-            if (j + 2 * BN < hi) load(s_a, j + 2 * BN);
-            work(s_b, j + BN);
-            staged();
+        if (g.negate) {
+#pragma unroll
+            for (int c = 0; c < MAPS; ++c)
+#pragma unroll
+                for (int k = 0; k < S::QS; ++k) q[c][k] = -q[c][k];
         }
-        if (st.spoilt(span)) s_bad = 1;
-        __syncthreads();
-        if (s_bad) {
-            st.reset();
-            for (int32_t j = lo; j < hi; j += BN) {
-                load(s_a, j);
+#pragma unroll 1
+        for (;;) {
+            staged();
+#pragma unroll 1
+            for (int32_t j = lo; j < hi; j += 2 * BN) {
+                if (j + BN < hi) load(s_b, j + BN);
+                work(s_a, j);
                 staged();
-                for (int sub = 0; sub < BN / 32; ++sub) {
-                    const int32_t j0 = j + sub * 32;
-                    if (j0 >= uhi || j0 + 32 <= ulo) continue;
-                    if (HEADS && (((j0 - lo) >> 5) & 1) != group) continue;
-                    step<T, DP, RT, true>(st, q, s_a, s_a + BN * RB, sub, map, j0, false, span, g, lane);
-                }
-                __syncthreads();
+                if (j + BN >= hi) break;
+                if (j + 2 * BN < hi) load(s_a, j + 2 * BN);
+                work(s_b, j + BN);
+                staged();
             }
+            if (finite) break;
+            if (st.spoilt() && span.lo < span.hi) s_bad = 1;
+            __syncthreads();
+            if (!s_bad) break;
+            finite = true;
+            st.reset();
+            load(s_a, lo);
+        }
+        if (finite) {
+            // the queries that see what is not finite get NaN
+#pragma unroll 1
+            for (int32_t j = lo; j < hi; j += BN) {
+                __syncthreads();
+                stage_finite<T, DP, BN, S::NT>(s_a, s_marks, vs, false, j, last);
+                __syncthreads();
+#pragma unroll 1
+                for (int r = 0; r < BN && j + r < hi; ++r) {
+                    if (HEADS && (((j + r - lo) >> 5) & (S::GROUPS - 1)) != group) continue;
+                    if (!marked_any<RB>(s_marks, r, 0, RB / 16)) continue;
+                    if (!sees(j + r, span, a.key_mask)) continue;
+#pragma unroll
+                    for (int c = 0; c < MAPS; ++c) spoil<T, RB, VT>(st.o[c], s_marks, r, half);
+                }
+            }
+            __syncthreads();
         }
     }
 
-    if (g.parts > 1) {
+    if (HEADS || g.parts > 1) {
         // unnormalised results, to be joined with the other parts'
         const int part = HEADS ? split * 2 + group : split;
 #pragma unroll
-        for (int c = 0; c < RT; ++c) {
+        for (int c = 0; c < MAPS; ++c) {
             const float l = half_sum(st.l[c]);
-            if (!mine[c]) continue;
-            const int64_t at = (((int64_t)part * a.Tq + i[c]) * a.Hq + h[c]) * 2 + map;
+            if (!mine) continue;
+            const int64_t at = (((int64_t)part * a.Tq + i) * a.Hq + h) * 2 + map0 + c;
             if (half == 0) g.part_ml[2 * at] = st.m[c], g.part_ml[2 * at + 1] = l;
             if (l == 0.f) continue;
             float* o = g.part_o + at * a.Dv;
 #pragma unroll
-            for (int t = 0; t < S::VT; ++t)
+            for (int t = 0; t < VT; ++t)
 #pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    const int d = t * 32 + 8 * (r / 4) + 4 * half + r % 4;
-                    if (d < a.Dv) o[d] = st.o[c][t][r];
+                for (int r4 = 0; r4 < 4; ++r4) {
+                    const int d = t * 32 + 8 * r4 + 4 * half;
+                    const f32x4 x = {st.o[c][t][4 * r4], st.o[c][t][4 * r4 + 1], st.o[c][t][4 * r4 + 2], st.o[c][t][4 * r4 + 3]};
+                    if (DMA || a.Dv % 4 == 0) {
+                        if (d < a.Dv) *reinterpret_cast<f32x4*>(o + d) = x;
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            if (d + e < a.Dv) o[d + e] = x[e];
+                    }
                 }
         }
         return;
     }
-    // normalise; the second map's waves hand their results over, the first's subtract them
+    if constexpr (!HEADS) {
+        float inv[MAPS];
 #pragma unroll
-    for (int c = 0; c < RT; ++c) {
-        const float l = half_sum(st.l[c]);
-        const bool none = !(span[c].lo < span[c].hi) || l == 0.f;      // no key, or only keys whose score is -inf
-        const float inv = none ? 0.f : 1.f / l;
-        if (a.lse && half == 0 && mine[c]) a.lse[(i[c] * a.Hq + h[c]) * 2 + map] = none ? INFINITY : st.m[c] + __builtin_amdgcn_logf(l);
+        for (int c = 0; c < MAPS; ++c) {
+            const float l = half_sum(st.l[c]);
+            const bool none = !(span.lo < span.hi) || l == 0.f;    // no key, or only keys whose score is -inf
+            inv[c] = none ? 0.f : 1.f / l;
+            if (a.lse && half == 0 && mine) a.lse[(i * a.Hq + h) * 2 + map0 + c] = none ? INFINITY : st.m[c] + __builtin_amdgcn_logf(l);
+            // (what an empty column gathered may be anything: it is not multiplied, it is cleared)
 #pragma unroll
-        for (int t = 0; t < S::VT; ++t)
+            for (int t = 0; t < VT; ++t)
 #pragma unroll
-            for (int r = 0; r < 16; ++r) st.o[c][t][r] = none ? 0.f : st.o[c][t][r] * inv;
-    }
-    struct alignas(4 * sizeof(T)) Four {
-        T e[4];
-    };
-    constexpr int SLOT = 64 * 16 * 4;                                   // a column tile's 32 x 32 results
-    constexpr int AT_ONCE = S::TILE / (2 * SLOT);                       // of them per row group in the first buffer
-#pragma unroll
-    for (int u0 = 0; u0 < RT * S::VT; u0 += AT_ONCE) {
-        __syncthreads();
-        char* box = s_a + group * AT_ONCE * SLOT + lane * 16;
-        if (map == 1) {
-#pragma unroll
-            for (int u = u0; u < u0 + AT_ONCE && u < RT * S::VT; ++u)
-#pragma unroll
-                for (int r4 = 0; r4 < 4; ++r4) {
-                    const f32x16& o = st.o[u / S::VT][u % S::VT];
-                    *reinterpret_cast<f32x4*>(box + (u - u0) * SLOT + r4 * 1024) = f32x4{o[4 * r4], o[4 * r4 + 1], o[4 * r4 + 2], o[4 * r4 + 3]};
-                }
+                for (int r = 0; r < 16; ++r) st.o[c][t][r] = none ? 0.f : st.o[c][t][r] * inv[c];
         }
-        __syncthreads();
+        const float lam = a.lam[h];
+        constexpr int SHARE = S::TILE / (S::WAVES / 2);                     // a wave's part of the two buffers
+        char* own = (wave < S::WAVES / 2 ? s_a : s_b) + wave % (S::WAVES / 2) * SHARE;
+        const uint64_t keep = __ballot(mine);
+        const auto kept = [&](int r) { return (keep >> r) & 1; };
+        if constexpr (MAPS == 2) {
+            if (a.o2.data) store_pieces<T, SHARE / 32, VT, DMA>(st.o[1], 1.f, own, lane, a.Dv, g.aligned, [&](int r) { return row_out<T>(a.o2, i0 + r, h); }, kept);
 #pragma unroll
-        for (int u = u0; u < u0 + AT_ONCE && u < RT * S::VT; ++u) {
-            const int c = u / S::VT, t = u % S::VT;
-            if (!mine[c]) continue;
-            const sgl_rows& to = map ? a.o2 : a.out;
-            if (!to.data) continue;
-            T* dst = row_out<T>(to, i[c], h[c]);
-            const float lam = a.lam[h[c]];
+            for (int t = 0; t < VT; ++t)
 #pragma unroll
-            for (int r4 = 0; r4 < 4; ++r4) {
-                f32x4 o2 = f32x4{0.f, 0.f, 0.f, 0.f};
-                if (map == 0) o2 = *reinterpret_cast<const f32x4*>(box + (u - u0) * SLOT + r4 * 1024);
-                const int d = t * 32 + 8 * r4 + 4 * half;
-                Four y;
+                for (int r = 0; r < 16; ++r) st.o[0][t][r] = __builtin_fmaf(-lam, st.o[1][t][r], st.o[0][t][r]);
+            store_pieces<T, SHARE / 32, VT, DMA>(st.o[0], 1.f, own, lane, a.Dv, g.aligned, [&](int r) { return row_out<T>(a.out, i0 + r, h); }, kept);
+        } else {
+            // the second map's waves hand their results over, the first's subtract them; a 32 x 32 tile takes 4 KB, half the
+            // groups use each buffer
+            constexpr int SLOT = 4096, AT_ONCE = S::TILE / (S::GROUPS / 2 * SLOT);
+            static_assert(AT_ONCE >= 1, "a result of every group fits");
+            char* box = (group < S::GROUPS / 2 ? s_a : s_b) + group % (S::GROUPS / 2) * AT_ONCE * SLOT + lane * 16;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) y.e[e] = (T)(map == 0 ? __builtin_fmaf(-lam, o2[e], st.o[c][t][4 * r4 + e]) : st.o[c][t][4 * r4 + e]);
-                if (g.aligned && d + 4 <= a.Dv) {
-                    *reinterpret_cast<Four*>(dst + d) = y;
-                } else {
+            for (int u0 = 0; u0 < VT; u0 += AT_ONCE) {
+                __syncthreads();
+                if (map0 == 1) {
 #pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        if (d + e < a.Dv) dst[d + e] = y.e[e];
+                    for (int u = u0; u < u0 + AT_ONCE && u < VT; ++u)
+#pragma unroll
+                        for (int r4 = 0; r4 < 4; ++r4) {
+                            const f32x16& o = st.o[0][u];
+                            *reinterpret_cast<f32x4*>(box + (u - u0) * SLOT + r4 * 1024) = f32x4{o[4 * r4], o[4 * r4 + 1], o[4 * r4 + 2], o[4 * r4 + 3]};
+                        }
+                }
+                __syncthreads();
+                if (map0 == 0) {
+#pragma unroll
+                    for (int u = u0; u < u0 + AT_ONCE && u < VT; ++u)
+#pragma unroll
+                        for (int r4 = 0; r4 < 4; ++r4) {
+                            const f32x4 o2 = *reinterpret_cast<const f32x4*>(box + (u - u0) * SLOT + r4 * 1024);
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) st.o[0][u][4 * r4 + e] = __builtin_fmaf(-lam, o2[e], st.o[0][u][4 * r4 + e]);
+                        }
                 }
             }
+            __syncthreads();
+            const sgl_rows& to = map0 ? a.o2 : a.out;
+            if (to.data) store_pieces<T, SHARE / 32, VT, DMA>(st.o[0], 1.f, own, lane, a.Dv, g.aligned, [&](int r) { return row_out<T>(to, i0 + r, h); }, kept);
         }
     }
 }
 
-// joins the parts of a (row, head): one wave each, values dealt to its lanes
+// Joins the parts of a (row, head), a block each: the weights of the parts first, then 8 groups of 32 lanes add up every eighth
+// part and are themselves added in order.
 template <typename T>
 __global__ __launch_bounds__(BLOCK) void join_kernel(AttnArgs g) {
+    constexpr int MOST = 2 * 64;
+    __shared__ float s_f[2][MOST], s_lse[2];
+    __shared__ __align__(16) float s_o[2][8][256];
     const sgl_diff_attn_args& a = g.a;
-    const int lane = threadIdx.x & 63;
-    const int64_t n = a.Tq * a.Hq, at = (int64_t)blockIdx.x * (BLOCK / 64) + (threadIdx.x >> 6);
-    if (at >= n) return;
+    const int64_t n = a.Tq * a.Hq, at = blockIdx.x;
     const int64_t i = at / a.Hq;
-    const int h = (int)(at % a.Hq);
+    const int h = (int)(at - i * a.Hq), wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
     const int32_t B = (int32_t)live_count(a.B_dev, a.B);
     const int32_t seq = a.q_ptr ? find_seq(a.q_ptr, B, i) : (i < B ? (int32_t)i : -1);
     if (seq < 0 && !(a.flags & SGL_ATTN_ZERO_REST)) return;
-    float o[2][4] = {}, lse[2];
+    if (wave < 2) {
+        // the parts' maxima and sums of map `wave`: two a lane
+        float m[2], l[2], top = NEG_INF, sum = 0.f;
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            const int p = lane + 64 * u;
+            const float* ml = g.part_ml + 2 * (((int64_t)p * n + at) * 2 + wave);
+            m[u] = p < g.parts ? ml[0] : NEG_INF;
+            l[u] = p < g.parts ? ml[1] : 0.f;
+            if (l[u] != 0.f) top = fmaxf(top, m[u]);
+        }
+#pragma unroll
+        for (int k = 1; k < 64; k <<= 1) top = fmaxf(top, __shfl_xor(top, k));
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            const float f = l[u] == 0.f ? 0.f : m[u] == top ? 1.f : exp2_hw(m[u] - top);
+            s_f[wave][lane + 64 * u] = f;
+            sum += l[u] == 0.f ? 0.f : l[u] * f;
+        }
+#pragma unroll
+        for (int k = 1; k < 64; k <<= 1) sum += __shfl_xor(sum, k);
+        const float inv = sum == 0.f ? 0.f : 1.f / sum;
+#pragma unroll
+        for (int u = 0; u < 2; ++u) s_f[wave][lane + 64 * u] *= inv;
+        if (lane == 0) {
+            s_lse[wave] = sum == 0.f ? INFINITY : top + __builtin_amdgcn_logf(sum);
+            if (a.lse) a.lse[at * 2 + wave] = s_lse[wave];
+        }
+    }
+    __syncthreads();
+    const int group = threadIdx.x >> 5, l32 = threadIdx.x & 31;
+    const bool vec = a.Dv % 4 == 0;
 #pragma unroll
     for (int m = 0; m < 2; ++m) {
-        float top = NEG_INF, sum = 0.f;
-        bool nan = false;
-        for (int p = lane; p < g.parts; p += 64) {
-            const float* ml = g.part_ml + 2 * (((int64_t)p * n + at) * 2 + m);
-            if (ml[1] != 0.f) top = fmaxf(top, ml[0]);
-            nan = nan || ml[1] != ml[1];
-        }
-        for (int k = 1; k < 64; k <<= 1) top = fmaxf(top, __shfl_xor(top, k));
-        for (int p = 0; p < g.parts; ++p) {
-            const int64_t k = ((int64_t)p * n + at) * 2 + m;
-            const float pm = g.part_ml[2 * k], pl = g.part_ml[2 * k + 1];
-            if (pl == 0.f) continue;                // (a part without keys wrote no result)
-            const float f = pm == top ? 1.f : exp2_hw(pm - top);
-            sum = __builtin_fmaf(pl, f, sum);
-            const float* src = g.part_o + k * a.Dv;
+        f32x4 acc[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+        for (int p = group; p < g.parts; p += 8) {
+            const float f = s_f[m][p];
+            if (f == 0.f) continue;                     // (a part without keys wrote no result)
+            const float* src = g.part_o + (((int64_t)p * n + at) * 2 + m) * a.Dv;
 #pragma unroll
-            for (int u = 0; u < 4; ++u)
-                if (lane + 64 * u < a.Dv) o[m][u] = __builtin_fmaf(src[lane + 64 * u], f, o[m][u]);
-        }
-        const bool none = sum == 0.f;
-        lse[m] = none ? INFINITY : top + __builtin_amdgcn_logf(sum);
+            for (int u = 0; u < 2; ++u) {
+                const int d = 4 * l32 + 128 * u;
+                f32x4 x = {0.f, 0.f, 0.f, 0.f};
+                if (vec) {
+                    if (d < a.Dv) x = *reinterpret_cast<const f32x4*>(src + d);
+                } else {
 #pragma unroll
-        for (int u = 0; u < 4; ++u) o[m][u] = none ? 0.f : o[m][u] / sum;
+                    for (int e = 0; e < 4; ++e)
+                        if (d + e < a.Dv) x[e] = src[d + e];
+                }
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc[u][e] = __builtin_fmaf(x[e], f, acc[u][e]);
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < 2; ++u) *reinterpret_cast<f32x4*>(&s_o[m][group][4 * l32 + 128 * u]) = acc[u];
     }
-    if (a.lse && lane < 2) a.lse[at * 2 + lane] = lse[lane];
-    const float lam = a.lam[h];
-    T* out = row_out<T>(a.out, i, h);
-    T* out2 = a.o2.data ? row_out<T>(a.o2, i, h) : nullptr;
+    __syncthreads();
+    const int d = threadIdx.x;
+    if (d >= a.Dv) return;
+    float o[2] = {0.f, 0.f};
 #pragma unroll
-    for (int u = 0; u < 4; ++u)
-        if (lane + 64 * u < a.Dv) {
-            out[lane + 64 * u] = (T)__builtin_fmaf(-lam, o[1][u], o[0][u]);
-            if (out2) out2[lane + 64 * u] = (T)o[1][u];
-        }
+    for (int m = 0; m < 2; ++m)
+#pragma unroll
+        for (int k = 0; k < 8; ++k) o[m] += s_o[m][k][d];
+    row_out<T>(a.out, i, h)[d] = (T)__builtin_fmaf(-a.lam[h], o[1], o[0]);
+    if (a.o2.data) row_out<T>(a.o2, i, h)[d] = (T)o[1];
 }
 
 template <typename T, int DP>
 void launch(const AttnArgs& g, hipStream_t st) {
     const FwdWork w = forward_work(g.a);
-    const dim3 grid((unsigned)(ceil_div<int64_t>(w.items, 8) * 8)), block(BLOCK);
-    const bool dma = g.aligned && g.a.D == DP && g.a.Dv == 2 * DP;
+    const dim3 grid((unsigned)(ceil_div<int64_t>(w.items, 8) * 8));
+    constexpr int ROW_NT = Shape<T, DP, false>::NT, HEAD_NT = Shape<T, DP, true>::NT;
+    const bool dma = g.aligned && g.a.D == DP && g.a.Dv == 2 * DP && dma_rows(g.a.k) && dma_rows(g.a.v);
     if (g.a.q_ptr) {
-        if (dma) hipLaunchKernelGGL((fwd_kernel<T, DP, false, true>), grid, block, 0, st, g, w);
-        else hipLaunchKernelGGL((fwd_kernel<T, DP, false, false>), grid, block, 0, st, g, w);
+        if (dma) hipLaunchKernelGGL((fwd_kernel<T, DP, false, true>), grid, dim3(ROW_NT), 0, st, g, w);
+        else hipLaunchKernelGGL((fwd_kernel<T, DP, false, false>), grid, dim3(ROW_NT), 0, st, g, w);
     } else {
-        if (dma) hipLaunchKernelGGL((fwd_kernel<T, DP, true, true>), grid, block, 0, st, g, w);
-        else hipLaunchKernelGGL((fwd_kernel<T, DP, true, false>), grid, block, 0, st, g, w);
+        if (dma) hipLaunchKernelGGL((fwd_kernel<T, DP, true, true>), grid, dim3(HEAD_NT), 0, st, g, w);
+        else hipLaunchKernelGGL((fwd_kernel<T, DP, true, false>), grid, dim3(HEAD_NT), 0, st, g, w);
     }
     if (g.parts > 1)
-        hipLaunchKernelGGL(join_kernel<T>, dim3((unsigned)ceil_div<int64_t>(g.a.Tq * g.a.Hq, BLOCK / 64)), block, 0, st, g);
+        hipLaunchKernelGGL(join_kernel<T>, dim3((unsigned)(g.a.Tq * g.a.Hq)), dim3(BLOCK), 0, st, g);
 }
 
 }  // namespace

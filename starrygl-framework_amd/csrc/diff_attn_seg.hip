@@ -24,7 +24,8 @@ __device__ __forceinline__ float lanes_sum(float x) {
 // EP values of a row as floats; zeros beyond len
 template <typename T>
 __device__ __forceinline__ void load_part(float (&f)[Mat<T>::EP], const T* src, int e, int len, bool live, int aligned) {
-    const typename Mat<T>::Frag x = global_frag<T>(src, e, len, live, aligned, false);
+    typename Mat<T>::Frag x = {};
+    if (live) x = global_frag<T, false>(src, e, len, aligned);
 #pragma unroll
     for (int j = 0; j < Mat<T>::EP; ++j) f[j] = (float)x[j];
 }
