@@ -457,56 +457,52 @@ __device__ __forceinline__ f32x16 zero16() {
     return z;
 }
 
-// 32 rows of results, one a lane of either half (the layout of the products), to memory through the wave's own piece of LDS
-// (32 rows of RB bytes): a row's elements lie in 2 x 16 registers of two lanes, eight bytes here and there; from LDS they go
-// out as whole 16-byte chunks side by side.  x[t]: 32 elements from 32 t; row r of them goes to dst(r) where keep(r) holds.
-template <typename T, int RB, int N, bool WHOLE, typename Dst, typename Keep>
-__device__ __forceinline__ void store_rows(const f32x16 (&x)[N], float scale, char* box, int lane, int len, int aligned, Dst dst, Keep keep) {
-    constexpr int BYTES = N * 32 * (int)sizeof(T), CH = BYTES / 16, EP = 16 / (int)sizeof(T);
-    static_assert(BYTES <= RB, "a row fits");
+// 32 rows of results, one a lane of either half (the layout of the products), to memory through the wave's own piece of LDS (32
+// rows of PIECE bytes): a row's elements lie in registers of two lanes, eight bytes here and there; from LDS they go out as
+// whole 16-byte chunks side by side.  val(t, r): register r of the 32 elements from 32 t; row k goes to base + k * stride
+// where bit k of `keep` is set.  The order is fixed, a few values at a time: a spilled register here would be read back behind the stores (loads
+// and stores return through one counter), which cost 28000 cycles a block.
+template <typename T, int PIECE, int N, bool WHOLE, typename Val>
+__device__ __forceinline__ void store_rows(Val val, char* box, int lane, int len, int aligned, T* base, int64_t stride, uint32_t keep) {
+    constexpr int FIT = PIECE / (32 * (int)sizeof(T)), AT = FIT >= N ? N : FIT >= 2 ? 2 : 1;           // 32-wide pieces at a time
+    static_assert(FIT >= 1, "one piece fits");
+    constexpr int BYTES = AT * 32 * (int)sizeof(T), CH = BYTES / 16, EP = 16 / (int)sizeof(T);
     struct alignas(4 * sizeof(T)) Four {
         T e[4];
     };
-    const int half = lane >> 5, col = lane & 31;
+    const int half = lane >> 5, col = lane & 31, c = lane % CH;
 #pragma unroll
-    for (int t = 0; t < N; ++t)
+    for (int t0 = 0; t0 < N; t0 += AT) {
 #pragma unroll
-        for (int r4 = 0; r4 < 4; ++r4) {
-            Four y;
+        for (int u = 0; u < AT; ++u) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) y.e[e] = (T)(x[t][4 * r4 + e] * scale);
-            const int b = (t * 32 + 8 * r4 + 4 * half) * (int)sizeof(T);
-            *reinterpret_cast<Four*>(box + col * BYTES + ((((b >> 4) ^ col) & (CH - 1)) << 4) + (b & 15)) = y;
+            for (int r4 = 0; r4 < 4; ++r4) {
+                Four y;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) y.e[e] = (T)val(t0 + u, 4 * r4 + e);
+                const int b = (u * 32 + 8 * r4 + 4 * half) * (int)sizeof(T);
+                *reinterpret_cast<Four*>(box + col * BYTES + ((((b >> 4) ^ col) & (CH - 1)) << 4) + (b & 15)) = y;
+            }
+            __builtin_amdgcn_sched_barrier(0);
         }
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        T* to = base + (lane / CH) * stride + t0 * 32 + c * EP;
+        const int left = len - t0 * 32 - c * EP;
 #pragma unroll
-    for (int i = 0; i < 32 * CH / 64; ++i) {
-        const int r = i * (64 / CH) + lane / CH, c = lane % CH;
-        const typename Mat<T>::Frag f = *reinterpret_cast<const typename Mat<T>::Frag*>(box + r * BYTES + (((c ^ r) & (CH - 1)) << 4));
-        if (!keep(r)) continue;
-        T* to = dst(r) + c * EP;
-        if (WHOLE || (aligned && (c + 1) * EP <= len)) {
-            *reinterpret_cast<typename Mat<T>::Frag*>(to) = f;
-        } else {
+        for (int i = 0; i < 32 * CH / 64; ++i) {
+            const int r = i * (64 / CH) + lane / CH;
+            const typename Mat<T>::Frag f = *reinterpret_cast<const typename Mat<T>::Frag*>(box + r * BYTES + (((c ^ r) & (CH - 1)) << 4));
+            if ((keep >> r) & 1) {
+                if (WHOLE || (aligned && left >= EP)) {
+                    *reinterpret_cast<typename Mat<T>::Frag*>(to) = f;
+                } else {
 #pragma unroll
-            for (int e = 0; e < EP; ++e)
-                if (c * EP + e < len) to[e] = f[e];
+                    for (int e = 0; e < EP; ++e)
+                        if (e < left) to[e] = f[e];
+                }
+            }
+            to += (64 / CH) * stride;
+            __builtin_amdgcn_sched_barrier(0);
         }
-    }
-}
-
-// store_rows of as many 32-element pieces at a time as PIECE bytes a row hold
-template <typename T, int PIECE, int N, bool WHOLE, typename Dst, typename Keep>
-__device__ __forceinline__ void store_pieces(const f32x16 (&x)[N], float scale, char* box, int lane, int len, int aligned, Dst dst, Keep keep) {
-    constexpr int FIT = PIECE / (32 * (int)sizeof(T)), AT = FIT >= N ? N : FIT >= 2 ? 2 : 1;
-    static_assert(FIT >= 1, "one piece fits");
-#pragma unroll
-    for (int t = 0; t < N; t += AT) {
-        f32x16 part[AT];
-#pragma unroll
-        for (int u = 0; u < AT; ++u) part[u] = x[t + u];
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-        store_rows<T, AT * 32 * (int)sizeof(T), AT, WHOLE>(part, scale, box, lane, len - t * 32, aligned, [&](int r) { return dst(r) + t * 32; }, keep);
     }
 }
 

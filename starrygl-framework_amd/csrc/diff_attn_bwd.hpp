@@ -25,7 +25,7 @@ struct Shape {
     // key side: a wave per 32 keys; from 512-byte rows on two waves share the keys, one sums dK, the other dV (each computes the
     // scores: 5/4 of the products, but the sums of one wave do not fit the registers of two a SIMD)
     static constexpr bool ROLES = RB >= 256;
-    static constexpr int K_WAVES = RB > 512 ? 2 : RB > 256 ? 8 : 4, K_ROWS = (ROLES ? K_WAVES / 2 : K_WAVES) * 32, K_OCC = RB > 512 ? 1 : 2;
+    static constexpr int K_WAVES = RB > 512 ? 2 : 4, K_ROWS = (ROLES ? K_WAVES / 2 : K_WAVES) * 32, K_OCC = RB > 512 ? 1 : 2;
     // the owned keys and values: fragments in registers, or read from a tile of their own in LDS
     static constexpr bool KEY_REGS = RB <= 128, VAL_REGS = RB <= 512;
     static constexpr int OWN = (KEY_REGS ? 0 : RB) + (VAL_REGS ? 0 : RB);       // bytes of an owned row in LDS
@@ -68,14 +68,6 @@ __device__ __forceinline__ void add_map(f32x16 (&acc)[N], const char* tile, int 
         if (map) add_product<T, RB, N, AHEAD>(acc, tile, row0, N, x, lane);
         else add_product<T, RB, N, AHEAD>(acc, tile, row0, 0, x, lane);
     }
-}
-
-template <int N>
-__device__ __forceinline__ void make_nan(f32x16 (&acc)[N]) {
-#pragma unroll
-    for (int t = 0; t < N; ++t)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) acc[t][r] = NAN;
 }
 
 // ---------------------------------------------------------------------------------------------- owned: query rows
@@ -199,6 +191,7 @@ __global__ __launch_bounds__((Shape<T, DP>::Q_WAVES * 64), (Shape<T, DP>::Q_OCC)
             add_map<T, RB, S::DT, AHEAD>(dq, buf, sub * 32, map, s, lane);
         }
     };
+    bool spoilt = false;        // the query sees something not finite: NaN
     if (lo < hi) {
 #pragma unroll 1
         for (;;) {
@@ -223,7 +216,6 @@ __global__ __launch_bounds__((Shape<T, DP>::Q_WAVES * 64), (Shape<T, DP>::Q_OCC)
         }
         if (finite) {
             // the queries that see what is not finite get NaN
-            bool spoilt = false;
 #pragma unroll 1
             for (int32_t j = lo; j < hi; j += BN) {
                 __syncthreads();
@@ -236,7 +228,7 @@ __global__ __launch_bounds__((Shape<T, DP>::Q_WAVES * 64), (Shape<T, DP>::Q_OCC)
                     spoilt = spoilt || marked_any<RB>(s_marks + BN * (RB / 16), r, 0, RB / 16) || marked_any<RB>(s_marks, r, map * (RB / 32), (map + 1) * (RB / 32));
                 }
             }
-            if (spoilt) make_nan(dq), sum = NAN;
+            if (spoilt) sum = NAN;
         }
     }
     float share = live ? sum : 0.f;
@@ -249,14 +241,13 @@ __global__ __launch_bounds__((Shape<T, DP>::Q_WAVES * 64), (Shape<T, DP>::Q_OCC)
         for (int w = 0; w < GROUPS; ++w) x += s_lam[w];
         g.lam_part[(int64_t)tile * a.Hq + h] = x;
     }
-    if (!live) clear();
-    const uint64_t keep = __ballot(i < a.Tq && (seq >= 0 || (a.flags & SGL_ATTN_ZERO_REST)));
+    const uint32_t keep = (uint32_t)__ballot(i < a.Tq && (seq >= 0 || (a.flags & SGL_ATTN_ZERO_REST)));
+    const float scale = map ? -lam * g.scale : g.scale;
     // (every wave's last look at the tiles lies before the barrier above)
-    store_rows<T, RB / 2, S::DT, DMA>(dq, map ? -lam * g.scale : g.scale, (wave < S::Q_WAVES / 2 ? s_a : s_b) + wave % (S::Q_WAVES / 2) * 16 * RB, lane, a.D, g.aligned,
-                             [&](int r) { return row_out<T>(a.d_q, i0 + r, 2 * h + map); }, [&](int r) { return (keep >> r) & 1; });
+    store_rows<T, RB / 2, S::DT, DMA>([&](int t, int r) { return spoilt ? NAN : live ? dq[t][r] * scale : 0.f; }, (wave < S::Q_WAVES / 2 ? s_a : s_b) + wave % (S::Q_WAVES / 2) * 16 * RB, lane, a.D,
+                                      g.aligned, row_out<T>(a.d_q, i0, 2 * h + map), a.d_q.row_stride, keep);
 }
 
-// ----------------------------------------------------------------------------------------------------- owned: keys
 // LDS of a block
 template <typename T, int DP>
 struct KvSmem {
@@ -269,7 +260,7 @@ template <typename T, int DP, bool DMA, bool DK, bool DV>
 __device__ __forceinline__ void kv_body(const AttnArgs& g, int32_t tiles, char* s_a, char* s_b, char* s_own, uint8_t* s_marks, int* s_lo, int* s_hi, int& s_bad) {
     typedef Shape<T, DP> S;
     typedef Mat<T> M;
-    constexpr int RB = S::RB, NT = S::K_WAVES * 64, ROWS = S::K_ROWS, GROUPS = ROWS / 32, BQ = KvSmem<T, DP>::BQ, TILE = KvSmem<T, DP>::TILE, AHEAD = RB <= 256 ? 4 : 2;
+    constexpr int RB = S::RB, NT = S::K_WAVES * 64, ROWS = S::K_ROWS, GROUPS = ROWS / 32, BQ = KvSmem<T, DP>::BQ, TILE = KvSmem<T, DP>::TILE, AHEAD = 2;
     const sgl_diff_attn_args& a = g.a;
     const int G = a.Hq / a.Hk;
     const uint32_t n = (uint32_t)tiles * (uint32_t)a.Hk, item = xcd_item(n);
@@ -425,6 +416,7 @@ __device__ __forceinline__ void kv_body(const AttnArgs& g, int32_t tiles, char* 
             add_map<T, RB, S::DT, AHEAD>(dk[1], buf, 0, 1, s[1], lane);
         }
     };
+    bool spoilt[2] = {false, false};        // a row with something not finite sees the key: NaN
     if (steps > 0) {
         int h, hn;                          // head and first row of the tile at work, and of the one being loaded
         int32_t i0, in;
@@ -474,7 +466,6 @@ __device__ __forceinline__ void kv_body(const AttnArgs& g, int32_t tiles, char* 
         }
         if (finite) {
             // the keys that a row with something not finite sees get NaN
-            bool spoilt[2] = {false, false};
             hn = hk * G, in = lo;
 #pragma unroll 1
             for (int32_t s = 0; s < steps; ++s) {
@@ -496,20 +487,20 @@ __device__ __forceinline__ void kv_body(const AttnArgs& g, int32_t tiles, char* 
                 next();
             }
             __syncthreads();
-            if (spoilt[0]) make_nan(dk[0]);
-            if (spoilt[1]) make_nan(dk[1]);
         }
     }
-    if (!shown) clear();
-    const uint64_t keep = __ballot(j < a.Tk && (seq >= 0 || (a.flags & SGL_ATTN_ZERO_REST)));
-    const auto kept = [&](int r) { return (keep >> r) & 1; };
-    // the walked side's tiles are free (the last barrier is behind every wave's last look at them): a wave has
-    // TILE / waves of them, dK goes out half by half, dV 32 or 64 values at a time
+    const uint32_t keep = (uint32_t)__ballot(j < a.Tk && (seq >= 0 || (a.flags & SGL_ATTN_ZERO_REST)));
+    // the walked side's tiles are free: the last barrier is behind every wave's last look at them
     char* box = s_a + wave * (TILE / S::K_WAVES);
     constexpr int PIECE = TILE / S::K_WAVES / 32;               // bytes of a row at a time
-    if constexpr (DK) store_pieces<T, PIECE, S::DT, DMA>(dk[0], g.scale, box, lane, a.D, g.aligned, [&](int r) { return row_out<T>(a.d_k, j0 + r, 2 * hk); }, kept);
-    if constexpr (DK) store_pieces<T, PIECE, S::DT, DMA>(dk[1], g.scale, box, lane, a.D, g.aligned, [&](int r) { return row_out<T>(a.d_k, j0 + r, 2 * hk + 1); }, kept);
-    if constexpr (DV) store_pieces<T, PIECE, S::VT, DMA>(dv, 1.f, box, lane, a.Dv, g.aligned, [&](int r) { return row_out<T>(a.d_v, j0 + r, hk); }, kept);
+    if constexpr (DK) {
+        store_rows<T, PIECE, S::DT, DMA>([&](int t, int r) { return spoilt[0] ? NAN : shown ? dk[0][t][r] * g.scale : 0.f; }, box, lane, a.D, g.aligned,
+                                         row_out<T>(a.d_k, j0, 2 * hk), a.d_k.row_stride, keep);
+        store_rows<T, PIECE, S::DT, DMA>([&](int t, int r) { return spoilt[1] ? NAN : shown ? dk[1][t][r] * g.scale : 0.f; }, box, lane, a.D, g.aligned,
+                                         row_out<T>(a.d_k, j0, 2 * hk + 1), a.d_k.row_stride, keep);
+    }
+    if constexpr (DV)
+        store_rows<T, PIECE, S::VT, DMA>([&](int t, int r) { return shown ? dv[t][r] : 0.f; }, box, lane, a.Dv, g.aligned, row_out<T>(a.d_v, j0, hk), a.d_v.row_stride, keep);
 }
 
 template <typename T, int DP, bool DMA>

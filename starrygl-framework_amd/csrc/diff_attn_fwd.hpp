@@ -309,32 +309,28 @@ __global__ __launch_bounds__((Shape<T, DP, HEADS>::NT), 2) void fwd_kernel(AttnA
         return;
     }
     if constexpr (!HEADS) {
-        float inv[MAPS];
+        float inv[MAPS];        // 0: no key, or only keys whose score is -inf (what such a column gathered may be anything)
 #pragma unroll
         for (int c = 0; c < MAPS; ++c) {
             const float l = half_sum(st.l[c]);
-            const bool none = !(span.lo < span.hi) || l == 0.f;    // no key, or only keys whose score is -inf
+            const bool none = !(span.lo < span.hi) || l == 0.f;
             inv[c] = none ? 0.f : 1.f / l;
             if (a.lse && half == 0 && mine) a.lse[(i * a.Hq + h) * 2 + map0 + c] = none ? INFINITY : st.m[c] + __builtin_amdgcn_logf(l);
-            // (what an empty column gathered may be anything: it is not multiplied, it is cleared)
-#pragma unroll
-            for (int t = 0; t < VT; ++t)
-#pragma unroll
-                for (int r = 0; r < 16; ++r) st.o[c][t][r] = none ? 0.f : st.o[c][t][r] * inv[c];
         }
         const float lam = a.lam[h];
         constexpr int SHARE = S::TILE / (S::WAVES / 2);                     // a wave's part of the two buffers
         char* own = (wave < S::WAVES / 2 ? s_a : s_b) + wave % (S::WAVES / 2) * SHARE;
-        const uint64_t keep = __ballot(mine);
-        const auto kept = [&](int r) { return (keep >> r) & 1; };
+        const uint32_t keep = (uint32_t)__ballot(mine);
         if constexpr (MAPS == 2) {
-            if (a.o2.data) store_pieces<T, SHARE / 32, VT, DMA>(st.o[1], 1.f, own, lane, a.Dv, g.aligned, [&](int r) { return row_out<T>(a.o2, i0 + r, h); }, kept);
+            const auto second = [&](int t, int r) { return inv[1] == 0.f ? 0.f : st.o[1][t][r] * inv[1]; };
+            store_rows<T, SHARE / 32, VT, DMA>([&](int t, int r) { return __builtin_fmaf(-lam, second(t, r), inv[0] == 0.f ? 0.f : st.o[0][t][r] * inv[0]); }, own, lane, a.Dv,
+                                               g.aligned, row_out<T>(a.out, i0, h), a.out.row_stride, keep);
+            if (a.o2.data) store_rows<T, SHARE / 32, VT, DMA>(second, own, lane, a.Dv, g.aligned, row_out<T>(a.o2, i0, h), a.o2.row_stride, keep);
+        } else {
 #pragma unroll
             for (int t = 0; t < VT; ++t)
 #pragma unroll
-                for (int r = 0; r < 16; ++r) st.o[0][t][r] = __builtin_fmaf(-lam, st.o[1][t][r], st.o[0][t][r]);
-            store_pieces<T, SHARE / 32, VT, DMA>(st.o[0], 1.f, own, lane, a.Dv, g.aligned, [&](int r) { return row_out<T>(a.out, i0 + r, h); }, kept);
-        } else {
+                for (int r = 0; r < 16; ++r) st.o[0][t][r] = inv[0] == 0.f ? 0.f : st.o[0][t][r] * inv[0];
             // the second map's waves hand their results over, the first's subtract them; a 32 x 32 tile takes 4 KB, half the
             // groups use each buffer
             constexpr int SLOT = 4096, AT_ONCE = S::TILE / (S::GROUPS / 2 * SLOT);
@@ -366,7 +362,8 @@ __global__ __launch_bounds__((Shape<T, DP, HEADS>::NT), 2) void fwd_kernel(AttnA
             }
             __syncthreads();
             const sgl_rows& to = map0 ? a.o2 : a.out;
-            if (to.data) store_pieces<T, SHARE / 32, VT, DMA>(st.o[0], 1.f, own, lane, a.Dv, g.aligned, [&](int r) { return row_out<T>(to, i0 + r, h); }, kept);
+            if (to.data)
+                store_rows<T, SHARE / 32, VT, DMA>([&](int t, int r) { return st.o[0][t][r]; }, own, lane, a.Dv, g.aligned, row_out<T>(to, i0, h), to.row_stride, keep);
         }
     }
 }
