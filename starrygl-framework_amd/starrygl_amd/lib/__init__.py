@@ -27,6 +27,27 @@ def load():
     return _lib
 
 
+_torch_ops = None
+
+
+def torch_ops():
+    """-> the compiled autograd side of the attention-layer operators (csrc/torch_ops.cpp), driving `load()`'s library."""
+    global _torch_ops
+    if _torch_ops is None:
+        lib = load()
+        try:
+            from . import sgl_torch
+        except ImportError as e:
+            raise ImportError(f"sgl_torch.so is missing or does not load ({e}): build it with `make -C starrygl-framework_amd/csrc` "
+                              "(or __graft_entry__.build())") from e
+        names = ("last_error_string", "rotary", "qk_norm_rotary", "qk_norm_rotary_backward_workspace_bytes",
+                 "qk_norm_rotary_backward", "diff_attn_workspace_bytes", "diff_attn", "diff_attn_backward_workspace_bytes",
+                 "diff_attn_backward")
+        sgl_torch.init([C.cast(getattr(lib, n), C.c_void_p).value for n in names])
+        _torch_ops = sgl_torch
+    return _torch_ops
+
+
 _hot = {}
 
 

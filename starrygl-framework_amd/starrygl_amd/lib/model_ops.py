@@ -83,6 +83,12 @@ class ModelOps:
         return RotaryParams(code, dim, rot, int(bool(interleaved)), int(bool(inverse)), 0, float(amplitude),
                             freq.data_ptr() if rot else None)
 
+    def check_rotary(self, x, pos, freq):
+        self._rows_check("x", x)
+        code = dtype_code(x, "x")
+        self._vec_check("pos", pos, "i64", (x.shape[0],))
+        return self._rotary_params(code, x.shape[2], freq, False, 1.0)
+
     def rotary(self, x, pos, freq, out=None, interleaved=False, amplitude=1.0, inverse=False, N_dev=None):
         """x [N, H, D] rotated by pos [N] (int64) times freq [R/2] (float64) -> out (default: a new tensor; x itself
         rotates in place).  Rows from N_dev[0] on are not written."""
@@ -134,6 +140,21 @@ class ModelOps:
             else:
                 self._written("y", s["y"])
         return arr
+
+    def check_qk_norm_rotary(self, xs, pos, weights, freq):
+        for x, n, w in zip(xs, pos, weights):
+            self._rows_check("x", x, xs[0].dtype)
+            if freq is not None:
+                self.check_rotary(x, n, freq)
+            if x.shape[2] != xs[0].shape[2]:
+                raise ValueError("queries and keys must have the same head size and type")
+            if w is not None:
+                if not w.is_floating_point():
+                    raise TypeError(f"weight must be a floating type, got {w.dtype}")
+                if tuple(w.shape) not in (tuple(x.shape[2:]), tuple(x.shape[1:])) or w.device != x.device:
+                    raise ValueError(f"weight must have the shape {tuple(x.shape[2:])} or {tuple(x.shape[1:])} and live on "
+                                     f"{x.device}, got {tuple(w.shape)} on {w.device}")
+        dtype_code(xs[0], "x")
 
     def qk_norm_rotary(self, sides, freq, eps=1e-6, interleaved=False, amplitude=1.0):
         """One launch over one or two sides (dicts with x, y, pos, weight, optionally N_dev): y = rotate(x * r * w)."""
@@ -190,6 +211,9 @@ class ModelOps:
         a.q, a.k, a.v = _rows(q), _rows(k), _rows(v)
         a.flags = _abi.ATTN_ZERO_REST if zero_rest else 0
         return a
+
+    def check_diff_attn(self, q, k, v, lam, k_ptr, q_ptr, scale, causal, window, key_mask):
+        self._attn_args(q, k, v, lam, k_ptr, q_ptr, scale, causal, window, key_mask, None, True)
 
     def diff_attn(self, q, k, v, lam, k_ptr, q_ptr=None, scale=None, causal=False, window=None, key_mask=None, B_dev=None,
                   zero_rest=False, out=None, lse=None, o2=None):

@@ -4,9 +4,8 @@ import math
 
 import torch
 import torch.nn as nn
-from torch.autograd.function import once_differentiable
 
-from ...lib import hot_path
+from ...lib import hot_path, torch_ops
 
 
 def rotary_frequencies(rot_dim, base=10000.0, scaling=None):
@@ -53,71 +52,17 @@ def _on_hip(t, what):
         raise RuntimeError(f"{what} runs on a HIP device: move its inputs to the GPU first")
 
 
-class _Rotary(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, pos, freq, interleaved, amplitude):
-        ctx.save_for_backward(pos, freq)
-        ctx.how = (interleaved, amplitude)
-        return hot_path(x.device).rotary(x, pos, freq, interleaved=interleaved, amplitude=amplitude)
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, grad):
-        pos, freq = ctx.saved_tensors
-        interleaved, amplitude = ctx.how
-        g = hot_path(grad.device).rotary(_inner(grad), pos, freq, interleaved=interleaved, amplitude=amplitude, inverse=True)
-        return g, None, None, None, None
-
-
 def rotary_encode(x, pos, freq, *, interleaved=False, amplitude=1.0):
     """x [N, H, D] (float32, bfloat16, float16) with the first R = 2 len(freq) values of every head rotated by the angles
     pos[n] * freq[i]: pair i is (i, i + R/2), or (2i, 2i + 1) when interleaved; the pair is also scaled by `amplitude`.
     pos [N] int64, freq float64 (`rotary_frequencies`).  Differentiable in x."""
     _on_hip(x, "rotary_encode")
-    x, pos = _inner(x), pos.contiguous()
-    if x.requires_grad and torch.is_grad_enabled():
-        return _Rotary.apply(x, pos, freq, bool(interleaved), float(amplitude))
-    return hot_path(x.device).rotary(x, pos, freq, interleaved=interleaved, amplitude=amplitude)
-
-
-class _QKNorm(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, q, k, pos_q, pos_k, wq, wk, freq, eps, interleaved, amplitude):
-        ctx.save_for_backward(q, k, pos_q, pos_k, wq, wk, freq)
-        ctx.how = (eps, interleaved, amplitude)
-        return _norm_forward(q, k, pos_q, pos_k, wq, wk, freq, eps, interleaved, amplitude)
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, gq, gk):
-        q, k, pos_q, pos_k, wq, wk, freq = ctx.saved_tensors
-        need = ctx.needs_input_grad
-        sides, got = [], [None] * 10
-        for i, (x, pos, w, g) in enumerate(((q, pos_q, wq, gq), (k, pos_k, wk, gk))):
-            want_w = w is not None and need[4 + i]
-            if not (need[i] or want_w):
-                continue
-            w32 = None if w is None else w.float().contiguous()
-            dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-            dw = torch.empty(w.shape, dtype=torch.float32, device=x.device) if want_w else None
-            sides.append(dict(x=x, y=_inner(g), dx=dx, pos=pos, weight=w32, dweight=dw))
-            got[i] = dx if need[i] else None
-            got[4 + i] = dw
-        eps, interleaved, amplitude = ctx.how
-        if sides:
-            hot_path(q.device).qk_norm_rotary_backward(sides, freq, eps, interleaved, amplitude)
-        for i, w in ((4, wq), (5, wk)):
-            if got[i] is not None and got[i].dtype != w.dtype:
-                got[i] = got[i].to(w.dtype)
-        return tuple(got)
-
-
-def _norm_forward(q, k, pos_q, pos_k, wq, wk, freq, eps, interleaved, amplitude):
-    f32 = lambda w: None if w is None else w.float().contiguous()  # noqa: E731
-    yq, yk = torch.empty(q.shape, dtype=q.dtype, device=q.device), torch.empty(k.shape, dtype=k.dtype, device=k.device)
-    hot_path(q.device).qk_norm_rotary([dict(x=q, y=yq, pos=pos_q, weight=f32(wq)), dict(x=k, y=yk, pos=pos_k, weight=f32(wk))],
-                                      freq, eps, interleaved, amplitude)
-    return yq, yk
+    y = torch_ops().rotary(x, pos, freq, interleaved, amplitude)
+    if y is None:
+        x, pos = _inner(x), pos.contiguous()
+        hot_path(x.device).check_rotary(x, pos, freq)
+        y = torch_ops().rotary(x, pos, freq, interleaved, amplitude)
+    return y
 
 
 def qk_norm_rotary(q, k, pos_q, pos_k, q_weight, k_weight, freq, *, eps=1e-6, interleaved=False, amplitude=1.0):
@@ -125,14 +70,16 @@ def qk_norm_rotary(q, k, pos_q, pos_k, q_weight, k_weight, freq, *, eps=1e-6, in
     launch, statistics in 32 bits.  pos_q [Nq], pos_k [Nk] int64 (ignored and allowed to be None when freq is None: the
     norm alone); weights [D] (shared by the heads), [H, D] or None.  Differentiable in q, k and the weights."""
     _on_hip(q, "qk_norm_rotary")
-    q, k = _inner(q), _inner(k)
-    pos_q = None if freq is None or pos_q is None else pos_q.contiguous()
-    pos_k = None if freq is None or pos_k is None else pos_k.contiguous()
-    if freq is not None and (pos_q is None or pos_k is None):
-        raise ValueError("qk_norm_rotary: a rotation needs pos_q and pos_k")
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, q_weight, k_weight)):
-        return _QKNorm.apply(q, k, pos_q, pos_k, q_weight, k_weight, freq, float(eps), bool(interleaved), float(amplitude))
-    return _norm_forward(q, k, pos_q, pos_k, q_weight, k_weight, freq, eps, interleaved, amplitude)
+    y = torch_ops().norm(q, k, pos_q, pos_k, q_weight, k_weight, freq, eps, interleaved, amplitude)
+    if y is None:
+        q, k = _inner(q), _inner(k)
+        if freq is not None:
+            if pos_q is None or pos_k is None:
+                raise ValueError("qk_norm_rotary: a rotation needs pos_q and pos_k")
+            pos_q, pos_k = pos_q.contiguous(), pos_k.contiguous()
+        hot_path(q.device).check_qk_norm_rotary((q, k), (pos_q, pos_k), (q_weight, k_weight), freq)
+        y = torch_ops().norm(q, k, pos_q, pos_k, q_weight, k_weight, freq, eps, interleaved, amplitude)
+    return y
 
 
 class RotaryEncoder(nn.Module):
