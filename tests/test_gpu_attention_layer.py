@@ -1,0 +1,190 @@
+"""The attention-layer operators as they are used together: sampled blocks -> projections -> norm and rotation by event
+times -> differential attention -> gradients.  Every operator of the run is held to its own 64-bit form and bounds, on the
+values that it was given in that run."""
+import numpy as np
+import pytest
+import torch
+
+import attn_plain as plain
+from starrygl_amd.nn.model import TemporalDiffAttention, attention, diff_attention, qk_norm_rotary, rotary_encode, rotary_frequencies
+from starrygl_amd.utils import synth
+
+pytestmark = pytest.mark.gpu
+
+
+def _within(got, want, tol, name):
+    got = got.detach().cpu().double()
+    assert got.shape == want.shape
+    bad = ((got - want).abs() > tol) | got.isnan()
+    assert not bad.any(), (name, int(bad.sum()), float((got - want).abs().max()))
+
+
+@pytest.fixture(scope="module")
+def blocks(hot):
+    from starrygl_amd.graph.graph import AsyncBlock, pyGraph
+    n, m, C = 400, 6000, 4
+    src, dst, ts, eid = synth.graph_stream(n, m, 1.15, 100_000, 3)
+    g = pyGraph(*(torch.from_numpy(a) for a in (src, dst, ts)), n, C, eid=torch.from_numpy(eid),
+                chunk_mapper=torch.from_numpy(np.arange(n) % C))
+    neg = torch.arange(20)
+    policy = dict(sample_type="recent", layers=2, fanout=6, allowed_offset=-1, equal_root_time=False, keep_root_time=False)
+    made = {}
+    for self_loop in (True, False):
+        g.async_sample(60_000, 60_400, torch.arange(C), policy,
+                       dict(test_generate_samples=neg, test_generate_samples_ts=torch.full((20,), 60_200)), op="r")
+        s = g.get_last_sample()
+        made[self_loop] = AsyncBlock.to_block(s.roots, s.neg_roots, s.neighbors, s.nodes_remapper_id, self_loop=self_loop), s
+    return n, m, made
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("heads,kv_heads,dim_head", [(2, 2, 32), (4, 1, 25)])
+def test_two_layers_over_sampled_blocks(blocks, monkeypatch, heads, kv_heads, dim_head, dtype):
+    n, m, made = blocks
+    (root, neg, mfgs, _), s = made[True]
+    torch.manual_seed(0)
+    dim, dim_edge = 24, 10
+    table, edges = torch.randn(n, dim), torch.randn(m, dim_edge)
+    layers = [TemporalDiffAttention(dim, dim_edge, dim, heads, kv_heads, dim_head).cuda().to(dtype) for _ in mfgs]
+    assert all(layer.rotary.freq.dtype == torch.float64 for layer in layers)
+    runs = []
+
+    def kept(q, k, v, lam, k_ptr):
+        lam.retain_grad()
+        out = diff_attention(q, k, v, lam, k_ptr)
+        out.retain_grad()
+        runs.append(dict(q=q, k=k, v=v, lam=lam, out=out, k_ptr=k_ptr))
+        return out
+
+    def normed(module, args, got):
+        for t in (*args[:2], *got):
+            t.retain_grad()
+        norms.append((args, got, module))
+
+    norms = []
+    monkeypatch.setattr(attention, "diff_attention", kept)
+    for layer in layers:
+        layer.rotary.register_forward_hook(normed)
+    h = table.to(dtype).cuda()[s.nodes_remapper_id[mfgs[0].srcdata["nid"]]].requires_grad_()
+    x = h
+    for layer, b in zip(layers, mfgs):
+        x = layer(b, x, edges.to(dtype).cuda()[b.edata["eid"]])
+        assert x.shape == (b.num_dst_nodes(), dim)
+    for r in runs:
+        r["v"].retain_grad()
+    x.float().square().mean().mul(512.0).backward()
+    assert len(runs) == len(norms) == 2 and h.grad.isfinite().all() and (h.grad != 0).any()
+    for layer in layers:
+        for name, p in layer.named_parameters():
+            assert p.grad is not None and p.grad.isfinite().all() and (p.grad != 0).any(), name
+    for r, ((q0, k0, tq, tk), (q1, k1), mod) in zip(runs, norms):
+        go = r["out"].grad
+        ref = plain.diff_attention(r["q"], r["k"], r["v"], r["lam"], r["k_ptr"], grad=go)
+        _within(r["out"], ref["out"], ref["out_tol"], "out")
+        _within(r["v"].grad, ref["dv"], ref["dv_tol"], "dv")
+        _within(r["lam"].grad, ref["dlam"], ref["dlam_tol"], "dlam")
+        _within(q1.grad, ref["dq"].flatten(1, 2), ref["dq_tol"].flatten(1, 2), "dq")
+        _within(k1.grad, ref["dk"].flatten(1, 2), ref["dk_tol"].flatten(1, 2), "dk")
+        freq = mod.freq.cpu()
+        for a, y, t, w, tag in ((q0, q1, tq, mod.q_weight, "q"), (k0, k1, tk, mod.k_weight, "k")):
+            a32, t, w32, g = a.detach().cpu(), t.cpu(), w.detach().cpu(), y.grad.cpu()
+            want, mag = plain.norm_rotate(a32, t, w32, freq, mod.eps)
+            _within(y, want, plain.rounding(dtype, want) + 2.0 ** -18 * mag, tag)
+            dx, dxm, dw, dwm = plain.norm_rotate_grads(a32, t, w32, freq, mod.eps, g)
+            _within(a.grad, dx, plain.rounding(dtype, dx) + 2.0 ** -17 * dxm, "d" + tag)
+            _within(w.grad, dw, plain.rounding(dtype, dw) + (2.0 ** -17 + a.shape[0] * a.shape[1] * plain.U) * dwm, "dw" + tag)
+
+
+def test_blocks_without_self_loops_and_destinations_without_edges(blocks):
+    _, _, made = blocks
+    (root, neg, mfgs, _), s = made[False]
+    b = mfgs[-1]                                            # the roots' own block
+    assert b.num_dst_nodes() == b.indptr.numel() - 1
+    layer = TemporalDiffAttention(8, 0, 5, heads=2, dim_head=16).cuda()
+    h, h_dst = torch.randn(b.num_src_nodes(), 8, device="cuda"), torch.randn(b.num_dst_nodes(), 8, device="cuda")
+    ts = torch.full((b.num_dst_nodes(),), 60_500, device="cuda")
+    y = layer(b, h, h_dst=h_dst, dst_ts=ts)
+    alone = (b.indptr[1:] == b.indptr[:-1]).nonzero().flatten()
+    full = torch.cat([torch.zeros(alone.numel(), 2 * 32, device="cuda"), h_dst[alone]], 1)
+    assert y.shape == (b.num_dst_nodes(), 5) and torch.allclose(y[alone], layer.out(full), rtol=1e-4, atol=1e-5)
+    with pytest.raises(ValueError, match="come together"):
+        layer(b, h, h_dst=h_dst)
+    with pytest.raises(ValueError, match="multiple"):
+        TemporalDiffAttention(8, 0, 5, heads=3, kv_heads=2)
+
+
+def _leaves(dtype=torch.float32):
+    g = torch.Generator().manual_seed(1)
+    r = lambda *s: torch.randn(*s, generator=g).to(dtype).cuda().requires_grad_()  # noqa: E731
+    return r(6, 2, 2, 16), r(20, 1, 2, 16), r(20, 1, 32), torch.tensor([0.3, 0.7], device="cuda", requires_grad=True)
+
+
+def test_gradients_are_not_differentiated_again(hot):
+    freq = rotary_frequencies(16)[0].cuda()
+    q, k, v, lam = _leaves()
+    pos = torch.arange(20, device="cuda")
+    ptr = torch.tensor([0, 3, 3, 8, 12, 15, 20], device="cuda")
+    runs = ((rotary_encode(v, pos, freq), [v]), (diff_attention(q, k, v, lam, ptr), [q, k, v, lam]),
+            (torch.cat(qk_norm_rotary(q[:, 0], k[:, 0], pos[:6], pos, None, None, freq)), [q, k]))
+    for y, leaves in runs:
+        once = torch.autograd.grad(y.sum(), leaves, retain_graph=True)
+        again = torch.autograd.grad(y.sum(), leaves, create_graph=True)         # the gradient itself is there
+        assert all(torch.equal(a, b) for a, b in zip(once, again))
+        with pytest.raises(RuntimeError, match="again"):
+            again[0].square().sum().backward()
+
+
+def test_some_of_the_gradients(hot):
+    """inputs that want no gradient, a side whose result is not used, one weight for both sides, a hook that edits"""
+    freq = rotary_frequencies(16)[0].cuda()
+    q, k, v, lam = _leaves()
+    ptr = torch.tensor([0, 3, 3, 8, 12, 15, 20], device="cuda")
+    whole = torch.autograd.grad(diff_attention(q, k, v, lam, ptr).square().sum(), [q, k, v, lam])
+    for i in range(4):
+        only = [t if j == i else t.detach() for j, t in enumerate((q, k, v, lam))]
+        assert torch.equal(torch.autograd.grad(diff_attention(*only, ptr).square().sum(), [only[i]])[0], whole[i])
+    w = torch.rand(16, device="cuda", requires_grad=True)
+    a, b = q.detach()[:, 0].requires_grad_(), k.detach()[:, 0].requires_grad_()
+    pa, pb = torch.arange(6, device="cuda"), torch.arange(20, device="cuda")
+    ya, yb = qk_norm_rotary(a, b, pa, pb, w, w, freq)
+    ga, gb, gw = torch.autograd.grad([ya, yb], [a, b, w], [torch.ones_like(ya), torch.ones_like(yb)], retain_graph=True)
+    (ga2,) = torch.autograd.grad(ya.sum(), a, retain_graph=True)
+    (gw1,) = torch.autograd.grad(ya.sum(), w, retain_graph=True)
+    (gw2,) = torch.autograd.grad(yb.sum(), w, retain_graph=True)
+    assert torch.equal(ga, ga2) and torch.equal(gw, gw1 + gw2)
+    yc, _ = qk_norm_rotary(a, b, None, None, w, None, None)                       # the norm alone: no positions, no freq
+    (gc,) = torch.autograd.grad(yc.sum(), w)
+    n = a.detach().cpu().double()
+    n = n * (n.square().mean(-1, keepdim=True) + 1e-6).rsqrt()
+    assert (gc.cpu().double() - n.sum((0, 1))).abs().max() <= (2.0 ** -17 + 12 * plain.U) * n.abs().sum((0, 1)).max()
+    with pytest.raises(RuntimeError, match="modified by an inplace"):
+        y = diff_attention(q, k, v, lam, ptr)
+        with torch.no_grad():
+            k.mul_(1.0)
+        y.sum().backward()
+
+
+def test_steps_on_two_streams_at_once(hot):
+    """forward and backward of two steps in flight on two streams, their workspaces apart"""
+    def step(seed):
+        g = torch.Generator().manual_seed(seed)
+        leaves = [torch.randn(*s, generator=g).bfloat16().cuda().requires_grad_() for s in ((300, 4, 2, 64), (900, 2, 2, 64), (900, 2, 128))]
+        lam = torch.rand(4, generator=g).cuda().requires_grad_()
+        ptr = torch.arange(0, 901, 3).cuda()
+        return [*leaves, lam], ptr
+    work = [step(1), step(2)]
+    want = []
+    for leaves, ptr in work:
+        y = diff_attention(*leaves, ptr)
+        want.append((y, torch.autograd.grad(y, leaves, torch.ones_like(y))))
+    torch.cuda.synchronize()
+    side = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = [None, None]
+    for _ in range(5):
+        for i, (leaves, ptr) in enumerate(work):
+            with torch.cuda.stream(side[i]):
+                y = diff_attention(*leaves, ptr)
+                got[i] = y, torch.autograd.grad(y, leaves, torch.ones_like(y))
+    torch.cuda.synchronize()
+    for (y0, g0), (y1, g1) in zip(want, got):
+        assert torch.equal(y0, y1) and all(torch.equal(a, b) for a, b in zip(g0, g1))
