@@ -245,6 +245,45 @@ __device__ __forceinline__ typename Mat<T>::Frag col_frag(const char* tile, int 
     }
 }
 
+// The same by the lane's part of the address, which the caller keeps: of row `col` and chunk 2 i + half (tile + 1024 (i / 4) + part
+// i % 4), of the transposed fragment of elements 32 t (part t % 2; fp32: part of rows 8 s, s odd or even).
+template <int RB>
+__device__ __forceinline__ int32_t lane_row(int col, int i, int half) {
+    return (col >> 3) * (RB / 128) * 1024 + ((col & 7) << 7) + ((((2 * i) & 7) ^ (half ^ mix(col))) << 4);
+}
+template <typename T, int RB>
+__device__ __forceinline__ int32_t lane_col(int e, int lane) {
+    const int half = lane >> 5;
+    if constexpr (sizeof(T) == 2) {
+        const int r = 4 * half + ((lane & 15) >> 2), c = ((lane >> 4) & 1) * 2 + ((lane & 3) >> 1);
+        return r * 128 + ((((4 * e) & 7) ^ (c ^ mix(r))) << 4) + (lane & 1) * 8;
+    } else {
+        const int r = 4 * half, c = (lane & 31) >> 2;
+        return (r << 7) + ((c ^ mix(r + 8 * e)) << 4) + (lane & 3) * 4;
+    }
+}
+template <typename T, int RB>
+__device__ __forceinline__ typename Mat<T>::Frag col_at(const char* tile, const int32_t (&by)[2], int32_t off, int s, int t) {
+    if constexpr (sizeof(T) == 2) {
+        const char* base = tile + (2 * s * (RB / 128) + (t >> 1)) * 1024;
+        typedef SGL_LDS s16x4 lds4;
+        union {
+            s16x8 v;
+            typename Mat<T>::Frag f;
+        } u;
+        const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(base + (by[t & 1] + off)));
+        const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(base + (RB / 128) * 1024 + ((by[t & 1] ^ 32) + off)));
+        u.v = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+        return u.f;
+    } else {
+        typename Mat<T>::Frag f;
+        const char* base = tile + (s * (RB / 128) + t) * 1024;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) f[j] = *reinterpret_cast<const float*>(base + (j << 7) + ((by[s & 1] ^ (mix(j) << 4)) + off));
+        return f;
+    }
+}
+
 // Fragments 0 .. N - 1 from LDS, `use`d in turn with the next DEPTH on their way.  The order is fixed: left to itself the
 // compiler, short of registers, reads each fragment into the same four and waits for it (a read takes as long as four
 // products).
@@ -259,8 +298,12 @@ struct Pipe {
     }
     template <typename Load, typename Use>
     __device__ __forceinline__ void drain(Load load, Use use) {
+        part<0, N>(load, use);
+    }
+    template <int FROM, int TO, typename Load, typename Use>
+    __device__ __forceinline__ void part(Load load, Use use) {
 #pragma unroll
-        for (int n = 0; n < N; ++n) {
+        for (int n = FROM; n < TO; ++n) {
             use(n, f[n % DEPTH]);
             if (n + DEPTH < N) f[n % DEPTH] = load(n + DEPTH);
             __builtin_amdgcn_sched_barrier(0);

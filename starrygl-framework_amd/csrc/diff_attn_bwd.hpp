@@ -22,14 +22,6 @@ struct Shape {
     static constexpr int DT = DP / 32, VT = 2 * DP / 32;        // 32-wide tiles of a half, of the values
     // query side: a wave per 32 rows and map, eight to a block while the registers of two a SIMD hold their operands
     static constexpr int Q_WAVES = RB > 256 ? (RB > 512 ? 4 : 8) : 4, Q_ROWS = Q_WAVES / 2 * 32, Q_OCC = RB <= 256 ? 3 : RB <= 512 ? 2 : 1;
-    // key side: a wave per 32 keys; from 512-byte rows on two waves share the keys, one sums dK, the other dV (each computes the
-    // scores: 5/4 of the products, but the sums of one wave do not fit the registers of two a SIMD)
-    static constexpr bool ROLES = RB >= 256;
-    static constexpr int K_WAVES = RB > 512 ? 2 : 4, K_ROWS = (ROLES ? K_WAVES / 2 : K_WAVES) * 32, K_OCC = RB > 512 ? 1 : 2;
-    // the owned keys and values: fragments in registers, or read from a tile of their own in LDS
-    static constexpr bool KEY_REGS = RB <= 128, VAL_REGS = RB <= 512;
-    static constexpr int OWN = (KEY_REGS ? 0 : RB) + (VAL_REGS ? 0 : RB);       // bytes of an owned row in LDS
-    static constexpr bool TWO = RB <= 512;                      // two buffers of the walked side
 };
 
 __device__ __forceinline__ float signed_c2(const AttnArgs& g) { return g.scale < 0.f ? -g.c2 : g.c2; }
@@ -44,24 +36,53 @@ __device__ __forceinline__ bool any_nan(const f32x16 (&x)[N]) {
     return b;
 }
 
-// acc[t] += (transposed rows row0.. of the tile, elements from 32 (t0 + t)) * x, x the results of 32 walked rows
+// results of 32 walked rows as right operands
+template <typename T>
+struct Operand {
+    static constexpr int EP = Mat<T>::EP, PS = 32 / (2 * EP);
+    typename Mat<T>::Frag f[PS];
+    // registers r, r + 1 (r even): rounded as a pair, one instruction
+    __device__ __forceinline__ void set2(int r, float x, float y) {
+        if constexpr (sizeof(T) == 2) {
+            typedef float f32x2 __attribute__((ext_vector_type(2)));
+            typedef T pair __attribute__((ext_vector_type(2)));
+            typedef uint32_t words __attribute__((ext_vector_type(4)));
+            words w = __builtin_bit_cast(words, f[r / EP]);
+            w[r % EP / 2] = __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{x, y}), pair));
+            f[r / EP] = __builtin_bit_cast(typename Mat<T>::Frag, w);
+        } else {
+            f[r / EP][r % EP] = x;
+            f[r / EP][r % EP + 1] = y;
+        }
+    }
+    __device__ __forceinline__ void mask(uint32_t see) {
+        asm volatile("" : "+v"(see));       // (or the 16 bits are kept from one mask to the next, whether there is one or not)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) f[r / EP][r % EP] = row_bit(see, r) ? f[r / EP][r % EP] : (T)0.f;
+    }
+};
+template <typename T>
+__device__ __forceinline__ Operand<T> operand(const f32x16& x) {
+    Operand<T> o;
+#pragma unroll
+    for (int k = 0; k < Operand<T>::PS; ++k) o.f[k] = to_frag<T>(x, k);
+    return o;
+}
+
+// acc[t] += (transposed rows row0.. of the tile, elements from 32 (t0 + t)) * x
 template <typename T, int RB, int N, int AHEAD>
-__device__ __forceinline__ void add_product(f32x16 (&acc)[N], const char* tile, int row0, int t0, const f32x16& x, int lane) {
+__device__ __forceinline__ void add_product(f32x16 (&acc)[N], const char* tile, int row0, int t0, const Operand<T>& x, int lane) {
     typedef Mat<T> M;
-    constexpr int PS = 32 / (2 * M::EP);
+    constexpr int PS = Operand<T>::PS;
     auto load = [&](int n) { return col_frag<T, RB>(tile, row0, n / N, t0 + n % N, lane); };
     Pipe<T, PS * N, AHEAD> ahead;
     ahead.fill(load);
-    typename M::Frag p;
-    ahead.drain(load, [&](int n, const typename M::Frag& f) {
-        if (n % N == 0) p = to_frag<T>(x, n / N);
-        acc[n % N] = M::mma(f, p, acc[n % N]);
-    });
+    ahead.drain(load, [&](int n, const typename M::Frag& f) { acc[n % N] = M::mma(f, x.f[n / N], acc[n % N]); });
 }
 
 // the same over half `map` of a head
 template <typename T, int RB, int N, int AHEAD>
-__device__ __forceinline__ void add_map(f32x16 (&acc)[N], const char* tile, int row0, int map, const f32x16& x, int lane) {
+__device__ __forceinline__ void add_map(f32x16 (&acc)[N], const char* tile, int row0, int map, const Operand<T>& x, int lane) {
     if constexpr (RB >= 256 && (N & 1) == 0) {
         add_product<T, RB, N, AHEAD>(acc, tile + map * (RB / 256) * 1024, row0, 0, x, lane);
     } else {
@@ -188,7 +209,7 @@ __global__ __launch_bounds__((Shape<T, DP>::Q_WAVES * 64), (Shape<T, DP>::Q_OCC)
                 sum = __builtin_fmaf(p, dp[r], sum);
                 s[r] = p * (dp[r] - t);            // (the second map's times -lam at the end)
             }
-            add_map<T, RB, S::DT, AHEAD>(dq, buf, sub * 32, map, s, lane);
+            add_map<T, RB, S::DT, AHEAD>(dq, buf, sub * 32, map, operand<T>(s), lane);
         }
     };
     bool spoilt = false;        // the query sees something not finite: NaN
@@ -248,37 +269,15 @@ __global__ __launch_bounds__((Shape<T, DP>::Q_WAVES * 64), (Shape<T, DP>::Q_OCC)
                                       g.aligned, row_out<T>(a.d_q, i0, 2 * h + map), a.d_q.row_stride, keep);
 }
 
-// LDS of a block
-template <typename T, int DP>
-struct KvSmem {
-    static constexpr int BQ = 32, TILE = 2 * BQ * Shape<T, DP>::RB;
-    static constexpr int STAT = BQ * 4 * 4;                     // lse and t of a row, two each
-};
-
-// DK, DV: what this wave sums
-template <typename T, int DP, bool DMA, bool DK, bool DV>
-__device__ __forceinline__ void kv_body(const AttnArgs& g, int32_t tiles, char* s_a, char* s_b, char* s_own, uint8_t* s_marks, int* s_lo, int* s_hi, int& s_bad) {
-    typedef Shape<T, DP> S;
-    typedef Mat<T> M;
-    constexpr int RB = S::RB, NT = S::K_WAVES * 64, ROWS = S::K_ROWS, GROUPS = ROWS / 32, BQ = KvSmem<T, DP>::BQ, TILE = KvSmem<T, DP>::TILE, AHEAD = 2;
-    const sgl_diff_attn_args& a = g.a;
-    const int G = a.Hq / a.Hk;
-    const uint32_t n = (uint32_t)tiles * (uint32_t)a.Hk, item = xcd_item(n);
-    if (item >= n) return;
-    // key heads side by side; of a causal call the early keys, which most rows see, come first
-    const int hk = (int)(item % (uint32_t)a.Hk);
-    const int32_t tile = (int32_t)(item / (uint32_t)a.Hk);
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, group = wave % GROUPS, half = lane >> 5, col = lane & 31;
-    const int32_t B = (int32_t)live_count(a.B_dev, a.B);
-    const int32_t j0 = tile * ROWS + group * 32, j = j0 + col;
+// the query rows that may see key j0 + col, and its sequence; shown: some do
+__device__ __forceinline__ Span rows_of(const sgl_diff_attn_args& a, int32_t B, int32_t j0, int32_t col, bool& shown, int32_t& seq) {
+    const int32_t j = j0 + col;
     const int32_t at[1] = {col};
     int32_t found[1];
     find_seqs<1>(a.k_ptr, B, j0, at, found);
-    const int32_t seq = j >= a.Tk ? -1 : found[0];
-    // the query rows that may see the key
+    seq = j >= a.Tk ? -1 : found[0];
     Span rows{0, 0};
-    bool shown = seq >= 0 && (a.key_mask == nullptr || a.key_mask[j]);
-    if (shown) {
+    if (seq >= 0 && (a.key_mask == nullptr || a.key_mask[j])) {
         const int64_t q0 = a.q_ptr ? clamp_to(a.q_ptr[seq], a.Tq) : seq, q1 = a.q_ptr ? clamp_to(a.q_ptr[seq + 1], a.Tq) : seq + 1;
         int64_t from = q0, to = q1;
         if (a.causal) {
@@ -289,10 +288,63 @@ __device__ __forceinline__ void kv_body(const AttnArgs& g, int32_t tiles, char* 
         if (from < to) rows = Span{(int32_t)from, (int32_t)to};
     }
     shown = rows.lo < rows.hi;
+    return rows;
+}
+
+// d_lam of a head: the row tiles' sums in their order
+template <int NT>
+__device__ __forceinline__ void sum_lam(const AttnArgs& g, int h, int32_t row_tiles, char* scratch) {
+    float* s_sum = reinterpret_cast<float*>(scratch);
+    float x = 0.f;
+    for (int k = threadIdx.x; k < row_tiles; k += NT) x += g.lam_part[(int64_t)k * g.a.Hq + h];
+    s_sum[threadIdx.x] = x;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        float y = 0.f;
+        for (int k = 0; k < NT; ++k) y += s_sum[k];
+        g.a.d_lam[h] = -y;
+    }
+}
+
+// ------------------------------------------------------------------------------------- owned: keys, rows up to 512 bytes
+// A wave owns 32 keys: both maps' scores, dP, dV and dK of a tile of 32 query rows, nothing twice.  The products alternate with
+// the vector instructions of the phase before (scores of the second map with the exponentials of the first, and so on), so
+// that both kinds overlap within a wave; from 256-byte rows on one wave a SIMD has the registers for that.  At 512 bytes the
+// sums of a wave take half of them; there two waves share the keys, take every other tile and add up at the end, and the keys
+// of the first map come from LDS.
+template <typename T, int DP>
+struct Keys {
+    static constexpr int RB = Shape<T, DP>::RB, SPLIT = RB > 256 ? 2 : 1, SUBS = 2, BQ = 32 * SUBS, TILE = 2 * BQ * RB, STAT = 3 * 256;
+    static constexpr int BUF = TILE + SUBS * STAT;              // rows; per 32 of them lse and t of both maps, lam
+    static constexpr int WAVES = 4, GROUPS = WAVES / SPLIT, ROWS = GROUPS * 32, OCC = RB < 256 ? 2 : 1, AHEAD = RB < 256 ? 2 : 4;
+    static constexpr int KEY_LDS = RB > 256;           // maps whose keys are read from LDS
+    static constexpr int OWN = KEY_LDS ? ROWS * RB / 2 * KEY_LDS : 16;
+};
+
+template <typename T, int DP, bool DMA>
+__device__ __forceinline__ void keys_body(const AttnArgs& g, int32_t tiles, char* s_a, char* s_b, char* s_own, uint8_t* s_marks, int* s_lo, int* s_hi, int& s_bad) {
+    typedef Shape<T, DP> S;
+    typedef Keys<T, DP> P;
+    typedef Mat<T> M;
+    constexpr int RB = S::RB, NT = P::WAVES * 64, ROWS = P::ROWS, GROUPS = P::GROUPS, BQ = P::BQ, TILE = P::TILE, AHEAD = P::AHEAD;
+    const sgl_diff_attn_args& a = g.a;
+    const int G = a.Hq / a.Hk;
+    const uint32_t n = (uint32_t)tiles * (uint32_t)a.Hk, item = xcd_item(n);
+    if (item >= n) return;
+    // key heads side by side; of a causal call the early keys, which most rows see, come first
+    const int hk = (int)(item % (uint32_t)a.Hk);
+    const int32_t tile = (int32_t)(item / (uint32_t)a.Hk);
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), group = wave % GROUPS, half = lane >> 5, col = lane & 31;
+    const int share = wave / GROUPS;                            // which of the tiles
+    const int32_t B = (int32_t)live_count(a.B_dev, a.B);
+    const int32_t j0 = tile * ROWS + group * 32, j = j0 + col;
+    bool shown;
+    int32_t seq;
+    const Span rows = rows_of(a, B, j0, col, shown, seq);
     // the wave's union, and the run of rows that see all its keys (if it has no key that none sees)
     Reach reach = reach_of(rows);
     if (!__all(shown)) reach.to = 0;
-    if (lane == 0) s_lo[group] = reach.lo, s_hi[group] = reach.hi;
+    if (lane == 0) s_lo[wave] = reach.lo, s_hi[wave] = reach.hi;
     if (threadIdx.x == 0) s_bad = 0;
     __syncthreads();
     int32_t lo = s_lo[0], hi = s_hi[0];
@@ -301,21 +353,314 @@ __device__ __forceinline__ void kv_body(const AttnArgs& g, int32_t tiles, char* 
     typename M::Frag k[2][S::QS], v[S::VS];
     {
         const int64_t jj = j < a.Tk ? j : 0;
-        if constexpr (S::KEY_REGS) {
 #pragma unroll
-            for (int m = 0; m < 2; ++m)
+        for (int m = P::KEY_LDS; m < 2; ++m)
 #pragma unroll
-                for (int e = 0; e < S::QS; ++e) k[m][e] = global_frag<T, DMA>(row<T>(a.k, jj, 2 * hk + m), (2 * e + half) * S::EP, a.D, g.aligned);
+            for (int e = 0; e < S::QS; ++e) k[m][e] = global_frag<T, DMA>(row<T>(a.k, jj, 2 * hk + m), (2 * e + half) * S::EP, a.D, g.aligned);
+        if constexpr (P::KEY_LDS == 2) Stager<T, DP, ROWS, NT, false, true>().load(s_own, halves<T>(a.k, hk, a.D), tile * ROWS, (int32_t)a.Tk - 1, g.aligned);
+        if constexpr (P::KEY_LDS == 1) Stager<T, DP / 2, ROWS, NT, false, false>().load(s_own, run<T>(a.k, 2 * hk, a.D), tile * ROWS, (int32_t)a.Tk - 1, g.aligned);
+#pragma unroll
+        for (int e = 0; e < S::VS; ++e) v[e] = global_frag<T, DMA>(row<T>(a.v, jj, hk), (2 * e + half) * S::EP, a.Dv, g.aligned);
+    }
+    f32x16 dk[2][S::DT], dv[S::VT];
+    auto clear = [&]() {
+#pragma unroll
+        for (int m = 0; m < 2; ++m)
+#pragma unroll
+            for (int d = 0; d < S::DT; ++d) dk[m][d] = zero16();
+#pragma unroll
+        for (int d = 0; d < S::VT; ++d) dv[d] = zero16();
+    };
+    clear();
+    const float c2 = __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(signed_c2(g))));
+    const int32_t last = (int32_t)a.Tq - 1;
+    const int32_t per_head = lo < hi ? (hi - lo + BQ - 1) / BQ : 0, steps = per_head * G;      // head by head, row tile by row tile
+    Stager<T, DP, BQ, NT, DMA, true> stage_q;
+    Stager<T, DP, BQ, NT, DMA, false> stage_go;
+    stage_q.plan(halves<T>(a.q, 0, a.D));
+    stage_go.plan(run<T>(a.d_out, 0, a.Dv));
+    bool finite = false;        // the pass without what is not finite
+    auto load = [&](char* buf, int h, int32_t i0) {
+        if (finite) {
+            stage_finite<T, DP, BQ, NT>(buf, s_marks, halves<T>(a.q, h, a.D), true, i0, last);
+            stage_finite<T, DP, BQ, NT>(buf + BQ * RB, s_marks + BQ * (RB / 16), run<T>(a.d_out, h, a.Dv), false, i0, last);
+        } else {
+            stage_q.load(buf, halves<T>(a.q, h, a.D), i0, last, g.aligned);
+            stage_go.load(buf + BQ * RB, run<T>(a.d_out, h, a.Dv), i0, last, g.aligned);
         }
-        if constexpr (S::VAL_REGS && DK) {
+        if (wave < 3) {
+            // 64 numbers each: lse, t of the rows, map by map, and lam 64 times (a load of its own in a step would wait for the
+            // tile that is on its way)
 #pragma unroll
-            for (int e = 0; e < S::VS; ++e) v[e] = global_frag<T, DMA>(row<T>(a.v, jj, hk), (2 * e + half) * S::EP, a.Dv, g.aligned);
+            for (int u = 0; u < P::SUBS; ++u) {
+                const int32_t i = min(i0 + 32 * u + (lane & 31), last);
+                const float* src = wave == 2 ? a.lam + h : (wave ? g.delta : a.lse) + ((int64_t)i * a.Hq + h) * 2 + (lane >> 5);
+                const int at0 = __builtin_amdgcn_readfirstlane(u * P::STAT + wave * 256);
+                __builtin_amdgcn_global_load_lds((SGL_GLOBAL void*)src, (SGL_LDS void*)(buf + TILE + at0), 4, 0, 0);
+            }
+        }
+    };
+    // The lane's parts of the addresses, fixed here (left alone the compiler keeps the sum of each with every buffer)
+    int32_t by_row[4], by_key[4], by_col[2], by_stat = 16 * half + share * P::STAT;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        if (P::KEY_LDS) by_key[e] = lane_row<RB / 2 * P::KEY_LDS>(col, e, half) + group * 4 * (RB * P::KEY_LDS / 256) * 1024;
+        by_row[e] = lane_row<RB>(col, e, half) + share * 4 * (RB / 128) * 1024;
+        asm volatile("" : "+v"(by_row[e]), "+v"(by_key[e]));
+    }
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+        by_col[e] = lane_col<T, RB>(e, lane) + share * 4 * (RB / 128) * 1024;
+        asm volatile("" : "+v"(by_col[e]));
+    }
+    asm volatile("" : "+v"(by_stat));
+    auto of_row = [](const char* tile, const int32_t (&by)[4], int i) { return *reinterpret_cast<const typename M::Frag*>(tile + (i >> 2) * 1024 + by[i & 3]); };
+    // 32 rows from i0, the first of which is row `sub` of the tile (beside the wave's share)
+    auto sub_step = [&](const char* buf, int32_t i0, int sub) {
+        i0 += 32 * share + sub;
+        if (i0 >= reach.hi || i0 + 32 <= reach.lo) return;
+        constexpr int PS = Operand<T>::PS, QS = S::QS, NK = S::DT * PS;
+        constexpr int N1 = QS, N2 = 2 * QS, N3 = N2 + S::VS, N4 = N3 + S::VT * PS, N5 = N4 + NK, N6 = N5 + NK;
+        const char* go = buf + BQ * RB + sub * RB;
+        const char* stat = buf + TILE + sub / 32 * P::STAT + by_stat;
+        buf += sub * RB;
+        f32x4 num[4];           // lse of the first map, then of the second, then t of either: a group is read a phase before its use
+#pragma unroll
+        for (int k = 0; k < 4; ++k) num[k] = *reinterpret_cast<const f32x4*>(stat + 32 * k);
+        const float lam = *reinterpret_cast<const float*>(stat + 512);
+        const bool some = !(i0 >= reach.from && i0 + 32 <= reach.to);
+        uint32_t see = 0;
+        if (some) see = span_bits(i0, rows) >> (4 * half);
+        f32x16 s[2], dp;
+        s[0] = s[1] = dp = zero16();
+        Operand<T> p, ds[2];
+        auto load_n = [&](int n) {
+            if (n < N2) return of_row(buf, by_row, n);
+            if (n < N3) return of_row(go, by_row, n - N2);
+            if (n < N4) return col_at<T, RB>(go, by_col, 0, (n - N3) / S::VT, (n - N3) % S::VT);
+            // dK of a map: the tiles of its half
+            const int m = n < N5 ? 0 : 1, u = n - (m ? N5 : N4);
+            return col_at<T, RB>(buf, by_col, 0, u / S::DT, m * S::DT + u % S::DT);
+        };
+        auto load_own = [&](int n) { return of_row(s_own, by_key, n); };
+        // exponentials, d_score of registers r, r + 1 of a map
+        auto exps = [&](int m, int r, float f) {
+#pragma unroll
+            for (int e = r; e < r + 2; ++e) s[m][e] = f * exp2_hw(__builtin_fmaf(s[m][e], c2, -num[r / 4][e % 4]));
+            if (r % 4 == 2) num[r / 4] = *reinterpret_cast<const f32x4*>(stat + 128 * (m + 1) + 32 * (r / 4));
+        };
+        auto scores = [&](int m, int r) {
+            ds[m].set2(r, s[m][r] * (dp[r] - num[r / 4][r % 4]), s[m][r + 1] * (dp[r + 1] - num[r / 4][r % 4 + 1]));
+            if (r % 4 == 2 && m == 0) num[r / 4] = *reinterpret_cast<const f32x4*>(stat + 384 + 32 * (r / 4));
+        };
+        constexpr int FROM_LDS = P::KEY_LDS * QS;
+        Pipe<T, N6, AHEAD> ahead;
+        Pipe<T, FROM_LDS, AHEAD> own;
+        if constexpr (P::KEY_LDS) own.fill(load_own);
+        ahead.fill(load_n);
+        auto score = [&](int n, const typename M::Frag& x) {
+            f32x16& to = s[n / QS];
+            if (n < FROM_LDS) {
+                to = M::mma(x, own.f[n % AHEAD], to);
+                if (n + AHEAD < FROM_LDS) own.f[n % AHEAD] = load_own(n + AHEAD);
+            } else {
+                to = M::mma(x, k[n / QS][n % QS], to);
+            }
+        };
+        ahead.template part<0, N1>(load_n, [&](int n, const typename M::Frag& x) { score(n, x); });
+        ahead.template part<N1, N2>(load_n, [&](int n, const typename M::Frag& x) {
+            score(n, x);
+#pragma unroll
+            for (int r = 8 * (n - N1) / QS * 2; r < 8 * (n - N1 + 1) / QS * 2; r += 2) exps(0, r, 1.f);
+        });
+        ahead.template part<N2, N3>(load_n, [&](int n, const typename M::Frag& x) {
+            dp = M::mma(x, v[n - N2], dp);
+#pragma unroll
+            for (int r = 8 * (n - N2) / S::VS * 2; r < 8 * (n - N2 + 1) / S::VS * 2; r += 2) {
+                exps(1, r, -lam);
+                p.set2(r, s[0][r] + s[1][r], s[0][r + 1] + s[1][r + 1]);
+            }
+        });
+        if (some) p.mask(see);
+        ahead.template part<N3, N4>(load_n, [&](int n, const typename M::Frag& x) {
+            constexpr int N = N4 - N3;
+            const int u = n - N3;
+            dv[u % S::VT] = M::mma(x, p.f[u / S::VT], dv[u % S::VT]);
+#pragma unroll
+            for (int r = 8 * u / N * 2; r < 8 * (u + 1) / N * 2; r += 2) scores(0, r);
+        });
+        if (some) ds[0].mask(see);
+        ahead.template part<N4, N5>(load_n, [&](int n, const typename M::Frag& x) {
+            const int u = n - N4;
+            dk[0][u % S::DT] = M::mma(x, ds[0].f[u / S::DT], dk[0][u % S::DT]);
+#pragma unroll
+            for (int r = 8 * u / NK * 2; r < 8 * (u + 1) / NK * 2; r += 2) scores(1, r);
+        });
+        if (some) ds[1].mask(see);
+        ahead.template part<N5, N6>(load_n, [&](int n, const typename M::Frag& x) {
+            const int u = n - N5;
+            dk[1][u % S::DT] = M::mma(x, ds[1].f[u / S::DT], dk[1][u % S::DT]);
+        });
+    };
+    auto step = [&](const char* buf, int32_t i0) {
+#pragma unroll
+        for (int sub = 0; sub < BQ; sub += 32 * P::SPLIT) sub_step(buf, i0, sub);
+    };
+    bool spoilt[2] = {false, false};        // a row with something not finite sees the key: NaN
+    if (steps > 0) {
+        int h, hn;                          // head and first row of the tile at work, and of the one being loaded
+        int32_t i0, in;
+        auto next = [&]() {
+            in += BQ;
+            if (in >= hi) in = lo, ++hn;
+        };
+#pragma unroll 1
+        for (;;) {
+            hn = hk * G, in = lo;
+            load(s_a, hn, in);
+            staged();
+#pragma unroll 1
+            for (int32_t s = 0; s < steps; s += 2) {
+                h = hn, i0 = in;
+                next();
+                if (s + 1 < steps) load(s_b, hn, in);
+                step(s_a, i0);
+                staged();
+                if (s + 1 >= steps) break;
+                h = hn, i0 = in;
+                next();
+                if (s + 2 < steps) load(s_a, hn, in);
+                step(s_b, i0);
+                staged();
+            }
+            if (finite) break;
+            if ((any_nan(dk[0]) || any_nan(dk[1]) || any_nan(dv)) && shown) s_bad = 1;
+            __syncthreads();
+            if (!s_bad) break;
+            finite = true;
+            clear();
+        }
+        if (finite) {
+            // the keys that a row with something not finite sees get NaN
+            hn = hk * G, in = lo;
+#pragma unroll 1
+            for (int32_t s = 0; s < steps; ++s) {
+                __syncthreads();
+                stage_finite<T, DP, BQ, NT>(s_a, s_marks, halves<T>(a.q, hn, a.D), true, in, last);
+                stage_finite<T, DP, BQ, NT>(s_a + BQ * RB, s_marks + BQ * (RB / 16), run<T>(a.d_out, hn, a.Dv), false, in, last);
+                __syncthreads();
+#pragma unroll 1
+                for (int r = 0; r < BQ; ++r) {
+                    if (in + r < rows.lo || in + r >= rows.hi) continue;
+                    const uint8_t* of_out = s_marks + BQ * (RB / 16);
+                    const bool o = marked_any<RB>(of_out, r, 0, RB / 16);
+                    spoilt[0] = spoilt[0] || o || marked_any<RB>(s_marks, r, 0, RB / 32);
+                    spoilt[1] = spoilt[1] || o || marked_any<RB>(s_marks, r, RB / 32, RB / 16);
+                    if (o) spoil<T, RB, S::VT>(dv, of_out, r, half);
+                }
+                next();
+            }
+            __syncthreads();
         }
     }
-    if constexpr (!S::KEY_REGS) {
-        Stager<T, DP, ROWS, NT, false, true>().load(s_own, halves<T>(a.k, hk, a.D), tile * ROWS, (int32_t)a.Tk - 1, g.aligned);
-        if constexpr (!S::VAL_REGS) Stager<T, DP, ROWS, NT, false, false>().load(s_own + ROWS * RB, run<T>(a.v, hk, a.Dv), tile * ROWS, (int32_t)a.Tk - 1, g.aligned);
+    const uint32_t keep = (uint32_t)__ballot(j < a.Tk && (seq >= 0 || (a.flags & SGL_ATTN_ZERO_REST)));
+    // the tiles are free: the last barrier is behind every wave's last look at them
+    if constexpr (P::SPLIT == 2) {
+        // the first wave takes dK, the second dV; each hands the other's part over
+        static_assert(2 * S::DT * 4096 * GROUPS <= TILE && S::VT * 4096 * GROUPS <= TILE, "parts fit");
+        char* mine = s_a + group * (2 * S::DT * 4096) + lane * 16;
+        char* other = s_b + group * (S::VT * 4096) + lane * 16;
+        auto put = [&](char* box, const f32x16& x) {
+#pragma unroll
+            for (int r4 = 0; r4 < 4; ++r4) *reinterpret_cast<f32x4*>(box + r4 * 1024) = f32x4{x[4 * r4], x[4 * r4 + 1], x[4 * r4 + 2], x[4 * r4 + 3]};
+        };
+        auto add = [&](const char* box, f32x16& x) {
+#pragma unroll
+            for (int r4 = 0; r4 < 4; ++r4) {
+                const f32x4 y = *reinterpret_cast<const f32x4*>(box + r4 * 1024);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x[4 * r4 + e] += y[e];
+            }
+        };
+        if (share) {
+#pragma unroll
+            for (int d = 0; d < S::DT; ++d) put(mine + d * 4096, dk[0][d]), put(mine + (S::DT + d) * 4096, dk[1][d]);
+        } else {
+#pragma unroll
+            for (int d = 0; d < S::VT; ++d) put(other + d * 4096, dv[d]);
+        }
+        __syncthreads();
+        if (share) {
+#pragma unroll
+            for (int d = 0; d < S::VT; ++d) add(other + d * 4096, dv[d]);
+        } else {
+#pragma unroll
+            for (int d = 0; d < S::DT; ++d) add(mine + d * 4096, dk[0][d]), add(mine + (S::DT + d) * 4096, dk[1][d]);
+        }
+        __syncthreads();
     }
+    constexpr int PIECE = TILE / P::WAVES / 32;                 // bytes of a row at a time
+    char* box = s_a + wave * (TILE / P::WAVES);
+    if (P::SPLIT == 1 || !share) {
+        store_rows<T, PIECE, S::DT, DMA>([&](int t, int r) { return spoilt[0] ? NAN : shown ? dk[0][t][r] * g.scale : 0.f; }, box, lane, a.D, g.aligned,
+                                         row_out<T>(a.d_k, j0, 2 * hk), a.d_k.row_stride, keep);
+        store_rows<T, PIECE, S::DT, DMA>([&](int t, int r) { return spoilt[1] ? NAN : shown ? dk[1][t][r] * g.scale : 0.f; }, box, lane, a.D, g.aligned,
+                                         row_out<T>(a.d_k, j0, 2 * hk + 1), a.d_k.row_stride, keep);
+    }
+    if (P::SPLIT == 1 || share)
+        store_rows<T, PIECE, S::VT, DMA>([&](int t, int r) { return shown ? dv[t][r] : 0.f; }, box, lane, a.Dv, g.aligned, row_out<T>(a.d_v, j0, hk), a.d_v.row_stride, keep);
+}
+
+template <typename T, int DP, bool DMA>
+__global__ __launch_bounds__((Keys<T, DP>::WAVES * 64), (Keys<T, DP>::OCC)) void bwd_keys_kernel(AttnArgs g, int32_t tiles, int32_t row_tiles) {
+    typedef Keys<T, DP> P;
+    __shared__ __align__(16) char s_a[P::BUF];
+    __shared__ __align__(16) char s_b[P::BUF];
+    __shared__ __align__(16) char s_own[P::OWN];
+    __shared__ __align__(8) uint8_t s_marks[2 * P::BQ * (P::RB / 16)];
+    __shared__ int s_lo[P::WAVES], s_hi[P::WAVES], s_bad;
+    const int64_t blocks = ceil_div<int64_t>((int64_t)tiles * g.a.Hk, 8) * 8;
+    if ((int64_t)blockIdx.x >= blocks) sum_lam<P::WAVES * 64>(g, (int)(blockIdx.x - blocks), row_tiles, s_a);
+    else keys_body<T, DP, DMA>(g, tiles, s_a, s_b, s_own, s_marks, s_lo, s_hi, s_bad);
+}
+
+// -------------------------------------------------------------------- owned: keys, rows of 1024 bytes (fp32, heads over 64)
+// Two waves share 32 keys: one sums dK, the other dV, each computes the scores (the sums of both do not fit a wave's
+// registers); keys and values are read from LDS, whose rest holds one tile of rows.
+template <typename T, int DP>
+struct Roles {
+    static constexpr int RB = Shape<T, DP>::RB, WAVES = 2, ROWS = 32, BQ = 32, TILE = 2 * BQ * RB;
+    static constexpr int STAT = BQ * 4 * 4;                     // lse and t of a row, two each
+    static constexpr int BUF = TILE + STAT, OWN = 2 * ROWS * RB;
+};
+
+// DK, DV: what this wave sums
+template <typename T, int DP, bool DMA, bool DK, bool DV>
+__device__ __forceinline__ void roles_body(const AttnArgs& g, int32_t tiles, char* s_a, char* s_own, uint8_t* s_marks, int& s_bad) {
+    typedef Shape<T, DP> S;
+    typedef Roles<T, DP> P;
+    typedef Mat<T> M;
+    constexpr int RB = S::RB, NT = P::WAVES * 64, ROWS = P::ROWS, BQ = P::BQ, TILE = P::TILE, AHEAD = 2;
+    const sgl_diff_attn_args& a = g.a;
+    const int G = a.Hq / a.Hk;
+    const uint32_t n = (uint32_t)tiles * (uint32_t)a.Hk, item = xcd_item(n);
+    if (item >= n) return;
+    // key heads side by side; of a causal call the early keys, which most rows see, come first
+    const int hk = (int)(item % (uint32_t)a.Hk);
+    const int32_t tile = (int32_t)(item / (uint32_t)a.Hk);
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5, col = lane & 31;
+    const int32_t B = (int32_t)live_count(a.B_dev, a.B);
+    const int32_t j0 = tile * ROWS, j = j0 + col;
+    bool shown;
+    int32_t seq;
+    const Span rows = rows_of(a, B, j0, col, shown, seq);
+    // the wave's union, and the run of rows that see all its keys (if it has no key that none sees)
+    Reach reach = reach_of(rows);
+    if (!__all(shown)) reach.to = 0;
+    if (threadIdx.x == 0) s_bad = 0;
+    const int32_t lo = reach.lo, hi = reach.hi;                 // (both waves have the same keys)
+    Stager<T, DP, ROWS, NT, false, true>().load(s_own, halves<T>(a.k, hk, a.D), j0, (int32_t)a.Tk - 1, g.aligned);
+    Stager<T, DP, ROWS, NT, false, false>().load(s_own + ROWS * RB, run<T>(a.v, hk, a.Dv), j0, (int32_t)a.Tk - 1, g.aligned);
     f32x16 dk[2][S::DT], dv[S::VT];
     auto clear = [&]() {
 #pragma unroll
@@ -331,7 +676,7 @@ __device__ __forceinline__ void kv_body(const AttnArgs& g, int32_t tiles, char* 
     const int32_t per_head = lo < hi ? (hi - lo + BQ - 1) / BQ : 0, steps = per_head * G;      // head by head, row tile by row tile
     auto load_stats = [&](char* buf, int h, int32_t i0) {
         // 64 numbers each: (lse_1, lse_2) and (t_1, t_2) of the rows
-        if (wave < 2) {
+        {
             const int32_t i = min(i0 + (lane >> 1), last);
             const float* src = (wave ? g.delta : a.lse) + ((int64_t)i * a.Hq + h) * 2 + (lane & 1);
             const int at0 = __builtin_amdgcn_readfirstlane(wave * 256);
@@ -365,21 +710,16 @@ __device__ __forceinline__ void kv_body(const AttnArgs& g, int32_t tiles, char* 
             return n < 2 * S::QS ? row_frag<T, RB>(buf, 0, col, n, half) : row_frag<T, RB>(buf + BQ * RB, 0, col, n - 2 * S::QS, half);
         };
         auto load_own = [&](int n) {
-            return n < 2 * S::QS ? row_frag<T, RB>(s_own, group * 32, col, n, half) : row_frag<T, RB>(s_own + ROWS * RB, group * 32, col, n - 2 * S::QS, half);
+            return n < 2 * S::QS ? row_frag<T, RB>(s_own, 0, col, n, half) : row_frag<T, RB>(s_own + ROWS * RB, 0, col, n - 2 * S::QS, half);
         };
-        constexpr int FRAGS = 2 * S::QS + (DK ? S::VS : 0), FROM_LDS = S::KEY_REGS ? 0 : S::VAL_REGS ? 2 * S::QS : FRAGS;
-        Pipe<T, FRAGS, AHEAD> ahead;
-        Pipe<T, FROM_LDS, AHEAD> own;
-        if constexpr (FROM_LDS > 0) own.fill(load_own);
+        constexpr int FRAGS = 2 * S::QS + (DK ? S::VS : 0);
+        Pipe<T, FRAGS, AHEAD> ahead, own;
+        own.fill(load_own);
         ahead.fill(load_row);
         ahead.drain(load_row, [&](int n, const typename M::Frag& f) {
             f32x16& to = n < S::QS ? s[0] : n < 2 * S::QS ? s[1] : dp;
-            if (n < FROM_LDS) {
-                to = M::mma(f, own.f[n % AHEAD], to);
-                if (n + AHEAD < FROM_LDS) own.f[n % AHEAD] = load_own(n + AHEAD);
-            } else {
-                to = M::mma(f, n < 2 * S::QS ? k[n / S::QS % 2][n % S::QS] : v[n < 2 * S::QS ? 0 : n - 2 * S::QS], to);
-            }
+            to = M::mma(f, own.f[n % AHEAD], to);
+            if (n + AHEAD < FRAGS) own.f[n % AHEAD] = load_own(n + AHEAD);
         });
         f32x16 x;               // P_1 - lam P_2
 #pragma unroll
@@ -410,16 +750,16 @@ __device__ __forceinline__ void kv_body(const AttnArgs& g, int32_t tiles, char* 
                 if constexpr (DV) x[r] = row_bit(see, r) ? x[r] : 0.f;
             }
         }
-        if constexpr (DV) add_product<T, RB, S::VT, AHEAD>(dv, buf + BQ * RB, 0, 0, x, lane);
+        if constexpr (DV) add_product<T, RB, S::VT, AHEAD>(dv, buf + BQ * RB, 0, 0, operand<T>(x), lane);
         if constexpr (DK) {
-            add_map<T, RB, S::DT, AHEAD>(dk[0], buf, 0, 0, s[0], lane);
-            add_map<T, RB, S::DT, AHEAD>(dk[1], buf, 0, 1, s[1], lane);
+            add_map<T, RB, S::DT, AHEAD>(dk[0], buf, 0, 0, operand<T>(s[0]), lane);
+            add_map<T, RB, S::DT, AHEAD>(dk[1], buf, 0, 1, operand<T>(s[1]), lane);
         }
     };
     bool spoilt[2] = {false, false};        // a row with something not finite sees the key: NaN
     if (steps > 0) {
-        int h, hn;                          // head and first row of the tile at work, and of the one being loaded
-        int32_t i0, in;
+        int hn;                             // head and first row of the tile
+        int32_t in;
         auto next = [&]() {
             in += BQ;
             if (in >= hi) in = lo, ++hn;
@@ -429,30 +769,13 @@ __device__ __forceinline__ void kv_body(const AttnArgs& g, int32_t tiles, char* 
             hn = hk * G, in = lo;
             load(s_a, hn, in);
             staged();
-            if constexpr (S::TWO) {
 #pragma unroll 1
-                for (int32_t s = 0; s < steps; s += 2) {
-                    h = hn, i0 = in;
-                    next();
-                    if (s + 1 < steps) load(s_b, hn, in);
-                    step(s_a, h, i0);
-                    staged();
-                    if (s + 1 >= steps) break;
-                    h = hn, i0 = in;
-                    next();
-                    if (s + 2 < steps) load(s_a, hn, in);
-                    step(s_b, h, i0);
-                    staged();
-                }
-            } else {
-#pragma unroll 1
-                for (int32_t s = 0; s < steps; ++s) {
-                    step(s_a, hn, in);
-                    __syncthreads();
-                    next();
-                    if (s + 1 < steps) load(s_a, hn, in);
-                    staged();
-                }
+            for (int32_t s = 0; s < steps; ++s) {
+                step(s_a, hn, in);
+                __syncthreads();
+                next();
+                if (s + 1 < steps) load(s_a, hn, in);
+                staged();
             }
             if (finite) break;
             bool bad = false;
@@ -491,8 +814,8 @@ __device__ __forceinline__ void kv_body(const AttnArgs& g, int32_t tiles, char* 
     }
     const uint32_t keep = (uint32_t)__ballot(j < a.Tk && (seq >= 0 || (a.flags & SGL_ATTN_ZERO_REST)));
     // the walked side's tiles are free: the last barrier is behind every wave's last look at them
-    char* box = s_a + wave * (TILE / S::K_WAVES);
-    constexpr int PIECE = TILE / S::K_WAVES / 32;               // bytes of a row at a time
+    char* box = s_a + wave * (TILE / P::WAVES);
+    constexpr int PIECE = TILE / P::WAVES / 32;               // bytes of a row at a time
     if constexpr (DK) {
         store_rows<T, PIECE, S::DT, DMA>([&](int t, int r) { return spoilt[0] ? NAN : shown ? dk[0][t][r] * g.scale : 0.f; }, box, lane, a.D, g.aligned,
                                          row_out<T>(a.d_k, j0, 2 * hk), a.d_k.row_stride, keep);
@@ -504,53 +827,43 @@ __device__ __forceinline__ void kv_body(const AttnArgs& g, int32_t tiles, char* 
 }
 
 template <typename T, int DP, bool DMA>
-__global__ __launch_bounds__((Shape<T, DP>::K_WAVES * 64), (Shape<T, DP>::K_OCC)) void bwd_kv_kernel(AttnArgs g, int32_t tiles, int32_t row_tiles) {
-    typedef Shape<T, DP> S;
-    constexpr int RB = S::RB, NT = S::K_WAVES * 64, BUF = KvSmem<T, DP>::TILE + KvSmem<T, DP>::STAT;
-    __shared__ __align__(16) char s_a[BUF];
-    __shared__ __align__(16) char s_b[S::TWO ? BUF : 16];
-    __shared__ __align__(16) char s_own[S::OWN ? S::K_ROWS * S::OWN : 16];
-    __shared__ __align__(8) uint8_t s_marks[2 * KvSmem<T, DP>::BQ * (RB / 16)];
-    __shared__ int s_lo[S::K_WAVES], s_hi[S::K_WAVES], s_bad;
+__global__ __launch_bounds__((Roles<T, DP>::WAVES * 64), 1) void bwd_roles_kernel(AttnArgs g, int32_t tiles, int32_t row_tiles) {
+    typedef Roles<T, DP> P;
+    __shared__ __align__(16) char s_a[P::BUF];
+    __shared__ __align__(16) char s_own[P::OWN];
+    __shared__ __align__(8) uint8_t s_marks[2 * P::BQ * (P::RB / 16)];
+    __shared__ int s_bad;
     const int64_t blocks = ceil_div<int64_t>((int64_t)tiles * g.a.Hk, 8) * 8;
-    if ((int64_t)blockIdx.x >= blocks) {
-        // the last Hq blocks: d_lam of a head
-        float* s_sum = reinterpret_cast<float*>(s_a);
-        const int h = (int)(blockIdx.x - blocks);
-        float x = 0.f;
-        for (int k = threadIdx.x; k < row_tiles; k += NT) x += g.lam_part[(int64_t)k * g.a.Hq + h];
-        s_sum[threadIdx.x] = x;
-        __syncthreads();
-        if (threadIdx.x == 0) {
-            float y = 0.f;
-            for (int k = 0; k < NT; ++k) y += s_sum[k];
-            g.a.d_lam[h] = -y;
-        }
-        return;
-    }
-    if constexpr (S::ROLES) {
-        // (the waves of a SIMD take both roles: waves go to the four SIMDs in turn)
-        if (((int)(threadIdx.x >> 6) < S::K_WAVES / 2) == (S::K_WAVES > 4 || (blockIdx.x >> 3) % 2 == 0)) kv_body<T, DP, DMA, true, false>(g, tiles, s_a, s_b, s_own, s_marks, s_lo, s_hi, s_bad);
-        else kv_body<T, DP, DMA, false, true>(g, tiles, s_a, s_b, s_own, s_marks, s_lo, s_hi, s_bad);
-    } else {
-        kv_body<T, DP, DMA, true, true>(g, tiles, s_a, s_b, s_own, s_marks, s_lo, s_hi, s_bad);
-    }
+    if ((int64_t)blockIdx.x >= blocks) return sum_lam<P::WAVES * 64>(g, (int)(blockIdx.x - blocks), row_tiles, s_a);
+    // (the waves of a SIMD take both roles: waves go to the four SIMDs in turn)
+    if (((int)(threadIdx.x >> 6) == 0) == ((blockIdx.x >> 3) % 2 == 0)) roles_body<T, DP, DMA, true, false>(g, tiles, s_a, s_own, s_marks, s_bad);
+    else roles_body<T, DP, DMA, false, true>(g, tiles, s_a, s_own, s_marks, s_bad);
 }
 
 template <typename T, int DP>
 void launch(const AttnArgs& g, hipStream_t st) {
     const sgl_diff_attn_args& a = g.a;
     typedef Shape<T, DP> S;
-    const int32_t qt = (int32_t)ceil_div<int64_t>(a.Tq, S::Q_ROWS), kt = (int32_t)ceil_div<int64_t>(a.Tk, S::K_ROWS);
+    const int32_t qt = (int32_t)ceil_div<int64_t>(a.Tq, S::Q_ROWS);
     const bool dma = g.aligned && a.D == DP && a.Dv == 2 * DP && dma_rows(a.k) && dma_rows(a.v) && dma_rows(a.q) && dma_rows(a.d_out);
     if (qt > 0) {
         const dim3 grid((unsigned)(ceil_div<int64_t>((int64_t)qt * a.Hq, 8) * 8)), block(S::Q_WAVES * 64);
         if (dma) hipLaunchKernelGGL((bwd_q_kernel<T, DP, true>), grid, block, 0, st, g, qt);
         else hipLaunchKernelGGL((bwd_q_kernel<T, DP, false>), grid, block, 0, st, g, qt);
     }
-    const dim3 grid((unsigned)(ceil_div<int64_t>((int64_t)kt * a.Hk, 8) * 8 + a.Hq)), block(S::K_WAVES * 64);
-    if (dma) hipLaunchKernelGGL((bwd_kv_kernel<T, DP, true>), grid, block, 0, st, g, kt, qt);
-    else hipLaunchKernelGGL((bwd_kv_kernel<T, DP, false>), grid, block, 0, st, g, kt, qt);
+    if constexpr (S::RB <= 512) {
+        typedef Keys<T, DP> P;
+        const int32_t kt = (int32_t)ceil_div<int64_t>(a.Tk, P::ROWS);
+        const dim3 grid((unsigned)(ceil_div<int64_t>((int64_t)kt * a.Hk, 8) * 8 + a.Hq)), block(P::WAVES * 64);
+        if (dma) hipLaunchKernelGGL((bwd_keys_kernel<T, DP, true>), grid, block, 0, st, g, kt, qt);
+        else hipLaunchKernelGGL((bwd_keys_kernel<T, DP, false>), grid, block, 0, st, g, kt, qt);
+    } else {
+        typedef Roles<T, DP> P;
+        const int32_t kt = (int32_t)ceil_div<int64_t>(a.Tk, P::ROWS);
+        const dim3 grid((unsigned)(ceil_div<int64_t>((int64_t)kt * a.Hk, 8) * 8 + a.Hq)), block(P::WAVES * 64);
+        if (dma) hipLaunchKernelGGL((bwd_roles_kernel<T, DP, true>), grid, block, 0, st, g, kt, qt);
+        else hipLaunchKernelGGL((bwd_roles_kernel<T, DP, false>), grid, block, 0, st, g, kt, qt);
+    }
 }
 
 }  // namespace
