@@ -91,8 +91,7 @@ size_t forward_need(const sgl_diff_attn_args& a, int32_t parts) {
     return parts > 1 ? align_up(n * 2 * sizeof(float)) + align_up(n * (size_t)a.Dv * sizeof(float)) : 0;
 }
 
-// query rows of a block of the backward kernels
-int64_t backward_row_tiles(const sgl_diff_attn_args& a) { return ceil_div<int64_t>(a.Tq, a.dtype == SGL_DT_F32 && heads_width(a) <= 64 ? 64 : 128); }
+int64_t backward_row_tiles(const sgl_diff_attn_args& a) { return ceil_div<int64_t>(a.Tq, QUERY_ROWS); }
 size_t backward_need(const sgl_diff_attn_args& a) {
     if (!a.q_ptr) return align_up((size_t)seg_blocks(a) * (size_t)a.Hq * sizeof(float));
     return align_up((size_t)a.Tq * (size_t)a.Hq * 2 * sizeof(float)) +

@@ -13,6 +13,8 @@ constexpr int BLOCK = 256;
 constexpr float NEG_INF = -INFINITY;
 constexpr float LOG2E = 1.44269504088896340736f;
 
+constexpr int QUERY_ROWS = 128;     // query rows of a block of the backward pass (a sum of t_2 in the workspace each)
+
 struct AttnArgs {
     sgl_diff_attn_args a;
     float scale;                // of the scores

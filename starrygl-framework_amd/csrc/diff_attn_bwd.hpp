@@ -20,8 +20,6 @@ struct Shape {
     static constexpr int QS = DP / (2 * EP);                    // steps over a half of a head
     static constexpr int VS = 2 * QS;                           // steps over the values
     static constexpr int DT = DP / 32, VT = 2 * DP / 32;        // 32-wide tiles of a half, of the values
-    // query side: a wave per 32 rows and map, eight to a block while the registers of two a SIMD hold their operands
-    static constexpr int Q_WAVES = RB > 256 ? (RB > 512 ? 4 : 8) : 4, Q_ROWS = Q_WAVES / 2 * 32, Q_OCC = RB <= 256 ? 3 : RB <= 512 ? 2 : 1;
 };
 
 __device__ __forceinline__ float signed_c2(const AttnArgs& g) { return g.scale < 0.f ? -g.c2 : g.c2; }
@@ -92,17 +90,26 @@ __device__ __forceinline__ void add_map(f32x16 (&acc)[N], const char* tile, int 
 }
 
 // ---------------------------------------------------------------------------------------------- owned: query rows
+// A wave owns 32 rows of a head: both maps' scores, dP and dQ of a tile of 32 keys, the products between the vector
+// instructions of the phase before, as above.
+template <typename T, int DP>
+struct Rows {
+    static constexpr int RB = Shape<T, DP>::RB, WAVES = 4, ROWS = QUERY_ROWS, OCC = RB <= 256 ? 2 : 1, AHEAD = RB <= 256 ? 2 : 4;
+    static constexpr int BN = RB <= 512 ? 64 : 32, TILE = 2 * BN * RB;
+    static_assert(ROWS == WAVES * 32, "the row tiles of the workspace");
+};
+
 template <typename T, int DP, bool DMA>
-__global__ __launch_bounds__((Shape<T, DP>::Q_WAVES * 64), (Shape<T, DP>::Q_OCC)) void bwd_q_kernel(AttnArgs g, int32_t tiles) {
+__global__ __launch_bounds__((Rows<T, DP>::WAVES * 64), (Rows<T, DP>::OCC)) void bwd_rows_kernel(AttnArgs g, int32_t tiles) {
     typedef Shape<T, DP> S;
+    typedef Rows<T, DP> P;
     typedef Mat<T> M;
-    constexpr int RB = S::RB, NT = S::Q_WAVES * 64, GROUPS = S::Q_WAVES / 2, AHEAD = 2;
-    constexpr int BN = RB <= 128 ? 64 : 32, TILE = 2 * BN * RB;
-    __shared__ __align__(16) char s_a[TILE];
-    __shared__ __align__(16) char s_b[TILE];
+    constexpr int RB = S::RB, NT = P::WAVES * 64, BN = P::BN, AHEAD = P::AHEAD;
+    __shared__ __align__(16) char s_a[P::TILE];
+    __shared__ __align__(16) char s_b[P::TILE];
     __shared__ __align__(8) uint8_t s_marks[2 * BN * (RB / 16)];
-    __shared__ int s_lo[GROUPS], s_hi[GROUPS], s_bad;
-    __shared__ float s_lam[GROUPS];
+    __shared__ int s_lo[P::WAVES], s_hi[P::WAVES], s_bad;
+    __shared__ float s_lam[P::WAVES];
     const sgl_diff_attn_args& a = g.a;
     const int G = a.Hq / a.Hk;
     const uint32_t n = (uint32_t)tiles * (uint32_t)a.Hq, item = xcd_item(n);
@@ -112,10 +119,9 @@ __global__ __launch_bounds__((Shape<T, DP>::Q_WAVES * 64), (Shape<T, DP>::Q_OCC)
     const int hk = (int)(rest / (uint32_t)tiles), h = hk * G + hg;
     int32_t tile = (int32_t)(rest % (uint32_t)tiles);
     if (a.causal) tile = tiles - 1 - tile;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5, col = lane & 31;
-    const int map = wave & 1, group = wave >> 1;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5, col = lane & 31;
     const int32_t B = (int32_t)live_count(a.B_dev, a.B);
-    const int32_t i0 = tile * S::Q_ROWS + group * 32, i = i0 + col;
+    const int32_t i0 = tile * P::ROWS + wave * 32, i = i0 + col;
     const int32_t at[1] = {col};
     int32_t found[1];
     find_seqs<1>(a.q_ptr, B, i0, at, found);
@@ -124,49 +130,55 @@ __global__ __launch_bounds__((Shape<T, DP>::Q_WAVES * 64), (Shape<T, DP>::Q_OCC)
     const bool live = span.lo < span.hi;
     Reach reach = reach_of(span);
     if (a.key_mask) reach.to = 0;
-    if (lane == 0 && map == 0) s_lo[group] = reach.lo, s_hi[group] = reach.hi;
+    if (lane == 0) s_lo[wave] = reach.lo, s_hi[wave] = reach.hi;
     if (threadIdx.x == 0) s_bad = 0;
     __syncthreads();
     int32_t lo = s_lo[0], hi = s_hi[0];
 #pragma unroll
-    for (int w = 1; w < GROUPS; ++w) lo = min(lo, s_lo[w]), hi = max(hi, s_hi[w]);
+    for (int w = 1; w < P::WAVES; ++w) lo = min(lo, s_lo[w]), hi = max(hi, s_hi[w]);
 
     // t_m = sum over the values of d_out * o_m, with o_1 = out + lam o_2
     const float lam = a.lam[h];
-    typename M::Frag q[S::QS], go[S::VS];
-    float t = 0.f;
+    typename M::Frag q[2][S::QS], go[S::VS];
+    float t[2] = {0.f, 0.f};
     const int64_t ii = i < a.Tq ? i : 0;
 #pragma unroll
-    for (int k = 0; k < S::QS; ++k) q[k] = global_frag<T, DMA>(row<T>(a.q, ii, 2 * h + map), (2 * k + half) * S::EP, a.D, g.aligned);
+    for (int m = 0; m < 2; ++m)
+#pragma unroll
+        for (int k = 0; k < S::QS; ++k) q[m][k] = global_frag<T, DMA>(row<T>(a.q, ii, 2 * h + m), (2 * k + half) * S::EP, a.D, g.aligned);
 #pragma unroll
     for (int k = 0; k < S::VS; ++k) {
         const int e = (2 * k + half) * S::EP;
         go[k] = global_frag<T, DMA>(row<T>(a.d_out, ii, h), e, a.Dv, g.aligned);
         const typename M::Frag y2 = global_frag<T, DMA>(row<T>(a.o2, ii, h), e, a.Dv, g.aligned);
-        if (map == 0) {
-            const typename M::Frag y = global_frag<T, DMA>(row<T>(a.out, ii, h), e, a.Dv, g.aligned);
+        const typename M::Frag y = global_frag<T, DMA>(row<T>(a.out, ii, h), e, a.Dv, g.aligned);
 #pragma unroll
-            for (int j = 0; j < S::EP; ++j) t = __builtin_fmaf((float)go[k][j], __builtin_fmaf(lam, (float)y2[j], (float)y[j]), t);
-        } else {
-#pragma unroll
-            for (int j = 0; j < S::EP; ++j) t = __builtin_fmaf((float)go[k][j], (float)y2[j], t);
+        for (int j = 0; j < S::EP; ++j) {
+            t[0] = __builtin_fmaf((float)go[k][j], __builtin_fmaf(lam, (float)y2[j], (float)y[j]), t[0]);
+            t[1] = __builtin_fmaf((float)go[k][j], (float)y2[j], t[1]);
         }
     }
-    t = half_sum(t);
-    const float lse = live ? a.lse[(i * a.Hq + h) * 2 + map] : INFINITY;
-    if (i < a.Tq && half == 0) g.delta[(i * a.Hq + h) * 2 + map] = t;
+    float lse[2];
+#pragma unroll
+    for (int m = 0; m < 2; ++m) {
+        t[m] = half_sum(t[m]);
+        lse[m] = live ? a.lse[(i * a.Hq + h) * 2 + m] : INFINITY;
+    }
+    if (i < a.Tq && half == 0) g.delta[(i * a.Hq + h) * 2] = t[0], g.delta[(i * a.Hq + h) * 2 + 1] = t[1];
 
     const Source ks = halves<T>(a.k, hk, a.D), vs = run<T>(a.v, hk, a.Dv);
     const int32_t last = (int32_t)a.Tk - 1;
-    f32x16 dq[S::DT];
-    float sum = 0.f;            // sum of P dP: of the second map -d_lam's share
+    f32x16 dq[2][S::DT];
+    float sum = 0.f;            // sum of P_2 dP: -d_lam's share
     auto clear = [&]() {
         sum = 0.f;
 #pragma unroll
-        for (int d = 0; d < S::DT; ++d) dq[d] = zero16();
+        for (int m = 0; m < 2; ++m)
+#pragma unroll
+            for (int d = 0; d < S::DT; ++d) dq[m][d] = zero16();
     };
     clear();
-    const float c2 = signed_c2(g);
+    const float c2 = __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(signed_c2(g))));
     Stager<T, DP, BN, NT, DMA, true> stage_k;
     Stager<T, DP, BN, NT, DMA, false> stage_v;
     stage_k.plan(ks);
@@ -181,38 +193,83 @@ __global__ __launch_bounds__((Shape<T, DP>::Q_WAVES * 64), (Shape<T, DP>::Q_OCC)
             stage_v.load(buf + BN * RB, vs, j, last, g.aligned);
         }
     };
+    // (the lane's parts of the addresses, as of the keys' kernel)
+    int32_t by_row[4], by_col[2];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        by_row[e] = lane_row<RB>(col, e, half);
+        asm volatile("" : "+v"(by_row[e]));
+    }
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+        by_col[e] = lane_col<T, RB>(e, lane);
+        asm volatile("" : "+v"(by_col[e]));
+    }
+    auto of_row = [](const char* base, const int32_t (&by)[4], int k) { return *reinterpret_cast<const typename M::Frag*>(base + (k >> 2) * 1024 + by[k & 3]); };
     auto work = [&](const char* buf, int32_t j) {
 #pragma unroll
         for (int sub = 0; sub < BN / 32; ++sub) {
             const int32_t j0 = j + sub * 32;
             if (j0 >= reach.hi || j0 + 32 <= reach.lo) continue;
-            f32x16 s = zero16(), dp = zero16();
-            auto load_row = [&](int n) {
-                return n < S::QS ? map_frag<T, RB>(buf, sub * 32, col, map, n, half) : row_frag<T, RB>(buf + BN * RB, sub * 32, col, n - S::QS, half);
+            constexpr int PS = Operand<T>::PS, QS = S::QS, NK = S::DT * PS, N1 = QS, N2 = 2 * QS, N3 = N2 + S::VS, N4 = N3 + NK, N5 = N4 + NK;
+            const char* kt = buf + sub * 32 * RB;
+            const char* vt = buf + (BN + sub * 32) * RB;
+            const bool some = !(j0 >= reach.from && j0 + 32 <= reach.to);
+            uint32_t see = 0;
+            if (some) see = (span_bits(j0, span) & mask_bits(a.key_mask, j0, lane, last)) >> (4 * half);
+            auto hide = [&](f32x16& x) {
+                uint32_t bits = see;
+                asm volatile("" : "+v"(bits));
+#pragma unroll
+                for (int r = 0; r < 16; ++r) x[r] = row_bit(bits, r) ? x[r] : 0.f;
             };
-            Pipe<T, S::QS + S::VS, AHEAD> ahead;
-            ahead.fill(load_row);
-            ahead.drain(load_row, [&](int n, const typename M::Frag& f) {
-                if (n < S::QS) s = M::mma(f, q[n < S::QS ? n : 0], s);
-                else dp = M::mma(f, go[n < S::QS ? 0 : n - S::QS], dp);
+            f32x16 s[2], dp;
+            s[0] = s[1] = dp = zero16();
+            Operand<T> ds[2];
+            auto load_n = [&](int n) {
+                if (n < N2) return of_row(kt, by_row, n);
+                if (n < N3) return of_row(vt, by_row, n - N2);
+                const int m = n < N4 ? 0 : 1, u = n - (m ? N4 : N3);
+                return col_at<T, RB>(kt, by_col, 0, u / S::DT, m * S::DT + u % S::DT);
+            };
+            auto exps = [&](int m, int r) {
+#pragma unroll
+                for (int e = r; e < r + 2; ++e) s[m][e] = exp2_hw(__builtin_fmaf(s[m][e], c2, -lse[m]));
+            };
+            auto scores = [&](int m, int r) { ds[m].set2(r, s[m][r] * (dp[r] - t[m]), s[m][r + 1] * (dp[r + 1] - t[m])); };
+            Pipe<T, N5, AHEAD> ahead;
+            ahead.fill(load_n);
+            ahead.template part<0, N1>(load_n, [&](int n, const typename M::Frag& x) { s[0] = M::mma(x, q[0][n], s[0]); });
+            ahead.template part<N1, N2>(load_n, [&](int n, const typename M::Frag& x) {
+                s[1] = M::mma(x, q[1][n - N1], s[1]);
+#pragma unroll
+                for (int r = 8 * (n - N1) / QS * 2; r < 8 * (n - N1 + 1) / QS * 2; r += 2) exps(0, r);
             });
-            if (!(j0 >= reach.from && j0 + 32 <= reach.to)) {
-                // (the score's product with c2 becomes -inf, whatever c2's sign)
-                const float hidden = c2 < 0.f ? INFINITY : NEG_INF;
-                const uint32_t see = (span_bits(j0, span) & mask_bits(a.key_mask, j0, lane, last)) >> (4 * half);
+            ahead.template part<N2, N3>(load_n, [&](int n, const typename M::Frag& x) {
+                dp = M::mma(x, go[n - N2], dp);
 #pragma unroll
-                for (int r = 0; r < 16; ++r) s[r] = row_bit(see, r) ? s[r] : hidden, dp[r] = row_bit(see, r) ? dp[r] : 0.f;
-            }
+                for (int r = 8 * (n - N2) / S::VS * 2; r < 8 * (n - N2 + 1) / S::VS * 2; r += 2) exps(1, r);
+            });
+            if (some) hide(s[0]), hide(s[1]);
 #pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                const float p = exp2_hw(__builtin_fmaf(s[r], c2, -lse));
-                sum = __builtin_fmaf(p, dp[r], sum);
-                s[r] = p * (dp[r] - t);            // (the second map's times -lam at the end)
-            }
-            add_map<T, RB, S::DT, AHEAD>(dq, buf, sub * 32, map, operand<T>(s), lane);
+            for (int r = 0; r < 16; r += 2) scores(0, r);
+            ahead.template part<N3, N4>(load_n, [&](int n, const typename M::Frag& x) {
+                const int u = n - N3;
+                dq[0][u % S::DT] = M::mma(x, ds[0].f[u / S::DT], dq[0][u % S::DT]);
+#pragma unroll
+                for (int r = 8 * u / NK * 2; r < 8 * (u + 1) / NK * 2; r += 2) {
+                    sum = __builtin_fmaf(s[1][r], dp[r], sum);
+                    sum = __builtin_fmaf(s[1][r + 1], dp[r + 1], sum);
+                    scores(1, r);           // (times -lam at the end)
+                }
+            });
+            ahead.template part<N4, N5>(load_n, [&](int n, const typename M::Frag& x) {
+                const int u = n - N4;
+                dq[1][u % S::DT] = M::mma(x, ds[1].f[u / S::DT], dq[1][u % S::DT]);
+            });
         }
     };
-    bool spoilt = false;        // the query sees something not finite: NaN
+    bool spoilt[2] = {false, false};        // the query sees something not finite: NaN
     if (lo < hi) {
 #pragma unroll 1
         for (;;) {
@@ -229,7 +286,7 @@ __global__ __launch_bounds__((Shape<T, DP>::Q_WAVES * 64), (Shape<T, DP>::Q_OCC)
                 staged();
             }
             if (finite) break;
-            if ((any_nan(dq) || sum != sum) && live) s_bad = 1;
+            if ((any_nan(dq[0]) || any_nan(dq[1]) || sum != sum) && live) s_bad = 1;
             __syncthreads();
             if (!s_bad) break;
             finite = true;
@@ -246,27 +303,33 @@ __global__ __launch_bounds__((Shape<T, DP>::Q_WAVES * 64), (Shape<T, DP>::Q_OCC)
 #pragma unroll 1
                 for (int r = 0; r < BN && j + r < hi; ++r) {
                     if (!sees(j + r, span, a.key_mask)) continue;
-                    spoilt = spoilt || marked_any<RB>(s_marks + BN * (RB / 16), r, 0, RB / 16) || marked_any<RB>(s_marks, r, map * (RB / 32), (map + 1) * (RB / 32));
+                    const bool o = marked_any<RB>(s_marks + BN * (RB / 16), r, 0, RB / 16);
+                    spoilt[0] = spoilt[0] || o || marked_any<RB>(s_marks, r, 0, RB / 32);
+                    spoilt[1] = spoilt[1] || o || marked_any<RB>(s_marks, r, RB / 32, RB / 16);
                 }
             }
-            if (spoilt) sum = NAN;
+            if (spoilt[1]) sum = NAN;
         }
     }
     float share = live ? sum : 0.f;
 #pragma unroll
     for (int m = 1; m < 64; m <<= 1) share += __shfl_xor(share, m);
-    if (lane == 0 && map == 1) s_lam[group] = share;
+    if (lane == 0) s_lam[wave] = share;
     __syncthreads();
     if (threadIdx.x == 0) {
         float x = 0.f;
-        for (int w = 0; w < GROUPS; ++w) x += s_lam[w];
+        for (int w = 0; w < P::WAVES; ++w) x += s_lam[w];
         g.lam_part[(int64_t)tile * a.Hq + h] = x;
     }
     const uint32_t keep = (uint32_t)__ballot(i < a.Tq && (seq >= 0 || (a.flags & SGL_ATTN_ZERO_REST)));
-    const float scale = map ? -lam * g.scale : g.scale;
     // (every wave's last look at the tiles lies before the barrier above)
-    store_rows<T, RB / 2, S::DT, DMA>([&](int t, int r) { return spoilt ? NAN : live ? dq[t][r] * scale : 0.f; }, (wave < S::Q_WAVES / 2 ? s_a : s_b) + wave % (S::Q_WAVES / 2) * 16 * RB, lane, a.D,
-                                      g.aligned, row_out<T>(a.d_q, i0, 2 * h + map), a.d_q.row_stride, keep);
+    char* box = (wave & 1 ? s_b : s_a) + (wave >> 1) * (P::TILE / 2);
+    constexpr int PIECE = RB / 2;                               // bytes of a row at a time
+    const float f0 = g.scale, f1 = -lam * g.scale;
+    store_rows<T, PIECE, S::DT, DMA>([&](int d, int r) { return spoilt[0] ? NAN : live ? dq[0][d][r] * f0 : 0.f; }, box, lane, a.D, g.aligned, row_out<T>(a.d_q, i0, 2 * h),
+                                     a.d_q.row_stride, keep);
+    store_rows<T, PIECE, S::DT, DMA>([&](int d, int r) { return spoilt[1] ? NAN : live ? dq[1][d][r] * f1 : 0.f; }, box, lane, a.D, g.aligned, row_out<T>(a.d_q, i0, 2 * h + 1),
+                                     a.d_q.row_stride, keep);
 }
 
 // the query rows that may see key j0 + col, and its sequence; shown: some do
@@ -844,12 +907,12 @@ template <typename T, int DP>
 void launch(const AttnArgs& g, hipStream_t st) {
     const sgl_diff_attn_args& a = g.a;
     typedef Shape<T, DP> S;
-    const int32_t qt = (int32_t)ceil_div<int64_t>(a.Tq, S::Q_ROWS);
+    const int32_t qt = (int32_t)ceil_div<int64_t>(a.Tq, QUERY_ROWS);
     const bool dma = g.aligned && a.D == DP && a.Dv == 2 * DP && dma_rows(a.k) && dma_rows(a.v) && dma_rows(a.q) && dma_rows(a.d_out);
     if (qt > 0) {
-        const dim3 grid((unsigned)(ceil_div<int64_t>((int64_t)qt * a.Hq, 8) * 8)), block(S::Q_WAVES * 64);
-        if (dma) hipLaunchKernelGGL((bwd_q_kernel<T, DP, true>), grid, block, 0, st, g, qt);
-        else hipLaunchKernelGGL((bwd_q_kernel<T, DP, false>), grid, block, 0, st, g, qt);
+        const dim3 grid((unsigned)(ceil_div<int64_t>((int64_t)qt * a.Hq, 8) * 8)), block(Rows<T, DP>::WAVES * 64);
+        if (dma) hipLaunchKernelGGL((bwd_rows_kernel<T, DP, true>), grid, block, 0, st, g, qt);
+        else hipLaunchKernelGGL((bwd_rows_kernel<T, DP, false>), grid, block, 0, st, g, qt);
     }
     if constexpr (S::RB <= 512) {
         typedef Keys<T, DP> P;

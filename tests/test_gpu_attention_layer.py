@@ -188,3 +188,31 @@ def test_steps_on_two_streams_at_once(hot):
     torch.cuda.synchronize()
     for (y0, g0), (y1, g1) in zip(want, got):
         assert torch.equal(y0, y1) and all(torch.equal(a, b) for a, b in zip(g0, g1))
+
+
+@pytest.mark.parametrize("dtype,D", [(torch.float32, 32), (torch.float32, 64), (torch.float32, 128), (torch.bfloat16, 32), (torch.float16, 64), (torch.bfloat16, 128)])
+@pytest.mark.parametrize("one_query", [False, True])
+def test_workspaces_are_kept_to(hot, monkeypatch, one_query, dtype, D):
+    """the bytes behind a workspace of the size that the library names stay as they were"""
+    kept = []
+
+    def scratch(n):
+        ws = torch.full((int(n) + (1 << 16),), 171, dtype=torch.uint8, device="cuda")
+        kept.append((ws, int(n)))
+        return ws
+
+    monkeypatch.setattr(hot, "_scratch", scratch)
+    g = torch.Generator().manual_seed(3)
+    r = lambda *s: torch.randn(*s, generator=g).to(dtype).cuda()  # noqa: E731
+    B, nk = 5, 700
+    nq = 1 if one_query else nk
+    q, k, v, go, lam = r(B * nq, 8, D), r(B * nk, 4, D), r(B * nk, 2, 2 * D), r(B * nq, 4, 2 * D), torch.rand(4, generator=g).cuda()
+    k_ptr = torch.arange(0, B * nk + 1, nk).cuda()
+    q_ptr = None if one_query else k_ptr
+    lse, o2 = torch.empty(B * nq, 4, 2, device="cuda"), torch.empty_like(go)
+    out = hot.diff_attn(q, k, v, lam, k_ptr, q_ptr, lse=lse, o2=o2)
+    hot.diff_attn_backward(go, q, k, v, lam, out, lse, o2, k_ptr, q_ptr)
+    w = torch.rand(D, device="cuda")
+    sides = [dict(x=t, y=t.clone(), dx=torch.empty_like(t), pos=None, weight=w, dweight=torch.empty_like(w)) for t in (q, k)]
+    hot.qk_norm_rotary_backward(sides, None)
+    assert kept and all((ws[n:] == 171).all() for ws, n in kept)
