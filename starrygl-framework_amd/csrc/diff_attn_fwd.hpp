@@ -23,7 +23,7 @@ struct Shape {
     static constexpr int RB = 2 * DP * (int)sizeof(T);          // bytes of a staged row, of keys and of values
     static constexpr int MAPS = !HEADS && RB <= 256 ? 2 : 1;    // of a wave
     static constexpr int WAVES = HEADS || MAPS == 2 ? 4 : 8, GROUPS = WAVES * MAPS / 2, NT = WAVES * 64;
-    static constexpr int BN = RB <= (HEADS ? 256 : 128) ? 64 : 32;      // keys of a tile
+    static constexpr int BN = RB <= 256 ? 64 : 32;    // keys of a tile
     static constexpr int TILE = 2 * BN * RB;
     static constexpr int EP = Mat<T>::EP;
     static constexpr int QS = DP / (2 * EP);                    // steps over a half of a head
