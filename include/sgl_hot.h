@@ -792,10 +792,12 @@ int32_t sgl_qk_norm_rotary_backward(const sgl_rotary_params* p, double eps, int3
  *   !causal, or i + nk - nq - window < j <= i + nk - nq  (window 0: no lower end),
  * and key_mask (NULL: all) is not 0 there.  A query that sees no key, or only keys
  * whose score is -inf, gives zeros and passes no gradient.  Values of keys that a
- * query does not see never reach its result, NaN and infinities included.
+ * query does not see never reach its result, NaN and infinities included; one that
+ * is seen makes what it enters NaN.
  * Rows of no sequence: zeros with SGL_ATTN_ZERO_REST, else left as they were.
  * B_dev (when given) is the live number of sequences, <= B.
- * 1 <= D <= 128, 1 <= Dv <= 256, Tq and Tk below 2^31. */
+ * 1 <= D <= 128, 1 <= Dv <= 256, Tq, Tk and B at most
+ * 2^31 - 256. */
 #define SGL_ATTN_ZERO_REST 1
 typedef struct {
     int32_t        dtype, Hq, Hk, D, Dv, causal;

@@ -27,8 +27,9 @@ FwdWork forward_work(const sgl_diff_attn_args& a) {
         units = (int64_t)w.tiles * a.Hq;
         keys = a.Tk / (a.B > 0 && a.B < w.tiles ? a.B : (w.tiles > 0 ? w.tiles : 1));
     }
-    // a call of fewer blocks than the chip holds side by side splits its key ranges, down to 256 keys a block (row tiles, whose
-    // partial results are as large as 2 x 128 rows of fp32, only when they would leave half of it idle)
+    // A call of fewer blocks than the chip holds side by side splits its key ranges, down to 256 keys a block.  16 histories of up to
+    // 32768 keys, 16 heads over 4: 1024 blocks 117 us and 9 to join them, 2048 116 and 13, 4096 126 and 23.  Row tiles, whose
+    // partial results are as large as 2 x 128 rows of fp32, are split only when they would leave half of the chip idle.
     int64_t splits = units > 0 ? (a.q_ptr ? 256 : 1024) / units : 1;
     if (splits > keys / 256) splits = keys / 256;
     w.splits = (int32_t)(splits < 1 ? 1 : splits > 64 ? 64 : splits);
@@ -38,7 +39,7 @@ FwdWork forward_work(const sgl_diff_attn_args& a) {
 
 namespace {
 
-constexpr int64_t GRID_MAX = 0x7FFFFFFF;
+constexpr int64_t GRID_MAX = 0x7FFFFFFF, COUNT_MAX = 0x7FFFFF00;
 
 int32_t check_args(const char* what, const sgl_diff_attn_args* a, bool backward) {
     if (!a) return fail(SGL_EINVAL, "%s: args is NULL", what);
@@ -46,7 +47,8 @@ int32_t check_args(const char* what, const sgl_diff_attn_args* a, bool backward)
     if (a->D < 1 || a->D > 128 || a->Dv < 1 || a->Dv > 256) return fail(SGL_ENOTSUP, "%s: D must lie in [1, 128] and Dv in [1, 256]", what);
     if (a->Hk < 1 || a->Hq < 1 || a->Hq % a->Hk || a->Hq > 65535) return fail(SGL_EINVAL, "%s: Hq must be a multiple of Hk (both in [1, 65535])", what);
     if (a->B < 0 || a->Tq < 0 || a->Tk < 0 || a->window < 0) return fail(SGL_EINVAL, "%s: negative size", what);
-    if (a->Tq > 0x7FFFFFFF || a->Tk > 0x7FFFFFFF || a->B > 0x7FFFFFFF) return fail(SGL_ENOTSUP, "%s: Tq, Tk and B must lie below 2^31", what);
+    // (rows are counted in 32 bits, and the last tile may reach past the last row)
+    if (a->Tq > COUNT_MAX || a->Tk > COUNT_MAX || a->B > COUNT_MAX) return fail(SGL_ENOTSUP, "%s: Tq, Tk and B must not exceed 2^31 - 256", what);
     if (a->window > 0 && !a->causal) return fail(SGL_EINVAL, "%s: a window needs causal", what);
     if (!a->q_ptr && a->Tq != a->B) return fail(SGL_EINVAL, "%s: without q_ptr there is one query per sequence (Tq = B)", what);
     if (!a->k_ptr || !a->lam) return fail(SGL_EINVAL, "%s: k_ptr/lam is NULL", what);
@@ -63,9 +65,16 @@ int32_t check_args(const char* what, const sgl_diff_attn_args* a, bool backward)
     return SGL_OK;
 }
 
-// Without q_ptr: sequences of fewer keys than this on average go without matrix units
-constexpr int64_t SEG_KEYS = 64;
-bool by_segments(const sgl_diff_attn_args& a) { return !a.q_ptr && a.Tk < SEG_KEYS * a.B; }
+// Without q_ptr: sequences of few keys on average go without matrix units, a wave per query and head, which reads a key once for
+// every query head of its group and walks it alone.  131072 keys in sequences of n, forward, matrix units against segments (us):
+//   16 heads over 4, 64 wide, bf16   n = 32: 260, 148   48: 187, 130   64: 145, 122   96: 115, 120   128: 91, 119
+//    8 heads over 8, 64 wide, bf16   n = 64: 196, 110   128: 142, 102   256: 124, 93   512: 107, 137
+//    2 heads over 2, 32 wide, fp32   n = 64: 64, 25   128: 49, 28   256: 43, 48   512: 44, 84
+// so groups of one or two heads stay there longer, if there is a wave for every SIMD.
+bool by_segments(const sgl_diff_attn_args& a) {
+    const int64_t keys = a.Hq / a.Hk <= 2 && a.B * a.Hq >= 1024 ? 192 : 64;
+    return !a.q_ptr && a.Tk < keys * a.B;
+}
 
 // every 16-byte chunk of a row is aligned and whole
 bool aligned_rows(const sgl_diff_attn_args& a, const sgl_rows& r, int64_t heads) {

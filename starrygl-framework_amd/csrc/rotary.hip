@@ -7,7 +7,8 @@
 //
 // All of it is bound by the rows it moves (x read once, the result written once; backward: x and dy read, dx
 // written), so the work per value is kept small: the angles of a row are formed once per block, reduced in fp64 and
-// parked in LDS as (cos, sin), and every head of the row reads them from there.
+// parked in LDS as (cos, sin), and every head of the row reads them from there.  262144 values a row side of 131072 rows in bf16
+// measured below.
 #include <math.h>
 
 #include "common.hpp"
