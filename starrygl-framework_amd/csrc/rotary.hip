@@ -7,8 +7,9 @@
 //
 // All of it is bound by the rows it moves (x read once, the result written once; backward: x and dy read, dx
 // written), so the work per value is kept small: the angles of a row are formed once per block, reduced in fp64 and
-// parked in LDS as (cos, sin), and every head of the row reads them from there.  262144 values a row side of 131072 rows in bf16
-// measured below.
+// parked in LDS as (cos, sin), and every head of the row reads them from there.  Reached, of the bytes a step cannot do without:
+// rotation 5.9 TB/s at 131072 rows of 4 KB, 3.2 at 120000 rows of 400 bytes; norm, forward and backward, 4.0 TB/s at 65536 rows
+// of 5 KB (a copy of 1 GiB: 5.0).
 #include <math.h>
 
 #include "common.hpp"
@@ -119,6 +120,10 @@ struct Where {
 // only with LP = 64).  A block walks tiles of `rows` rows; the tile's (row, head) vectors are dealt to its groups.
 template <typename T, int VW, bool INTER, int NI, int OP>
 __global__ __launch_bounds__(BLOCK) void rows_kernel(Args g, int32_t lp_log2) {
+    // Vectors on their way in a group.  Step (forward and gradient) of the rotation, 1, 2, 4 of them: 120000 rows of 2 heads of 50 in
+    // fp32 (one value a lane) 73, 63, 60 us; 131072 rows of 16 heads of 128 in bf16, half rotated (16 bytes a lane) 396, 366, 403 us.  The
+    // norm's registers are full with one: 65536 events, 40 heads of 64 in bf16, 331, 348, 387 us.
+    constexpr int UN = NI > 1 || OP != OP_ROT ? 1 : VW * sizeof(T) <= 8 ? 4 : 2;
     extern __shared__ __align__(16) float2 s_cs[];
     const bool second = (int32_t)blockIdx.x >= g.blocks0;
     const Side& s = g.s[second];
@@ -170,131 +175,137 @@ __global__ __launch_bounds__(BLOCK) void rows_kernel(Args g, int32_t lp_log2) {
                 __syncthreads();
             }
             const int32_t vectors = one_head ? rows : rows * s.heads;
-            // whole waves stay in the loop (the reductions below need the lanes of a group, which lie in one wave)
-            for (int32_t v0 = 0; v0 < vectors; v0 += groups) {
-                const int32_t v = v0 + group;
-                const bool live = v < vectors;
-                const int32_t r = live ? (one_head ? v : fast_div(v, s.heads_div)) : 0;
-                const int32_t h = one_head ? pass : (live ? v - r * s.heads : 0);
-                const T* __restrict__ xv = x + (row0 + r) * s.x_row + h * s.x_head;
-                float a[NI][VW], b[NI][VW], ga[NI][VW], gb[NI][VW];
-                float sum = 0.0f;
+            // whole waves stay in the loop (the reductions below need the lanes of a group, which lie in one wave); a group has
+            // UN vectors on their way at a time
+            for (int32_t v0 = 0; v0 < vectors; v0 += UN * groups) {
+                int32_t rr[UN], hh[UN];
+                bool live[UN];
+                float a[UN][NI][VW], b[UN][NI][VW], ga[UN][NI][VW], gb[UN][NI][VW];
+                Vec<T, VW> va[UN][NI], vb[UN][NI], ya[UN][NI], yb[UN][NI];
 #pragma unroll
-                for (int i = 0; i < NI; ++i) {
-                    const int32_t p = lane + i * 64;
-                    const bool on = live && p < g.pairs;
-#pragma unroll
-                    for (int e = 0; e < VW; ++e) a[i][e] = b[i][e] = ga[i][e] = gb[i][e] = 0.0f;
-                    if (!on) continue;
-                    const Where<VW, INTER> w(p, half, dim);
-                    const Vec<T, VW> va = *reinterpret_cast<const Vec<T, VW>*>(xv + w.a);
-                    Vec<T, VW> vb;
-#pragma unroll
-                    for (int e = 0; e < VW; ++e) vb.e[e] = (T)0.0f;
-                    if (w.b >= 0) vb = *reinterpret_cast<const Vec<T, VW>*>(xv + w.b);
-                    if constexpr (OP == OP_NORM_BWD) {
-                        const T* __restrict__ yv = y + (row0 + r) * s.y_row + h * s.y_head;
-                        const Vec<T, VW> ya = *reinterpret_cast<const Vec<T, VW>*>(yv + w.a);
-                        Vec<T, VW> yb;
-#pragma unroll
-                        for (int e = 0; e < VW; ++e) yb.e[e] = (T)0.0f;
-                        if (w.b >= 0) yb = *reinterpret_cast<const Vec<T, VW>*>(yv + w.b);
-#pragma unroll
-                        for (int e = 0; e < VW; ++e) ga[i][e] = (float)ya.e[e], gb[i][e] = (float)yb.e[e];
-                    }
-#pragma unroll
-                    for (int e = 0; e < VW; ++e) {
-                        a[i][e] = (float)va.e[e];
-                        b[i][e] = (float)vb.e[e];
-                        if (OP != OP_ROT) sum = __builtin_fmaf(a[i][e], a[i][e], __builtin_fmaf(b[i][e], b[i][e], sum));
-                    }
-                }
-                float inv = 1.0f;
-                if constexpr (OP != OP_ROT) {
-                    for (int32_t m = 1; m < (1 << lp_log2); m <<= 1) sum += __shfl_xor(sum, m);
-                    inv = 1.0f / __builtin_sqrtf(__builtin_fmaf(sum, inv_dim, g.eps));
-                }
-                float dot = 0.0f;
-                if constexpr (OP == OP_NORM_BWD) {
+                for (int u = 0; u < UN; ++u) {
+                    const int32_t v = v0 + u * groups + group;
+                    live[u] = v < vectors;
+                    rr[u] = live[u] ? (one_head ? v : fast_div(v, s.heads_div)) : 0;
+                    hh[u] = one_head ? pass : (live[u] ? v - rr[u] * s.heads : 0);
+                    const T* __restrict__ xv = x + (row0 + rr[u]) * s.x_row + hh[u] * s.x_head;
+                    const T* __restrict__ yv = OP == OP_NORM_BWD ? y + (row0 + rr[u]) * s.y_row + hh[u] * s.y_head : nullptr;
 #pragma unroll
                     for (int i = 0; i < NI; ++i) {
                         const int32_t p = lane + i * 64;
-                        if (!live || p >= g.pairs) continue;
+#pragma unroll
+                        for (int e = 0; e < VW; ++e) va[u][i].e[e] = vb[u][i].e[e] = ya[u][i].e[e] = yb[u][i].e[e] = (T)0.0f;
+                        if (!live[u] || p >= g.pairs) continue;
                         const Where<VW, INTER> w(p, half, dim);
-                        if (w.t >= 0) {
+                        va[u][i] = *reinterpret_cast<const Vec<T, VW>*>(xv + w.a);
+                        if (w.b >= 0) vb[u][i] = *reinterpret_cast<const Vec<T, VW>*>(xv + w.b);
+                        if constexpr (OP == OP_NORM_BWD) {
+                            ya[u][i] = *reinterpret_cast<const Vec<T, VW>*>(yv + w.a);
+                            if (w.b >= 0) yb[u][i] = *reinterpret_cast<const Vec<T, VW>*>(yv + w.b);
+                        }
+                    }
+                }
+#pragma unroll
+                for (int u = 0; u < UN; ++u) {
+                    const int32_t r = rr[u], h = hh[u];
+                    float sum = 0.0f;
+#pragma unroll
+                    for (int i = 0; i < NI; ++i)
+#pragma unroll
+                        for (int e = 0; e < VW; ++e) {
+                            a[u][i][e] = (float)va[u][i].e[e];
+                            b[u][i][e] = (float)vb[u][i].e[e];
+                            ga[u][i][e] = (float)ya[u][i].e[e];
+                            gb[u][i][e] = (float)yb[u][i].e[e];
+                            if (OP != OP_ROT) sum = __builtin_fmaf(a[u][i][e], a[u][i][e], __builtin_fmaf(b[u][i][e], b[u][i][e], sum));
+                        }
+                    float inv = 1.0f;
+                    if constexpr (OP != OP_ROT) {
+                        for (int32_t m = 1; m < (1 << lp_log2); m <<= 1) sum += __shfl_xor(sum, m);
+                        inv = 1.0f / __builtin_sqrtf(__builtin_fmaf(sum, inv_dim, g.eps));
+                    }
+                    float dot = 0.0f;
+                    if constexpr (OP == OP_NORM_BWD) {
+#pragma unroll
+                        for (int i = 0; i < NI; ++i) {
+                            const int32_t p = lane + i * 64;
+                            if (!live[u] || p >= g.pairs) continue;
+                            const Where<VW, INTER> w(p, half, dim);
+                            if (w.t >= 0) {
+                                const float2* __restrict__ cs = s_cs + r * half + w.t;
+                                if constexpr (INTER && VW > 1) {
+#pragma unroll
+                                    for (int e = 0; e < VW; e += 2) {
+                                        turn(ga[u][i][e], ga[u][i][e + 1], cs[e / 2].x, cs[e / 2].y);
+                                        turn(gb[u][i][e], gb[u][i][e + 1], cs[VW / 2 + e / 2].x, cs[VW / 2 + e / 2].y);
+                                    }
+                                } else {
+#pragma unroll
+                                    for (int e = 0; e < VW; ++e) turn(ga[u][i][e], gb[u][i][e], cs[e].x, cs[e].y);
+                                }
+                            }
+#pragma unroll
+                            for (int e = 0; e < VW; ++e) {
+                                const float xa = a[u][i][e] * inv, xb = b[u][i][e] * inv;
+                                da[i][e] = __builtin_fmaf(ga[u][i][e], xa, da[i][e]);
+                                db[i][e] = __builtin_fmaf(gb[u][i][e], xb, db[i][e]);
+                                ga[u][i][e] *= wa[i][e];
+                                gb[u][i][e] *= wb[i][e];
+                                dot = __builtin_fmaf(ga[u][i][e], xa, __builtin_fmaf(gb[u][i][e], xb, dot));
+                                a[u][i][e] = xa;
+                                b[u][i][e] = xb;
+                            }
+                        }
+                        for (int32_t m = 1; m < (1 << lp_log2); m <<= 1) dot += __shfl_xor(dot, m);
+                        dot *= inv_dim;
+                    }
+                    if (!live[u]) continue;
+                    T* __restrict__ ov = out + (row0 + r) * s.o_row + h * s.o_head;
+#pragma unroll
+                    for (int i = 0; i < NI; ++i) {
+                        const int32_t p = lane + i * 64;
+                        if (p >= g.pairs) continue;
+                        const Where<VW, INTER> w(p, half, dim);
+                        if constexpr (OP == OP_NORM) {
+                            if (per_head) {
+                                const float* wp = s.weight + h * s.w_stride;
+#pragma unroll
+                                for (int e = 0; e < VW; ++e) {
+                                    wa[i][e] = wp[w.a + e];
+                                    if (w.b >= 0) wb[i][e] = wp[w.b + e];
+                                }
+                            }
+#pragma unroll
+                            for (int e = 0; e < VW; ++e) {
+                                a[u][i][e] = a[u][i][e] * inv * wa[i][e];
+                                b[u][i][e] = b[u][i][e] * inv * wb[i][e];
+                            }
+                        }
+                        if constexpr (OP == OP_NORM_BWD) {
+#pragma unroll
+                            for (int e = 0; e < VW; ++e) {
+                                a[u][i][e] = inv * __builtin_fmaf(-a[u][i][e], dot, ga[u][i][e]);
+                                b[u][i][e] = inv * __builtin_fmaf(-b[u][i][e], dot, gb[u][i][e]);
+                            }
+                        } else if (w.t >= 0) {
                             const float2* __restrict__ cs = s_cs + r * half + w.t;
                             if constexpr (INTER && VW > 1) {
 #pragma unroll
                                 for (int e = 0; e < VW; e += 2) {
-                                    turn(ga[i][e], ga[i][e + 1], cs[e / 2].x, cs[e / 2].y);
-                                    turn(gb[i][e], gb[i][e + 1], cs[VW / 2 + e / 2].x, cs[VW / 2 + e / 2].y);
+                                    turn(a[u][i][e], a[u][i][e + 1], cs[e / 2].x, cs[e / 2].y);
+                                    turn(b[u][i][e], b[u][i][e + 1], cs[VW / 2 + e / 2].x, cs[VW / 2 + e / 2].y);
                                 }
                             } else {
 #pragma unroll
-                                for (int e = 0; e < VW; ++e) turn(ga[i][e], gb[i][e], cs[e].x, cs[e].y);
+                                for (int e = 0; e < VW; ++e) turn(a[u][i][e], b[u][i][e], cs[e].x, cs[e].y);
                             }
                         }
+                        Vec<T, VW> oa, ob;
 #pragma unroll
-                        for (int e = 0; e < VW; ++e) {
-                            const float xa = a[i][e] * inv, xb = b[i][e] * inv;
-                            da[i][e] = __builtin_fmaf(ga[i][e], xa, da[i][e]);
-                            db[i][e] = __builtin_fmaf(gb[i][e], xb, db[i][e]);
-                            ga[i][e] *= wa[i][e];
-                            gb[i][e] *= wb[i][e];
-                            dot = __builtin_fmaf(ga[i][e], xa, __builtin_fmaf(gb[i][e], xb, dot));
-                            a[i][e] = xa;
-                            b[i][e] = xb;
-                        }
+                        for (int e = 0; e < VW; ++e) oa.e[e] = (T)a[u][i][e], ob.e[e] = (T)b[u][i][e];
+                        *reinterpret_cast<Vec<T, VW>*>(ov + w.a) = oa;
+                        if (w.b >= 0) *reinterpret_cast<Vec<T, VW>*>(ov + w.b) = ob;
                     }
-                    for (int32_t m = 1; m < (1 << lp_log2); m <<= 1) dot += __shfl_xor(dot, m);
-                    dot *= inv_dim;
-                }
-                if (!live) continue;
-                T* __restrict__ ov = out + (row0 + r) * s.o_row + h * s.o_head;
-#pragma unroll
-                for (int i = 0; i < NI; ++i) {
-                    const int32_t p = lane + i * 64;
-                    if (p >= g.pairs) continue;
-                    const Where<VW, INTER> w(p, half, dim);
-                    if constexpr (OP == OP_NORM) {
-                        if (per_head) {
-                            const float* wp = s.weight + h * s.w_stride;
-#pragma unroll
-                            for (int e = 0; e < VW; ++e) {
-                                wa[i][e] = wp[w.a + e];
-                                if (w.b >= 0) wb[i][e] = wp[w.b + e];
-                            }
-                        }
-#pragma unroll
-                        for (int e = 0; e < VW; ++e) {
-                            a[i][e] = a[i][e] * inv * wa[i][e];
-                            b[i][e] = b[i][e] * inv * wb[i][e];
-                        }
-                    }
-                    if constexpr (OP == OP_NORM_BWD) {
-#pragma unroll
-                        for (int e = 0; e < VW; ++e) {
-                            a[i][e] = inv * __builtin_fmaf(-a[i][e], dot, ga[i][e]);
-                            b[i][e] = inv * __builtin_fmaf(-b[i][e], dot, gb[i][e]);
-                        }
-                    } else if (w.t >= 0) {
-                        const float2* __restrict__ cs = s_cs + r * half + w.t;
-                        if constexpr (INTER && VW > 1) {
-#pragma unroll
-                            for (int e = 0; e < VW; e += 2) {
-                                turn(a[i][e], a[i][e + 1], cs[e / 2].x, cs[e / 2].y);
-                                turn(b[i][e], b[i][e + 1], cs[VW / 2 + e / 2].x, cs[VW / 2 + e / 2].y);
-                            }
-                        } else {
-#pragma unroll
-                            for (int e = 0; e < VW; ++e) turn(a[i][e], b[i][e], cs[e].x, cs[e].y);
-                        }
-                    }
-                    Vec<T, VW> va, vb;
-#pragma unroll
-                    for (int e = 0; e < VW; ++e) va.e[e] = (T)a[i][e], vb.e[e] = (T)b[i][e];
-                    *reinterpret_cast<Vec<T, VW>*>(ov + w.a) = va;
-                    if (w.b >= 0) *reinterpret_cast<Vec<T, VW>*>(ov + w.b) = vb;
                 }
             }
         }
@@ -408,8 +419,9 @@ int lanes_log2(int32_t pairs) {
 }
 
 // Rows of a tile: enough (row, head) vectors for every group to get `trips` of them, within the table and the range of
-// fast_div.  Four trips amortise the barriers of a tile; a call too small to give the chip's 256 CUs four blocks each at
-// that size gets one trip.
+// fast_div.  Four trips amortise the barriers of a tile (120000 rows of 2 heads of 50, fp32, with 1, 4, 8 trips: 39, 27, 28
+// us; norm of 65536 events, 40 heads of 64, bf16, forward: 187, 133 us with 1, 4); a call too small to give the chip's 256 CUs
+// four blocks each at that size gets one trip.
 void set_side(Side& s, int32_t heads, int64_t N_max, int lp_log2, int32_t half, int64_t max_blocks) {
     s.heads = heads;
     s.N_max = N_max;
