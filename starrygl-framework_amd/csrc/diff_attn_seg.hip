@@ -5,9 +5,9 @@
 // head's key, the others the second, all of them the value; 64 / L keys are looked at side by side.  Nothing is read twice
 // and nothing waits for another wave: a backward wave has a key's scores, probabilities and d_out v product at hand, and
 // writes dK and dV as it goes.  Bound by the rows it moves: 2 D + Dv products a key and head stand against as many elements
-// read (and written, backward).  12000 roots with up to 10 neighbours, 2 heads over 2, 32 wide, fp32: forward 29 us, backward 45
-// us and 4 to sum d_lam, 2.5 TB/s of what a step cannot do without (5.0 by a large copy): the calls are short, and a wave waits
-// for its one or two rounds of loads.
+// read (and written, backward).  12000 roots with up to 10 neighbours, 2 heads over 2, 32 wide, fp32: forward 26 us, backward 38
+// us and 4 to sum d_lam (29, 45 and 4 without fetching the next keys before the present ones are worked on): the calls are short,
+// and a wave waits for its one or two rounds of loads.
 #include "diff_attn.hpp"
 
 namespace sgl {
@@ -45,6 +45,18 @@ __device__ __forceinline__ void store_part(T* dst, const float (&f)[Mat<T>::EP],
     }
 }
 
+// what a lane holds of a key and its value, still as it came: the next keys' are fetched before the present ones are worked on
+template <typename T>
+struct KeyPart {
+    typename Mat<T>::Frag k, v;
+    bool in, see;               // a key of the sequence; one that the query sees
+};
+template <typename T>
+__device__ __forceinline__ void widen(float (&f)[Mat<T>::EP], const typename Mat<T>::Frag& x) {
+#pragma unroll
+    for (int j = 0; j < Mat<T>::EP; ++j) f[j] = (float)x[j];
+}
+
 struct Lanes {
     int slot, half, e, ev;      // key of a pass, half of the head, first element of the half, first of the value
     template <int L, int EP>
@@ -58,6 +70,18 @@ struct Lanes {
         return s;
     }
 };
+
+template <typename T>
+__device__ __forceinline__ KeyPart<T> fetch(const sgl_diff_attn_args& a, Span span, int32_t j, int hk, const Lanes& ln, int aligned) {
+    KeyPart<T> x = {};
+    x.in = j < span.hi;
+    x.see = x.in && (a.key_mask == nullptr || a.key_mask[j]);
+    if (x.see) {
+        x.k = global_frag<T, false>(row<T>(a.k, j, 2 * hk + ln.half), ln.e, a.D, aligned);
+        x.v = global_frag<T, false>(row<T>(a.v, j, hk), ln.ev, a.Dv, aligned);
+    }
+    return x;
+}
 
 template <typename T, int L>
 __global__ __launch_bounds__(BLOCK) void seg_fwd_kernel(AttnArgs g) {
@@ -74,15 +98,17 @@ __global__ __launch_bounds__(BLOCK) void seg_fwd_kernel(AttnArgs g) {
     const Lanes ln = Lanes::make<L, EP>(lane);
     const float c2 = g.scale < 0.f ? -g.c2 : g.c2;
     float q[EP], o[2][EP], m[2] = {NEG_INF, NEG_INF}, l[2] = {0.f, 0.f};
+    KeyPart<T> next = fetch<T>(a, span, span.lo + ln.slot, hk, ln, g.aligned);
     load_part<T>(q, row<T>(a.q, i, 2 * h + ln.half), ln.e, a.D, true, g.aligned);
 #pragma unroll
     for (int j = 0; j < EP; ++j) o[0][j] = o[1][j] = 0.f;
     for (int32_t j0 = span.lo; j0 < span.hi; j0 += SLOTS) {
-        const int32_t j = j0 + ln.slot;
-        const bool see = j < span.hi && (a.key_mask == nullptr || a.key_mask[j]);
+        const KeyPart<T> key = next;
+        next = fetch<T>(a, span, j0 + SLOTS + ln.slot, hk, ln, g.aligned);
+        const bool see = key.see;
         float k[EP], v[EP];
-        load_part<T>(k, row<T>(a.k, see ? j : span.lo, 2 * hk + ln.half), ln.e, a.D, see, g.aligned);
-        load_part<T>(v, row<T>(a.v, see ? j : span.lo, hk), ln.ev, a.Dv, see, g.aligned);
+        widen<T>(k, key.k);
+        widen<T>(v, key.v);
         float x = 0.f;
 #pragma unroll
         for (int e = 0; e < EP; ++e) x = __builtin_fmaf(q[e], k[e], x);
@@ -169,13 +195,16 @@ __global__ __launch_bounds__(BLOCK) void seg_bwd_kernel(AttnArgs g) {
         };
 #pragma unroll
         for (int e = 0; e < EP; ++e) dq[e] = 0.f;
+        KeyPart<T> next = fetch<T>(a, span, span.lo + ln.slot, hk, ln, g.aligned);
         if (DQ || G == 1) of_head(head);
         for (int32_t j0 = span.lo; j0 < span.hi; j0 += SLOTS) {
             const int32_t j = j0 + ln.slot;
-            const bool in = j < span.hi, see = in && (a.key_mask == nullptr || a.key_mask[j]);
+            const KeyPart<T> key = next;
+            next = fetch<T>(a, span, j0 + SLOTS + ln.slot, hk, ln, g.aligned);
+            const bool in = key.in, see = key.see;
             float k[EP], v[EP], dk[EP], dv[EP];
-            load_part<T>(k, row<T>(a.k, see ? j : span.lo, 2 * hk + ln.half), ln.e, a.D, see, g.aligned);
-            load_part<T>(v, row<T>(a.v, see ? j : span.lo, hk), ln.ev, a.Dv, see, g.aligned);
+            widen<T>(k, key.k);
+            widen<T>(v, key.v);
 #pragma unroll
             for (int e = 0; e < EP; ++e) dk[e] = dv[e] = 0.f;
             for (int hg = 0; hg < (DQ ? 1 : G); ++hg) {
