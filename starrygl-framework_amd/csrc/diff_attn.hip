@@ -76,18 +76,17 @@ bool by_segments(const sgl_diff_attn_args& a) {
     return !a.q_ptr && a.Tk < keys * a.B;
 }
 
-// every 16-byte chunk of a row is aligned and whole
-bool aligned_rows(const sgl_diff_attn_args& a, const sgl_rows& r, int64_t heads) {
-    const int64_t ep = a.dtype == SGL_DT_F32 ? 4 : 8;
-    return r.data == nullptr || (reinterpret_cast<uintptr_t>(r.data) % 16 == 0 && r.row_stride % ep == 0 && (heads == 1 || r.head_stride % ep == 0));
-}
-bool aligned_args(const sgl_diff_attn_args& a) {
-    const int64_t ep = a.dtype == SGL_DT_F32 ? 4 : 8;
-    bool ok = a.D % ep == 0 && a.Dv % ep == 0;
-    for (const sgl_rows* r : {&a.q, &a.k, &a.d_q, &a.d_k}) ok = ok && aligned_rows(a, *r, 2);
-    for (const sgl_rows* r : {&a.out, &a.o2, &a.d_out}) ok = ok && aligned_rows(a, *r, a.Hq);
-    for (const sgl_rows* r : {&a.v, &a.d_v}) ok = ok && aligned_rows(a, *r, a.Hk);
-    return ok;
+// the widest pieces, of 16 bytes at most, that all rows divide into
+int32_t grain_of(const sgl_diff_attn_args& a) {
+    const int64_t item = a.dtype == SGL_DT_F32 ? 4 : 2;
+    uint64_t bits = 16 | (uint64_t)(a.D * item) | (uint64_t)(a.Dv * item);
+    auto rows = [&](const sgl_rows& r, int64_t heads) {
+        if (r.data) bits |= reinterpret_cast<uintptr_t>(r.data) | (uint64_t)(r.row_stride * item) | (heads > 1 ? (uint64_t)(r.head_stride * item) : 0);
+    };
+    for (const sgl_rows* r : {&a.q, &a.k, &a.d_q, &a.d_k}) rows(*r, 2);
+    for (const sgl_rows* r : {&a.out, &a.o2, &a.d_out}) rows(*r, a.Hq);
+    for (const sgl_rows* r : {&a.v, &a.d_v}) rows(*r, a.Hk);
+    return (int32_t)(bits & (~bits + 1));       // the lowest bit
 }
 
 int32_t forward_parts(const sgl_diff_attn_args& a) {
@@ -122,7 +121,7 @@ extern "C" int32_t sgl_diff_attn(const sgl_diff_attn_args* a, void* workspace, s
     if (int32_t rc = check_args("diff_attn", a, false)) return rc;
     if (a->Tq == 0) return SGL_OK;
     AttnArgs g = attn_args(*a);
-    g.aligned = aligned_args(*a);
+    g.grain = grain_of(*a);
     g.parts = forward_parts(*a);
     const size_t need = forward_need(*a, g.parts);
     if (need > 0) {
@@ -149,7 +148,7 @@ extern "C" int32_t sgl_diff_attn_backward(const sgl_diff_attn_args* a, void* wor
     const size_t need = backward_need(*a);
     if (!workspace || workspace_bytes < need) return fail(SGL_ENOMEM, "diff_attn_backward: workspace of %zu bytes, %zu needed", workspace_bytes, need);
     AttnArgs g = attn_args(*a);
-    g.aligned = aligned_args(*a);
+    g.grain = grain_of(*a);
     Arena ws(workspace, workspace_bytes);
     if (!a->q_ptr) {
         g.lam_part = ws.take<float>((size_t)seg_blocks(*a) * (size_t)a->Hq);

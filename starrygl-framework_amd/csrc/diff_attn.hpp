@@ -20,7 +20,7 @@ struct AttnArgs {
     float scale;                // of the scores
     float c2;                   // |scale| log2(e): scores enter exponentials of base 2
     int32_t negate;             // scale < 0: the operand that stays in registers changes its sign (exact)
-    int32_t aligned;            // every row of q, k, v (and of the gradients read) is a whole number of 16-byte chunks
+    int32_t grain;              // bytes, 16 at most, that divide the address of every row and the length of every row's head
     int32_t parts;              // forward: partial results per (row, head, map), joined by a second kernel; 1: none
     float* part_ml;             // [parts, Tq * Hq, 2, 2]: running maximum (in powers of two) and sum
     float* part_o;              // [parts, Tq * Hq, 2, Dv]
@@ -314,6 +314,64 @@ struct Pipe {
     }
 };
 
+// A chunk of 16 bytes of which `left` elements are a row's (none, where left <= 0), the others zero; rows of other widths than whole
+// chunks move in pieces of `grain` bytes (a training step of 8 sequences of 1024, 8 heads, causal: 50 wide in bf16, pieces of 4
+// bytes, 466 us; 100 wide in fp16, pieces of 8, 1040 us; element by element 532 and 1407).
+template <typename T>
+__device__ __forceinline__ typename Mat<T>::Frag load_chunk(const T* src, int left, int grain) {
+    constexpr int EP = Mat<T>::EP;
+    union {
+        typename Mat<T>::Frag f;
+        uint4 w16;
+        uint2 w8[2];
+        uint32_t w4[4];
+    } u;
+    u.w16 = uint4{0, 0, 0, 0};
+    if (grain == 16) {
+        if (left > 0) u.w16 = *reinterpret_cast<const uint4*>(src);
+    } else if (grain == 8) {
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+            if (left > k * (EP / 2)) u.w8[k] = reinterpret_cast<const uint2*>(src)[k];
+    } else if (grain == 4 || sizeof(T) == 4) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            if (left > k * (EP / 4)) u.w4[k] = reinterpret_cast<const uint32_t*>(src)[k];
+    } else {
+        typename Mat<T>::Frag f;
+#pragma unroll
+        for (int k = 0; k < EP; ++k) f[k] = left > k ? src[k] : (T)0.0f;
+        return f;
+    }
+    return u.f;
+}
+template <typename T>
+__device__ __forceinline__ void store_chunk(T* dst, const typename Mat<T>::Frag& f, int left, int grain) {
+    constexpr int EP = Mat<T>::EP;
+    union {
+        typename Mat<T>::Frag f;
+        uint4 w16;
+        uint2 w8[2];
+        uint32_t w4[4];
+    } u;
+    u.f = f;
+    if (grain == 16) {
+        if (left > 0) *reinterpret_cast<uint4*>(dst) = u.w16;
+    } else if (grain == 8) {
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+            if (left > k * (EP / 2)) reinterpret_cast<uint2*>(dst)[k] = u.w8[k];
+    } else if (grain == 4 || sizeof(T) == 4) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            if (left > k * (EP / 4)) reinterpret_cast<uint32_t*>(dst)[k] = u.w4[k];
+    } else {
+#pragma unroll
+        for (int k = 0; k < EP; ++k)
+            if (left > k) dst[k] = u.f[k];
+    }
+}
+
 // where chunk c of a staged row comes from: the two halves of a head ([2][D], D <= DP each), or one head of Dv <= 2 DP
 struct Source {
     const void* data;
@@ -370,7 +428,7 @@ struct Stager {
                 }
         }
     }
-    __device__ __forceinline__ void load(char* tile, const Source& s, int32_t row0, int32_t last, int aligned) const {
+    __device__ __forceinline__ void load(char* tile, const Source& s, int32_t row0, int32_t last, int grain) const {
         if constexpr (DMA) {
             const int wave = threadIdx.x >> 6;
             if (row0 + ROWS - 1 <= last) {
@@ -406,13 +464,7 @@ struct Stager {
                 const int32_t n = row0 + r < last ? row0 + r : last;
                 const int e = TWO ? (c % (CH / 2)) * EP : c * EP;
                 const T* src = base + (int64_t)n * s.row_stride + (TWO ? (c / (CH / 2)) * s.half_stride : 0) + e;
-                Frag f;
-                if (aligned && e + EP <= s.len) {
-                    f = *reinterpret_cast<const Frag*>(src);
-                } else {
-#pragma unroll
-                    for (int j = 0; j < EP; ++j) f[j] = e + j < s.len ? src[j] : (T)0.0f;
-                }
+                const Frag f = load_chunk<T>(src, s.len - e, grain);
                 *reinterpret_cast<Frag*>(tile + at<RB>(r, c)) = f;
             }
         }
@@ -484,16 +536,9 @@ __device__ __forceinline__ void staged() {
 
 // EP elements from element e of a row, kept in registers; zero beyond len.  WHOLE: every chunk is whole and aligned.
 template <typename T, bool WHOLE>
-__device__ __forceinline__ typename Mat<T>::Frag global_frag(const T* src, int e, int len, int aligned) {
-    typename Mat<T>::Frag f;
-    constexpr int EP = Mat<T>::EP;
-    if (WHOLE || (aligned && e + EP <= len)) {
-        f = *reinterpret_cast<const typename Mat<T>::Frag*>(src + e);
-    } else {
-#pragma unroll
-        for (int j = 0; j < EP; ++j) f[j] = e + j < len ? src[e + j] : (T)0.0f;
-    }
-    return f;
+__device__ __forceinline__ typename Mat<T>::Frag global_frag(const T* src, int e, int len, int grain) {
+    if constexpr (WHOLE) return *reinterpret_cast<const typename Mat<T>::Frag*>(src + e);
+    else return load_chunk<T>(src + e, len - e, grain);
 }
 
 __device__ __forceinline__ f32x16 zero16() {
@@ -509,7 +554,7 @@ __device__ __forceinline__ f32x16 zero16() {
 // where bit k of `keep` is set.  The order is fixed, a few values at a time: a spilled register here would be read back behind the stores (loads
 // and stores return through one counter), which cost 28000 cycles a block.
 template <typename T, int PIECE, int N, bool WHOLE, typename Val>
-__device__ __forceinline__ void store_rows(Val val, char* box, int lane, int len, int aligned, T* base, int64_t stride, uint32_t keep) {
+__device__ __forceinline__ void store_rows(Val val, char* box, int lane, int len, int grain, T* base, int64_t stride, uint32_t keep) {
     constexpr int FIT = PIECE / (32 * (int)sizeof(T)), AT = FIT >= N ? N : FIT >= 2 ? 2 : 1;           // 32-wide pieces at a time
     static_assert(FIT >= 1, "one piece fits");
     constexpr int BYTES = AT * 32 * (int)sizeof(T), CH = BYTES / 16, EP = 16 / (int)sizeof(T);
@@ -538,13 +583,8 @@ __device__ __forceinline__ void store_rows(Val val, char* box, int lane, int len
             const int r = i * (64 / CH) + lane / CH;
             const typename Mat<T>::Frag f = *reinterpret_cast<const typename Mat<T>::Frag*>(box + r * BYTES + (((c ^ r) & (CH - 1)) << 4));
             if ((keep >> r) & 1) {
-                if (WHOLE || (aligned && left >= EP)) {
-                    *reinterpret_cast<typename Mat<T>::Frag*>(to) = f;
-                } else {
-#pragma unroll
-                    for (int e = 0; e < EP; ++e)
-                        if (e < left) to[e] = f[e];
-                }
+                if constexpr (WHOLE) *reinterpret_cast<typename Mat<T>::Frag*>(to) = f;
+                else store_chunk<T>(to, f, left, grain);
             }
             to += (64 / CH) * stride;
             __builtin_amdgcn_sched_barrier(0);

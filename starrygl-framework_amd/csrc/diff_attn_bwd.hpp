@@ -151,13 +151,13 @@ __global__ __launch_bounds__((Rows<T, DP>::WAVES * 64), (Rows<T, DP>::OCC)) void
 #pragma unroll
     for (int m = 0; m < 2; ++m)
 #pragma unroll
-        for (int k = 0; k < S::QS; ++k) q[m][k] = global_frag<T, DMA>(row<T>(a.q, ii, 2 * h + m), (2 * k + half) * S::EP, a.D, g.aligned);
+        for (int k = 0; k < S::QS; ++k) q[m][k] = global_frag<T, DMA>(row<T>(a.q, ii, 2 * h + m), (2 * k + half) * S::EP, a.D, g.grain);
 #pragma unroll
     for (int k = 0; k < S::VS; ++k) {
         const int e = (2 * k + half) * S::EP;
-        go[k] = global_frag<T, DMA>(row<T>(a.d_out, ii, h), e, a.Dv, g.aligned);
-        const typename M::Frag y2 = global_frag<T, DMA>(row<T>(a.o2, ii, h), e, a.Dv, g.aligned);
-        const typename M::Frag y = global_frag<T, DMA>(row<T>(a.out, ii, h), e, a.Dv, g.aligned);
+        go[k] = global_frag<T, DMA>(row<T>(a.d_out, ii, h), e, a.Dv, g.grain);
+        const typename M::Frag y2 = global_frag<T, DMA>(row<T>(a.o2, ii, h), e, a.Dv, g.grain);
+        const typename M::Frag y = global_frag<T, DMA>(row<T>(a.out, ii, h), e, a.Dv, g.grain);
 #pragma unroll
         for (int j = 0; j < S::EP; ++j) {
             t[0] = __builtin_fmaf((float)go[k][j], __builtin_fmaf(lam, (float)y2[j], (float)y[j]), t[0]);
@@ -195,8 +195,8 @@ __global__ __launch_bounds__((Rows<T, DP>::WAVES * 64), (Rows<T, DP>::OCC)) void
             stage_finite<T, DP, BN, NT>(buf, s_marks, ks, true, j, last);
             stage_finite<T, DP, BN, NT>(buf + BN * RB, s_marks + BN * (RB / 16), vs, false, j, last);
         } else {
-            stage_k.load(buf, ks, j, last, g.aligned);
-            stage_v.load(buf + BN * RB, vs, j, last, g.aligned);
+            stage_k.load(buf, ks, j, last, g.grain);
+            stage_v.load(buf + BN * RB, vs, j, last, g.grain);
         }
     };
     // (the lane's parts of the addresses, as of the keys' kernel)
@@ -334,9 +334,9 @@ __global__ __launch_bounds__((Rows<T, DP>::WAVES * 64), (Rows<T, DP>::OCC)) void
     char* box = (wave & 1 ? s_b : s_a) + (wave >> 1) * (P::TILE / 2);
     constexpr int PIECE = RB / 2;                               // bytes of a row at a time
     const float f0 = g.scale, f1 = -lam * g.scale;
-    store_rows<T, PIECE, S::DT, DMA>([&](int d, int r) { return spoilt[0] ? NAN : live ? dq[0][d][r] * f0 : 0.f; }, box, lane, a.D, g.aligned, row_out<T>(a.d_q, i0, 2 * h),
+    store_rows<T, PIECE, S::DT, DMA>([&](int d, int r) { return spoilt[0] ? NAN : live ? dq[0][d][r] * f0 : 0.f; }, box, lane, a.D, g.grain, row_out<T>(a.d_q, i0, 2 * h),
                                      a.d_q.row_stride, keep);
-    store_rows<T, PIECE, S::DT, DMA>([&](int d, int r) { return spoilt[1] ? NAN : live ? dq[1][d][r] * f1 : 0.f; }, box, lane, a.D, g.aligned, row_out<T>(a.d_q, i0, 2 * h + 1),
+    store_rows<T, PIECE, S::DT, DMA>([&](int d, int r) { return spoilt[1] ? NAN : live ? dq[1][d][r] * f1 : 0.f; }, box, lane, a.D, g.grain, row_out<T>(a.d_q, i0, 2 * h + 1),
                                      a.d_q.row_stride, keep);
 }
 
@@ -427,11 +427,11 @@ __device__ __forceinline__ void keys_body(const AttnArgs& g, int32_t tiles, char
 #pragma unroll
         for (int m = P::KEY_LDS; m < 2; ++m)
 #pragma unroll
-            for (int e = 0; e < S::QS; ++e) k[m][e] = global_frag<T, DMA>(row<T>(a.k, jj, 2 * hk + m), (2 * e + half) * S::EP, a.D, g.aligned);
-        if constexpr (P::KEY_LDS == 2) Stager<T, DP, ROWS, NT, false, true>().load(s_own, halves<T>(a.k, hk, a.D), tile * ROWS, (int32_t)a.Tk - 1, g.aligned);
-        if constexpr (P::KEY_LDS == 1) Stager<T, DP / 2, ROWS, NT, false, false>().load(s_own, run<T>(a.k, 2 * hk, a.D), tile * ROWS, (int32_t)a.Tk - 1, g.aligned);
+            for (int e = 0; e < S::QS; ++e) k[m][e] = global_frag<T, DMA>(row<T>(a.k, jj, 2 * hk + m), (2 * e + half) * S::EP, a.D, g.grain);
+        if constexpr (P::KEY_LDS == 2) Stager<T, DP, ROWS, NT, false, true>().load(s_own, halves<T>(a.k, hk, a.D), tile * ROWS, (int32_t)a.Tk - 1, g.grain);
+        if constexpr (P::KEY_LDS == 1) Stager<T, DP / 2, ROWS, NT, false, false>().load(s_own, run<T>(a.k, 2 * hk, a.D), tile * ROWS, (int32_t)a.Tk - 1, g.grain);
 #pragma unroll
-        for (int e = 0; e < S::VS; ++e) v[e] = global_frag<T, DMA>(row<T>(a.v, jj, hk), (2 * e + half) * S::EP, a.Dv, g.aligned);
+        for (int e = 0; e < S::VS; ++e) v[e] = global_frag<T, DMA>(row<T>(a.v, jj, hk), (2 * e + half) * S::EP, a.Dv, g.grain);
     }
     f32x16 dk[2][S::DT], dv[S::VT];
     auto clear = [&]() {
@@ -456,8 +456,8 @@ __device__ __forceinline__ void keys_body(const AttnArgs& g, int32_t tiles, char
             stage_finite<T, DP, BQ, NT>(buf, s_marks, halves<T>(a.q, h, a.D), true, i0, last);
             stage_finite<T, DP, BQ, NT>(buf + BQ * RB, s_marks + BQ * (RB / 16), run<T>(a.d_out, h, a.Dv), false, i0, last);
         } else {
-            stage_q.load(buf, halves<T>(a.q, h, a.D), i0, last, g.aligned);
-            stage_go.load(buf + BQ * RB, run<T>(a.d_out, h, a.Dv), i0, last, g.aligned);
+            stage_q.load(buf, halves<T>(a.q, h, a.D), i0, last, g.grain);
+            stage_go.load(buf + BQ * RB, run<T>(a.d_out, h, a.Dv), i0, last, g.grain);
         }
         if (wave < 3) {
             // 64 numbers each: lse, t of the rows, map by map, and lam 64 times (a load of its own in a step would wait for the
@@ -673,13 +673,13 @@ __device__ __forceinline__ void keys_body(const AttnArgs& g, int32_t tiles, char
     constexpr int PIECE = TILE / P::WAVES / 32;                 // bytes of a row at a time
     char* box = s_a + wave * (TILE / P::WAVES);
     if (P::SPLIT == 1 || !share) {
-        store_rows<T, PIECE, S::DT, DMA>([&](int t, int r) { return spoilt[0] ? NAN : shown ? dk[0][t][r] * g.scale : 0.f; }, box, lane, a.D, g.aligned,
+        store_rows<T, PIECE, S::DT, DMA>([&](int t, int r) { return spoilt[0] ? NAN : shown ? dk[0][t][r] * g.scale : 0.f; }, box, lane, a.D, g.grain,
                                          row_out<T>(a.d_k, j0, 2 * hk), a.d_k.row_stride, keep);
-        store_rows<T, PIECE, S::DT, DMA>([&](int t, int r) { return spoilt[1] ? NAN : shown ? dk[1][t][r] * g.scale : 0.f; }, box, lane, a.D, g.aligned,
+        store_rows<T, PIECE, S::DT, DMA>([&](int t, int r) { return spoilt[1] ? NAN : shown ? dk[1][t][r] * g.scale : 0.f; }, box, lane, a.D, g.grain,
                                          row_out<T>(a.d_k, j0, 2 * hk + 1), a.d_k.row_stride, keep);
     }
     if (P::SPLIT == 1 || share)
-        store_rows<T, PIECE, S::VT, DMA>([&](int t, int r) { return shown ? dv[t][r] : 0.f; }, box, lane, a.Dv, g.aligned, row_out<T>(a.d_v, j0, hk), a.d_v.row_stride, keep);
+        store_rows<T, PIECE, S::VT, DMA>([&](int t, int r) { return shown ? dv[t][r] : 0.f; }, box, lane, a.Dv, g.grain, row_out<T>(a.d_v, j0, hk), a.d_v.row_stride, keep);
 }
 
 template <typename T, int DP, bool DMA>
@@ -730,8 +730,8 @@ __device__ __forceinline__ void roles_body(const AttnArgs& g, int32_t tiles, cha
     if (!__all(shown)) reach.to = 0;
     if (threadIdx.x == 0) s_bad = 0;
     const int32_t lo = reach.lo, hi = reach.hi;                 // (both waves have the same keys)
-    Stager<T, DP, ROWS, NT, false, true>().load(s_own, halves<T>(a.k, hk, a.D), j0, (int32_t)a.Tk - 1, g.aligned);
-    Stager<T, DP, ROWS, NT, false, false>().load(s_own + ROWS * RB, run<T>(a.v, hk, a.Dv), j0, (int32_t)a.Tk - 1, g.aligned);
+    Stager<T, DP, ROWS, NT, false, true>().load(s_own, halves<T>(a.k, hk, a.D), j0, (int32_t)a.Tk - 1, g.grain);
+    Stager<T, DP, ROWS, NT, false, false>().load(s_own + ROWS * RB, run<T>(a.v, hk, a.Dv), j0, (int32_t)a.Tk - 1, g.grain);
     f32x16 dk[2][S::DT], dv[S::VT];
     auto clear = [&]() {
 #pragma unroll
@@ -764,8 +764,8 @@ __device__ __forceinline__ void roles_body(const AttnArgs& g, int32_t tiles, cha
             stage_finite<T, DP, BQ, NT>(buf, s_marks, halves<T>(a.q, h, a.D), true, i0, last);
             stage_finite<T, DP, BQ, NT>(buf + BQ * RB, s_marks + BQ * (RB / 16), run<T>(a.d_out, h, a.Dv), false, i0, last);
         } else {
-            stage_q.load(buf, halves<T>(a.q, h, a.D), i0, last, g.aligned);
-            stage_go.load(buf + BQ * RB, run<T>(a.d_out, h, a.Dv), i0, last, g.aligned);
+            stage_q.load(buf, halves<T>(a.q, h, a.D), i0, last, g.grain);
+            stage_go.load(buf + BQ * RB, run<T>(a.d_out, h, a.Dv), i0, last, g.grain);
         }
         load_stats(buf, h, i0);
     };
@@ -888,13 +888,13 @@ __device__ __forceinline__ void roles_body(const AttnArgs& g, int32_t tiles, cha
     char* box = s_a + wave * (TILE / P::WAVES);
     constexpr int PIECE = TILE / P::WAVES / 32;               // bytes of a row at a time
     if constexpr (DK) {
-        store_rows<T, PIECE, S::DT, DMA>([&](int t, int r) { return spoilt[0] ? NAN : shown ? dk[0][t][r] * g.scale : 0.f; }, box, lane, a.D, g.aligned,
+        store_rows<T, PIECE, S::DT, DMA>([&](int t, int r) { return spoilt[0] ? NAN : shown ? dk[0][t][r] * g.scale : 0.f; }, box, lane, a.D, g.grain,
                                          row_out<T>(a.d_k, j0, 2 * hk), a.d_k.row_stride, keep);
-        store_rows<T, PIECE, S::DT, DMA>([&](int t, int r) { return spoilt[1] ? NAN : shown ? dk[1][t][r] * g.scale : 0.f; }, box, lane, a.D, g.aligned,
+        store_rows<T, PIECE, S::DT, DMA>([&](int t, int r) { return spoilt[1] ? NAN : shown ? dk[1][t][r] * g.scale : 0.f; }, box, lane, a.D, g.grain,
                                          row_out<T>(a.d_k, j0, 2 * hk + 1), a.d_k.row_stride, keep);
     }
     if constexpr (DV)
-        store_rows<T, PIECE, S::VT, DMA>([&](int t, int r) { return shown ? dv[t][r] : 0.f; }, box, lane, a.Dv, g.aligned, row_out<T>(a.d_v, j0, hk), a.d_v.row_stride, keep);
+        store_rows<T, PIECE, S::VT, DMA>([&](int t, int r) { return shown ? dv[t][r] : 0.f; }, box, lane, a.Dv, g.grain, row_out<T>(a.d_v, j0, hk), a.d_v.row_stride, keep);
 }
 
 template <typename T, int DP, bool DMA>
@@ -916,7 +916,7 @@ void launch(const AttnArgs& g, hipStream_t st) {
     const sgl_diff_attn_args& a = g.a;
     typedef Shape<T, DP> S;
     const int32_t qt = (int32_t)ceil_div<int64_t>(a.Tq, QUERY_ROWS);
-    const bool dma = g.aligned && a.D == DP && a.Dv == 2 * DP && dma_rows(a.k) && dma_rows(a.v) && dma_rows(a.q) && dma_rows(a.d_out);
+    const bool dma = g.grain == 16 && a.D == DP && a.Dv == 2 * DP && dma_rows(a.k) && dma_rows(a.v) && dma_rows(a.q) && dma_rows(a.d_out);
     if (qt > 0) {
         const dim3 grid((unsigned)(ceil_div<int64_t>((int64_t)qt * a.Hq, 8) * 8)), block(Rows<T, DP>::WAVES * 64);
         if (dma) hipLaunchKernelGGL((bwd_rows_kernel<T, DP, true>), grid, block, 0, st, g, qt);

@@ -201,7 +201,7 @@ __global__ __launch_bounds__((Shape<T, DP, HEADS>::NT), (HEADS && Shape<T, DP, H
     for (int c = 0; c < MAPS; ++c)
 #pragma unroll
         for (int k = 0; k < S::QS; ++k)
-            q[c][k] = global_frag<T, DMA>(row<T>(a.q, mine ? i : 0, 2 * h + map0 + c), (2 * k + half) * S::EP, a.D, g.aligned);
+            q[c][k] = global_frag<T, DMA>(row<T>(a.q, mine ? i : 0, 2 * h + map0 + c), (2 * k + half) * S::EP, a.D, g.grain);
     mine = mine && (seq >= 0 || (a.flags & SGL_ATTN_ZERO_REST));
     Reach reach = reach_of(span);
     if (a.key_mask) reach.to = 0;
@@ -229,9 +229,9 @@ __global__ __launch_bounds__((Shape<T, DP, HEADS>::NT), (HEADS && Shape<T, DP, H
     stage_v.plan(vs);
     bool finite = false;        // the pass without what is not finite
     auto load = [&](char* buf, int32_t j) {
-        stage_k.load(buf, ks, j, last, g.aligned);
+        stage_k.load(buf, ks, j, last, g.grain);
         if (finite) stage_finite<T, DP, BN, S::NT>(buf + BN * RB, s_marks, vs, false, j, last);
-        else stage_v.load(buf + BN * RB, vs, j, last, g.aligned);
+        else stage_v.load(buf + BN * RB, vs, j, last, g.grain);
     };
     auto work = [&](const char* buf, int32_t j) {
 #pragma unroll
@@ -335,8 +335,8 @@ __global__ __launch_bounds__((Shape<T, DP, HEADS>::NT), (HEADS && Shape<T, DP, H
         if constexpr (MAPS == 2) {
             const auto second = [&](int t, int r) { return inv[1] == 0.f ? 0.f : st.o[1][t][r] * inv[1]; };
             store_rows<T, SHARE / 32, VT, DMA>([&](int t, int r) { return __builtin_fmaf(-lam, second(t, r), inv[0] == 0.f ? 0.f : st.o[0][t][r] * inv[0]); }, own, lane, a.Dv,
-                                               g.aligned, row_out<T>(a.out, i0, h), a.out.row_stride, keep);
-            if (a.o2.data) store_rows<T, SHARE / 32, VT, DMA>(second, own, lane, a.Dv, g.aligned, row_out<T>(a.o2, i0, h), a.o2.row_stride, keep);
+                                               g.grain, row_out<T>(a.out, i0, h), a.out.row_stride, keep);
+            if (a.o2.data) store_rows<T, SHARE / 32, VT, DMA>(second, own, lane, a.Dv, g.grain, row_out<T>(a.o2, i0, h), a.o2.row_stride, keep);
         } else {
 #pragma unroll
             for (int t = 0; t < VT; ++t)
@@ -374,7 +374,7 @@ __global__ __launch_bounds__((Shape<T, DP, HEADS>::NT), (HEADS && Shape<T, DP, H
             __syncthreads();
             const sgl_rows& to = map0 ? a.o2 : a.out;
             if (to.data)
-                store_rows<T, SHARE / 32, VT, DMA>([&](int t, int r) { return st.o[0][t][r]; }, own, lane, a.Dv, g.aligned, row_out<T>(to, i0, h), to.row_stride, keep);
+                store_rows<T, SHARE / 32, VT, DMA>([&](int t, int r) { return st.o[0][t][r]; }, own, lane, a.Dv, g.grain, row_out<T>(to, i0, h), to.row_stride, keep);
         }
     }
 }
@@ -467,7 +467,7 @@ void launch(const AttnArgs& g, hipStream_t st) {
     const FwdWork w = forward_work(g.a);
     const dim3 grid((unsigned)(ceil_div<int64_t>(w.items, 8) * 8));
     constexpr int ROW_NT = Shape<T, DP, false>::NT, HEAD_NT = Shape<T, DP, true>::NT;
-    const bool dma = g.aligned && g.a.D == DP && g.a.Dv == 2 * DP && dma_rows(g.a.k) && dma_rows(g.a.v);
+    const bool dma = g.grain == 16 && g.a.D == DP && g.a.Dv == 2 * DP && dma_rows(g.a.k) && dma_rows(g.a.v);
     if (g.a.q_ptr) {
         if (dma) hipLaunchKernelGGL((fwd_kernel<T, DP, false, true>), grid, dim3(ROW_NT), 0, st, g, w);
         else hipLaunchKernelGGL((fwd_kernel<T, DP, false, false>), grid, dim3(ROW_NT), 0, st, g, w);

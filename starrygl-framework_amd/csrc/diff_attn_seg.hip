@@ -25,24 +25,18 @@ __device__ __forceinline__ float lanes_sum(float x) {
 
 // EP values of a row as floats; zeros beyond len
 template <typename T>
-__device__ __forceinline__ void load_part(float (&f)[Mat<T>::EP], const T* src, int e, int len, bool live, int aligned) {
+__device__ __forceinline__ void load_part(float (&f)[Mat<T>::EP], const T* src, int e, int len, bool live, int grain) {
     typename Mat<T>::Frag x = {};
-    if (live) x = global_frag<T, false>(src, e, len, aligned);
+    if (live) x = global_frag<T, false>(src, e, len, grain);
 #pragma unroll
     for (int j = 0; j < Mat<T>::EP; ++j) f[j] = (float)x[j];
 }
 template <typename T>
-__device__ __forceinline__ void store_part(T* dst, const float (&f)[Mat<T>::EP], float scale, int e, int len, int aligned) {
+__device__ __forceinline__ void store_part(T* dst, const float (&f)[Mat<T>::EP], float scale, int e, int len, int grain) {
     typename Mat<T>::Frag x;
 #pragma unroll
     for (int j = 0; j < Mat<T>::EP; ++j) x[j] = (T)(f[j] * scale);
-    if (aligned && e + Mat<T>::EP <= len) {
-        *reinterpret_cast<typename Mat<T>::Frag*>(dst + e) = x;
-    } else {
-#pragma unroll
-        for (int j = 0; j < Mat<T>::EP; ++j)
-            if (e + j < len) dst[e + j] = x[j];
-    }
+    store_chunk<T>(dst + e, x, len - e, grain);
 }
 
 // what a lane holds of a key and its value, still as it came: the next keys' are fetched before the present ones are worked on
@@ -72,13 +66,13 @@ struct Lanes {
 };
 
 template <typename T>
-__device__ __forceinline__ KeyPart<T> fetch(const sgl_diff_attn_args& a, Span span, int32_t j, int hk, const Lanes& ln, int aligned) {
+__device__ __forceinline__ KeyPart<T> fetch(const sgl_diff_attn_args& a, Span span, int32_t j, int hk, const Lanes& ln, int grain) {
     KeyPart<T> x = {};
     x.in = j < span.hi;
     x.see = x.in && (a.key_mask == nullptr || a.key_mask[j]);
     if (x.see) {
-        x.k = global_frag<T, false>(row<T>(a.k, j, 2 * hk + ln.half), ln.e, a.D, aligned);
-        x.v = global_frag<T, false>(row<T>(a.v, j, hk), ln.ev, a.Dv, aligned);
+        x.k = global_frag<T, false>(row<T>(a.k, j, 2 * hk + ln.half), ln.e, a.D, grain);
+        x.v = global_frag<T, false>(row<T>(a.v, j, hk), ln.ev, a.Dv, grain);
     }
     return x;
 }
@@ -98,13 +92,13 @@ __global__ __launch_bounds__(BLOCK) void seg_fwd_kernel(AttnArgs g) {
     const Lanes ln = Lanes::make<L, EP>(lane);
     const float c2 = g.scale < 0.f ? -g.c2 : g.c2;
     float q[EP], o[2][EP], m[2] = {NEG_INF, NEG_INF}, l[2] = {0.f, 0.f};
-    KeyPart<T> next = fetch<T>(a, span, span.lo + ln.slot, hk, ln, g.aligned);
-    load_part<T>(q, row<T>(a.q, i, 2 * h + ln.half), ln.e, a.D, true, g.aligned);
+    KeyPart<T> next = fetch<T>(a, span, span.lo + ln.slot, hk, ln, g.grain);
+    load_part<T>(q, row<T>(a.q, i, 2 * h + ln.half), ln.e, a.D, true, g.grain);
 #pragma unroll
     for (int j = 0; j < EP; ++j) o[0][j] = o[1][j] = 0.f;
     for (int32_t j0 = span.lo; j0 < span.hi; j0 += SLOTS) {
         const KeyPart<T> key = next;
-        next = fetch<T>(a, span, j0 + SLOTS + ln.slot, hk, ln, g.aligned);
+        next = fetch<T>(a, span, j0 + SLOTS + ln.slot, hk, ln, g.grain);
         const bool see = key.see;
         float k[EP], v[EP];
         widen<T>(k, key.k);
@@ -149,10 +143,10 @@ __global__ __launch_bounds__(BLOCK) void seg_fwd_kernel(AttnArgs g) {
     }
     if (ln.slot != 0) return;
     const float lam = a.lam[h];
-    if (a.o2.data) store_part<T>(row_out<T>(a.o2, i, h), o[1], 1.f, ln.ev, a.Dv, g.aligned);
+    if (a.o2.data) store_part<T>(row_out<T>(a.o2, i, h), o[1], 1.f, ln.ev, a.Dv, g.grain);
 #pragma unroll
     for (int e = 0; e < EP; ++e) o[0][e] = __builtin_fmaf(-lam, o[1][e], o[0][e]);
-    store_part<T>(row_out<T>(a.out, i, h), o[0], 1.f, ln.ev, a.Dv, g.aligned);
+    store_part<T>(row_out<T>(a.out, i, h), o[0], 1.f, ln.ev, a.Dv, g.grain);
 }
 
 // DQ: a wave's unit is (sequence, query head), it sums dQ and d_lam's share.  DKV: (sequence, key head), it writes dK and dV,
@@ -178,10 +172,10 @@ __global__ __launch_bounds__(BLOCK) void seg_bwd_kernel(AttnArgs g) {
         auto of_head = [&](int h) {
             float y[EP], y2[EP];
             lam = a.lam[h];
-            load_part<T>(q, row<T>(a.q, i, 2 * h + ln.half), ln.e, a.D, true, g.aligned);
-            load_part<T>(go, row<T>(a.d_out, i, h), ln.ev, a.Dv, true, g.aligned);
-            load_part<T>(y, row<T>(a.out, i, h), ln.ev, a.Dv, true, g.aligned);
-            load_part<T>(y2, row<T>(a.o2, i, h), ln.ev, a.Dv, true, g.aligned);
+            load_part<T>(q, row<T>(a.q, i, 2 * h + ln.half), ln.e, a.D, true, g.grain);
+            load_part<T>(go, row<T>(a.d_out, i, h), ln.ev, a.Dv, true, g.grain);
+            load_part<T>(y, row<T>(a.out, i, h), ln.ev, a.Dv, true, g.grain);
+            load_part<T>(y2, row<T>(a.o2, i, h), ln.ev, a.Dv, true, g.grain);
             t[0] = t[1] = 0.f;
 #pragma unroll
             for (int e = 0; e < EP; ++e) {
@@ -195,12 +189,12 @@ __global__ __launch_bounds__(BLOCK) void seg_bwd_kernel(AttnArgs g) {
         };
 #pragma unroll
         for (int e = 0; e < EP; ++e) dq[e] = 0.f;
-        KeyPart<T> next = fetch<T>(a, span, span.lo + ln.slot, hk, ln, g.aligned);
+        KeyPart<T> next = fetch<T>(a, span, span.lo + ln.slot, hk, ln, g.grain);
         if (DQ || G == 1) of_head(head);
         for (int32_t j0 = span.lo; j0 < span.hi; j0 += SLOTS) {
             const int32_t j = j0 + ln.slot;
             const KeyPart<T> key = next;
-            next = fetch<T>(a, span, j0 + SLOTS + ln.slot, hk, ln, g.aligned);
+            next = fetch<T>(a, span, j0 + SLOTS + ln.slot, hk, ln, g.grain);
             const bool in = key.in, see = key.see;
             float k[EP], v[EP], dk[EP], dv[EP];
             widen<T>(k, key.k);
@@ -236,8 +230,8 @@ __global__ __launch_bounds__(BLOCK) void seg_bwd_kernel(AttnArgs g) {
                 }
             }
             if (DKV && in) {
-                store_part<T>(row_out<T>(a.d_k, j, 2 * hk + ln.half), dk, g.scale, ln.e, a.D, g.aligned);
-                store_part<T>(row_out<T>(a.d_v, j, hk), dv, 1.f, ln.ev, a.Dv, g.aligned);
+                store_part<T>(row_out<T>(a.d_k, j, 2 * hk + ln.half), dk, g.scale, ln.e, a.D, g.grain);
+                store_part<T>(row_out<T>(a.d_v, j, hk), dv, 1.f, ln.ev, a.Dv, g.grain);
             }
         }
         if (DQ) {
@@ -246,7 +240,7 @@ __global__ __launch_bounds__(BLOCK) void seg_bwd_kernel(AttnArgs g) {
 #pragma unroll
                 for (int k = L; k < 64; k <<= 1) dq[e] += __shfl_xor(dq[e], k);
             }
-            if (ln.slot == 0) store_part<T>(row_out<T>(a.d_q, i, 2 * head + ln.half), dq, span.lo < span.hi ? g.scale : 0.f, ln.e, a.D, g.aligned);
+            if (ln.slot == 0) store_part<T>(row_out<T>(a.d_q, i, 2 * head + ln.half), dq, span.lo < span.hi ? g.scale : 0.f, ln.e, a.D, g.grain);
         }
     }
     if (DKV && zero) {
@@ -255,8 +249,8 @@ __global__ __launch_bounds__(BLOCK) void seg_bwd_kernel(AttnArgs g) {
         const float none[EP] = {};
         for (int64_t r = first * SLOTS + ln.slot; r < k0 + (a.Tk - k1); r += stride * SLOTS) {
             const int64_t j = r < k0 ? r : r - k0 + k1;
-            store_part<T>(row_out<T>(a.d_k, j, 2 * hk + ln.half), none, 1.f, ln.e, a.D, g.aligned);
-            store_part<T>(row_out<T>(a.d_v, j, hk), none, 1.f, ln.ev, a.Dv, g.aligned);
+            store_part<T>(row_out<T>(a.d_k, j, 2 * hk + ln.half), none, 1.f, ln.e, a.D, g.grain);
+            store_part<T>(row_out<T>(a.d_v, j, hk), none, 1.f, ln.ev, a.Dv, g.grain);
         }
     }
     if (DQ) {
