@@ -8,8 +8,8 @@
 // type for those products, once each; everything else is fp32.
 //
 // Bound by the matrix and vector instructions of a wave, which alternate in the order written here.  8 sequences of 2048, 16
-// heads over 4, 64 wide, causal, bf16: rows 290 us (0.71 PFLOP/s), keys 436 us (0.63 PFLOP/s); 2 of 4096, 8 over 2, 128 wide:
-// 450 us (0.92) and 900 us (0.61).  A map to a wave, dP formed twice: rows 367 and 507 us.  Keys with dK and dV in waves of their
+// heads over 4, 64 wide, causal, bf16: rows 295 us (0.70 PFLOP/s), keys 455 us (0.60 PFLOP/s); 2 of 4096, 8 over 2, 128 wide:
+// 460 us (0.90) and 757 us (0.73).  A map to a wave, dP formed twice: rows 367 and 507 us.  Keys with dK and dV in waves of their
 // own, scores formed twice: 525 and 1098 us; a map to a wave, dP twice: 517 and 981 us.
 #pragma once
 
@@ -382,18 +382,20 @@ __device__ __forceinline__ void sum_lam(const AttnArgs& g, int h, int32_t row_ti
 // the vector instructions of the phase before (scores of the second map with the exponentials of the first, and so on), so
 // that both kinds overlap within a wave; from 256-byte rows on one wave a SIMD has the registers for that.  At 512 bytes the
 // sums of a wave take half of them; there two waves share the keys, take every other tile and add up at the end, and the keys
-// of the first map come from LDS.
+// of the first map and a quarter of the values come from LDS (or the sums are moved to memory and back in every step).
 template <typename T, int DP>
 struct Keys {
     static constexpr int RB = Shape<T, DP>::RB, SPLIT = RB > 256 ? 2 : 1, SUBS = 2, BQ = 32 * SUBS, TILE = 2 * BQ * RB, STAT = 3 * 256;
     static constexpr int BUF = TILE + SUBS * STAT;              // rows; per 32 of them lse and t of both maps, lam
-    static constexpr int WAVES = 4, GROUPS = WAVES / SPLIT, ROWS = GROUPS * 32, OCC = RB < 256 ? 2 : 1, AHEAD = RB < 256 ? 2 : 4;
+    static constexpr int WAVES = 4, GROUPS = WAVES / SPLIT, ROWS = GROUPS * 32, OCC = RB < 256 ? 2 : 1, AHEAD = RB == 256 ? 4 : 2;
     static constexpr int KEY_LDS = RB > 256;           // maps whose keys are read from LDS
     static constexpr int OWN = KEY_LDS ? ROWS * RB / 2 * KEY_LDS : 16;
+    static constexpr int VAL_LDS = RB > 256 ? Shape<T, DP>::VS / 4 : 0;     // fragments of the values, a lane's beside the next lane's
+    static constexpr int VAL = VAL_LDS ? VAL_LDS * GROUPS * 1024 : 16;
 };
 
 template <typename T, int DP, bool DMA>
-__device__ __forceinline__ void keys_body(const AttnArgs& g, int32_t tiles, char* s_a, char* s_b, char* s_own, uint8_t* s_marks, int* s_lo, int* s_hi, int& s_bad) {
+__device__ __forceinline__ void keys_body(const AttnArgs& g, int32_t tiles, char* s_a, char* s_b, char* s_own, char* s_val, uint8_t* s_marks, int* s_lo, int* s_hi, int& s_bad) {
     typedef Shape<T, DP> S;
     typedef Keys<T, DP> P;
     typedef Mat<T> M;
@@ -421,7 +423,9 @@ __device__ __forceinline__ void keys_body(const AttnArgs& g, int32_t tiles, char
     int32_t lo = s_lo[0], hi = s_hi[0];
 #pragma unroll
     for (int w = 1; w < GROUPS; ++w) lo = min(lo, s_lo[w]), hi = max(hi, s_hi[w]);
-    typename M::Frag k[2][S::QS], v[S::VS];
+    constexpr int V_REGS = S::VS - P::VAL_LDS;
+    typename M::Frag k[2][S::QS], v[V_REGS];
+    int32_t by_val = group * 1024 + lane * 16;
     {
         const int64_t jj = j < a.Tk ? j : 0;
 #pragma unroll
@@ -431,7 +435,12 @@ __device__ __forceinline__ void keys_body(const AttnArgs& g, int32_t tiles, char
         if constexpr (P::KEY_LDS == 2) Stager<T, DP, ROWS, NT, false, true>().load(s_own, halves<T>(a.k, hk, a.D), tile * ROWS, (int32_t)a.Tk - 1, g.grain);
         if constexpr (P::KEY_LDS == 1) Stager<T, DP / 2, ROWS, NT, false, false>().load(s_own, run<T>(a.k, 2 * hk, a.D), tile * ROWS, (int32_t)a.Tk - 1, g.grain);
 #pragma unroll
-        for (int e = 0; e < S::VS; ++e) v[e] = global_frag<T, DMA>(row<T>(a.v, jj, hk), (2 * e + half) * S::EP, a.Dv, g.grain);
+        for (int e = 0; e < V_REGS; ++e) v[e] = global_frag<T, DMA>(row<T>(a.v, jj, hk), (2 * e + half) * S::EP, a.Dv, g.grain);
+        if (P::VAL_LDS && share == 0) {
+#pragma unroll
+            for (int e = 0; e < P::VAL_LDS; ++e)
+                *reinterpret_cast<typename M::Frag*>(s_val + e * GROUPS * 1024 + by_val) = global_frag<T, DMA>(row<T>(a.v, jj, hk), (2 * (V_REGS + e) + half) * S::EP, a.Dv, g.grain);
+        }
     }
     f32x16 dk[2][S::DT], dv[S::VT];
     auto clear = [&]() {
@@ -484,12 +493,12 @@ __device__ __forceinline__ void keys_body(const AttnArgs& g, int32_t tiles, char
         by_col[e] = lane_col<T, RB>(e, lane) + share * 4 * (RB / 128) * 1024;
         asm volatile("" : "+v"(by_col[e]));
     }
-    asm volatile("" : "+v"(by_stat));
+    asm volatile("" : "+v"(by_stat), "+v"(by_val));
     auto of_row = [](const char* tile, const int32_t (&by)[4], int i) { return *reinterpret_cast<const typename M::Frag*>(tile + (i >> 2) * 1024 + by[i & 3]); };
     // 32 rows from i0, the first of which is row `sub` of the tile (beside the wave's share)
-    auto sub_step = [&](const char* buf, int32_t i0, int sub) {
+    auto sub_step = [&](const char* buf, int32_t i0, int sub, auto load_next) {
         i0 += 32 * share + sub;
-        if (i0 >= reach.hi || i0 + 32 <= reach.lo) return;
+        if (i0 >= reach.hi || i0 + 32 <= reach.lo) return load_next();
         constexpr int PS = Operand<T>::PS, QS = S::QS, NK = S::DT * PS;
         constexpr int N1 = QS, N2 = 2 * QS, N3 = N2 + S::VS, N4 = N3 + S::VT * PS, N5 = N4 + NK, N6 = N5 + NK;
         const char* go = buf + BQ * RB + sub * RB;
@@ -525,6 +534,8 @@ __device__ __forceinline__ void keys_body(const AttnArgs& g, int32_t tiles, char
             if (r % 4 == 2 && m == 0) num[r / 4] = *reinterpret_cast<const f32x4*>(stat + 384 + 32 * (r / 4));
         };
         constexpr int FROM_LDS = P::KEY_LDS * QS;
+        auto load_val = [&](int e) { return *reinterpret_cast<const typename M::Frag*>(s_val + e * GROUPS * 1024 + by_val); };
+        Pipe<T, P::VAL_LDS, 2> values;
         Pipe<T, N6, AHEAD> ahead;
         Pipe<T, FROM_LDS, AHEAD> own;
         if constexpr (P::KEY_LDS) own.fill(load_own);
@@ -545,13 +556,23 @@ __device__ __forceinline__ void keys_body(const AttnArgs& g, int32_t tiles, char
             for (int r = 8 * (n - N1) / QS * 2; r < 8 * (n - N1 + 1) / QS * 2; r += 2) exps(0, r, 1.f);
         });
         ahead.template part<N2, N3>(load_n, [&](int n, const typename M::Frag& x) {
-            dp = M::mma(x, v[n - N2], dp);
+            const int u = n - N2;
+            if (P::VAL_LDS && u == V_REGS - 2) values.fill(load_val);
+            if (u < V_REGS) {
+                dp = M::mma(x, v[u], dp);
+            } else {
+                dp = M::mma(x, values.f[(u - V_REGS) % 2], dp);
+                if (u + 2 < S::VS) values.f[(u - V_REGS) % 2] = load_val(u + 2 - V_REGS);
+            }
 #pragma unroll
             for (int r = 8 * (n - N2) / S::VS * 2; r < 8 * (n - N2 + 1) / S::VS * 2; r += 2) {
                 exps(1, r, -lam);
                 p.set2(r, s[0][r] + s[1][r], s[0][r + 1] + s[1][r + 1]);
             }
         });
+        // (what the registers do not hold is read back in the phases above, where it would wait for these loads: at 512 bytes a
+        // row the kernel above takes 985 us with them in front)
+        load_next();
         if (some) p.mask(see);
         ahead.template part<N3, N4>(load_n, [&](int n, const typename M::Frag& x) {
             constexpr int N = N4 - N3;
@@ -573,9 +594,14 @@ __device__ __forceinline__ void keys_body(const AttnArgs& g, int32_t tiles, char
             dk[1][u % S::DT] = M::mma(x, ds[1].f[u / S::DT], dk[1][u % S::DT]);
         });
     };
-    auto step = [&](const char* buf, int32_t i0) {
-#pragma unroll
-        for (int sub = 0; sub < BQ; sub += 32 * P::SPLIT) sub_step(buf, i0, sub);
+    auto step = [&](const char* buf, int32_t i0, auto load_next) {
+        if constexpr (P::SPLIT == 2) {
+            sub_step(buf, i0, 0, load_next);
+        } else {
+            load_next();
+            sub_step(buf, i0, 0, [] {});
+            sub_step(buf, i0, 32, [] {});
+        }
     };
     bool spoilt[2] = {false, false};        // a row with something not finite sees the key: NaN
     if (steps > 0) {
@@ -594,14 +620,16 @@ __device__ __forceinline__ void keys_body(const AttnArgs& g, int32_t tiles, char
             for (int32_t s = 0; s < steps; s += 2) {
                 h = hn, i0 = in;
                 next();
-                if (s + 1 < steps) load(s_b, hn, in);
-                step(s_a, i0);
+                step(s_a, i0, [&] {
+                    if (s + 1 < steps) load(s_b, hn, in);
+                });
                 staged();
                 if (s + 1 >= steps) break;
                 h = hn, i0 = in;
                 next();
-                if (s + 2 < steps) load(s_a, hn, in);
-                step(s_b, i0);
+                step(s_b, i0, [&] {
+                    if (s + 2 < steps) load(s_a, hn, in);
+                });
                 staged();
             }
             if (finite) break;
@@ -653,20 +681,25 @@ __device__ __forceinline__ void keys_body(const AttnArgs& g, int32_t tiles, char
                 for (int e = 0; e < 4; ++e) x[4 * r4 + e] += y[e];
             }
         };
+        // (the ends of the branches differ: merged, they would address the sums, and these would lie in memory from the start)
         if (share) {
 #pragma unroll
             for (int d = 0; d < S::DT; ++d) put(mine + d * 4096, dk[0][d]), put(mine + (S::DT + d) * 4096, dk[1][d]);
+            asm volatile("; keys handed over");
         } else {
 #pragma unroll
             for (int d = 0; d < S::VT; ++d) put(other + d * 4096, dv[d]);
+            asm volatile("; values handed over");
         }
         __syncthreads();
         if (share) {
 #pragma unroll
             for (int d = 0; d < S::VT; ++d) add(other + d * 4096, dv[d]);
+            asm volatile("; values joined");
         } else {
 #pragma unroll
             for (int d = 0; d < S::DT; ++d) add(mine + d * 4096, dk[0][d]), add(mine + (S::DT + d) * 4096, dk[1][d]);
+            asm volatile("; keys joined");
         }
         __syncthreads();
     }
@@ -688,11 +721,12 @@ __global__ __launch_bounds__((Keys<T, DP>::WAVES * 64), (Keys<T, DP>::OCC)) void
     __shared__ __align__(16) char s_a[P::BUF];
     __shared__ __align__(16) char s_b[P::BUF];
     __shared__ __align__(16) char s_own[P::OWN];
+    __shared__ __align__(16) char s_val[P::VAL];
     __shared__ __align__(8) uint8_t s_marks[2 * P::BQ * (P::RB / 16)];
     __shared__ int s_lo[P::WAVES], s_hi[P::WAVES], s_bad;
     const int64_t blocks = ceil_div<int64_t>((int64_t)tiles * g.a.Hk, 8) * 8;
     if ((int64_t)blockIdx.x >= blocks) sum_lam<P::WAVES * 64>(g, (int)(blockIdx.x - blocks), row_tiles, s_a);
-    else keys_body<T, DP, DMA>(g, tiles, s_a, s_b, s_own, s_marks, s_lo, s_hi, s_bad);
+    else keys_body<T, DP, DMA>(g, tiles, s_a, s_b, s_own, s_val, s_marks, s_lo, s_hi, s_bad);
 }
 
 // -------------------------------------------------------------------- owned: keys, rows of 1024 bytes (fp32, heads over 64)
