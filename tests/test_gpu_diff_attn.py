@@ -359,3 +359,50 @@ def test_empty_calls(hot):
     y = diff_attention(*leaves, kp, torch.zeros(2, dtype=torch.long, device="cuda"))
     grads = torch.autograd.grad(y.sum(), leaves)
     assert all(not g.any() for g in grads)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_many_sequences_most_of_them_empty(hot, dtype):
+    """runs of more empty sequences than a wave looks at side by side, thousands of pointers, rows and keys before and behind"""
+    rng = np.random.default_rng(5)
+    B = 5000
+    nq, nk = np.zeros(B, np.int64), np.zeros(B, np.int64)
+    some = rng.choice(B, 120, replace=False)
+    some = some[(some < 1000) | (some > 1300)]
+    nq[some], nk[some] = rng.integers(0, 5, some.size), rng.integers(0, 40, some.size)
+    nq[700:900] = 0
+    q_ptr, k_ptr = _ptr(nq, 3), _ptr(nk, 2)
+    q, k, v, lam, go = _inputs(int(q_ptr[-1]) + 4, int(k_ptr[-1]) + 6, 2, 1, 32, 64, dtype, 7)
+    _check(q, k, v, lam, go, k_ptr, q_ptr)
+    _check(q, k, v, lam, go, k_ptr, q_ptr, causal=True, window=4)
+
+
+def test_a_window_wider_than_any_sequence(hot):
+    q, k, v, lam, _ = _inputs(90, 90, 2, 2, 32, 64, BF16, 3)
+    p = _ptr([40, 50])
+    free = diff_attention(q, k, v, lam, p, p, causal=True)
+    for window in (50, 2 ** 31 - 1, 2 ** 31, 2 ** 62):
+        assert torch.equal(diff_attention(q, k, v, lam, p, p, causal=True, window=window), free)
+
+
+@pytest.mark.parametrize("one_query", [False, True])
+def test_offsets_past_32_bits(hot, one_query):
+    """sequences at the end of tensors of more than 2^31 elements: what stands before them belongs to none"""
+    if torch.cuda.mem_get_info()[0] < 40 << 30:
+        pytest.skip("needs 40 GB")
+    T = (1 << 31) // 512 + 1000
+    nk, nq = [200, 100], [1, 1] if one_query else [200, 100]
+    q, k, v, lam, go = _inputs(sum(nq), 300, 8, 4, 64, 128, BF16, 11)
+    big = [torch.zeros(T, *t.shape[1:], dtype=BF16, device="cuda") for t in (k, v)]
+    for b, t in zip(big, (k, v)):
+        b[-300:] = t
+        b.requires_grad_()
+    leaves = [q.requires_grad_(), *big, lam.requires_grad_()]
+    q_ptr = None if one_query else _ptr(nq)
+    y = diff_attention(*leaves, _ptr(nk, T - 300), q_ptr)
+    got = torch.autograd.grad(y, leaves, go)
+    ref = plain.diff_attention(q, k, v, lam, _ptr(nk), q_ptr, grad=go)
+    _within(y, ref, "out")
+    for name, t in zip(("dq", "dk", "dv", "dlam"), got):
+        _within(t[-300:] if name in ("dk", "dv") else t, ref, name)
+    assert not got[1][:-300].any() and not got[2][:-300].any()
