@@ -179,17 +179,14 @@ struct Mat<float> {
 };
 
 // fp32 results of rows (of the result above) 2 EP s .. 2 EP (s + 1) as the right operand of a step that contracts over
-// them: the registers EP s .. EP s + EP - 1 of a lane, which stand for the rows `row_of(s, j, half)`
+// them: the registers EP s .. EP s + EP - 1 of a lane, which stand for the rows
+// row(s, j, half) = 2 EP s + 8 (j / 4) + 4 half + j % 4
 template <typename T>
 __device__ __forceinline__ typename Mat<T>::Frag to_frag(const f32x16& x, int s) {
     typename Mat<T>::Frag f;
 #pragma unroll
     for (int j = 0; j < Mat<T>::EP; ++j) f[j] = (T)x[s * Mat<T>::EP + j];
     return f;
-}
-template <typename T>
-__device__ __forceinline__ int row_of(int s, int j, int half) {
-    return 2 * Mat<T>::EP * s + 8 * (j / 4) + 4 * half + j % 4;
 }
 
 // LDS image of rows of RB bytes: pieces of 8 rows x 8 chunks (16 bytes each), 1 KB, the pieces of 8 rows side by side.  Row r is
@@ -218,7 +215,7 @@ __device__ __forceinline__ typename Mat<T>::Frag map_frag(const char* tile, int 
     else return map ? row_frag<T, RB>(tile, row0, col, i + 2, half) : row_frag<T, RB>(tile, row0, col, i, half);
 }
 
-// column fragment: elements (row0 + row_of(s, j, half), 32 t + lane column), row0 a multiple of 16: the transposed left operand
+// column fragment: elements (row0 + row(s, j, half), 32 t + lane column), row0 a multiple of 16: the transposed left operand
 // whose 32 rows are the 32 elements from 32 t of the tile's rows
 template <typename T, int RB>
 __device__ __forceinline__ typename Mat<T>::Frag col_frag(const char* tile, int row0, int s, int t, int lane) {

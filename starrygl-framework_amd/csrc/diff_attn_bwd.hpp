@@ -84,17 +84,6 @@ __device__ __forceinline__ void add_product(f32x16 (&acc)[N], const char* tile, 
     ahead.drain(load, [&](int n, const typename M::Frag& f) { acc[n % N] = M::mma(f, x.f[n / N], acc[n % N]); });
 }
 
-// the same over half `map` of a head
-template <typename T, int RB, int N, int AHEAD>
-__device__ __forceinline__ void add_map(f32x16 (&acc)[N], const char* tile, int row0, int map, const Operand<T>& x, int lane) {
-    if constexpr (RB >= 256 && (N & 1) == 0) {
-        add_product<T, RB, N, AHEAD>(acc, tile + map * (RB / 256) * 1024, row0, 0, x, lane);
-    } else {
-        if (map) add_product<T, RB, N, AHEAD>(acc, tile, row0, N, x, lane);
-        else add_product<T, RB, N, AHEAD>(acc, tile, row0, 0, x, lane);
-    }
-}
-
 // ---------------------------------------------------------------------------------------------- owned: query rows
 // A wave owns 32 rows of a head: both maps' scores, dP and dQ of a tile of 32 keys, the products between the vector
 // instructions of the phase before, as above.
@@ -730,18 +719,20 @@ __global__ __launch_bounds__((Keys<T, DP>::WAVES * 64), (Keys<T, DP>::OCC)) void
 }
 
 // -------------------------------------------------------------------- owned: keys, rows of 1024 bytes (fp32, heads over 64)
-// Two waves share 32 keys: one sums dK, the other dV, each computes the scores (the sums of both do not fit a wave's
-// registers); keys and values are read from LDS, whose rest holds one tile of rows.
+// Four waves share 32 keys: two sum a map's dK each, two half of dV's columns; each computes the scores that it needs, the former
+// dP too (no wave's registers hold more of the sums).  Keys and values are read from LDS, whose rest holds one tile of rows.
+// 8 sequences of 1024, 8 heads 128 wide, causal: 1306 us; two waves, one for dK and one for dV, 1834.
 template <typename T, int DP>
 struct Roles {
-    static constexpr int RB = Shape<T, DP>::RB, WAVES = 2, ROWS = 32, BQ = 32, TILE = 2 * BQ * RB;
-    static constexpr int STAT = BQ * 4 * 4;                     // lse and t of a row, two each
+    static constexpr int RB = Shape<T, DP>::RB, WAVES = 4, ROWS = 32, BQ = 32, TILE = 2 * BQ * RB;
+    static constexpr int STAT = 2 * 256;                        // lse and t of the rows, map by map
     static constexpr int BUF = TILE + STAT, OWN = 2 * ROWS * RB;
+    static_assert(sizeof(T) == 4 && RB >= 256, "a tile of 32 values is a piece of the image");
 };
 
-// DK, DV: what this wave sums
-template <typename T, int DP, bool DMA, bool DK, bool DV>
-__device__ __forceinline__ void roles_body(const AttnArgs& g, int32_t tiles, char* s_a, char* s_own, uint8_t* s_marks, int& s_bad) {
+// DK: this wave sums dK of map `part`; else half `part` of dV's columns
+template <typename T, int DP, bool DMA, bool DK>
+__device__ __forceinline__ void roles_body(const AttnArgs& g, int32_t tiles, char* s_a, char* s_own, uint8_t* s_marks, int& s_bad, int part) {
     typedef Shape<T, DP> S;
     typedef Roles<T, DP> P;
     typedef Mat<T> M;
@@ -763,27 +754,23 @@ __device__ __forceinline__ void roles_body(const AttnArgs& g, int32_t tiles, cha
     Reach reach = reach_of(rows);
     if (!__all(shown)) reach.to = 0;
     if (threadIdx.x == 0) s_bad = 0;
-    const int32_t lo = reach.lo, hi = reach.hi;                 // (both waves have the same keys)
+    const int32_t lo = reach.lo, hi = reach.hi;                 // (the waves have the same keys)
     Stager<T, DP, ROWS, NT, false, true>().load(s_own, halves<T>(a.k, hk, a.D), j0, (int32_t)a.Tk - 1, g.grain);
     Stager<T, DP, ROWS, NT, false, false>().load(s_own + ROWS * RB, run<T>(a.v, hk, a.Dv), j0, (int32_t)a.Tk - 1, g.grain);
-    f32x16 dk[2][S::DT], dv[S::VT];
+    constexpr int N = DK ? S::DT : S::VT / 2;                   // 32-wide tiles of the sum
+    f32x16 acc[N];
     auto clear = [&]() {
 #pragma unroll
-        for (int m = 0; m < 2; ++m)
-#pragma unroll
-            for (int d = 0; d < S::DT; ++d) dk[m][d] = zero16();
-#pragma unroll
-        for (int d = 0; d < S::VT; ++d) dv[d] = zero16();
+        for (int d = 0; d < N; ++d) acc[d] = zero16();
     };
     clear();
     const int32_t last = (int32_t)a.Tq - 1;
     const float c2 = signed_c2(g);
     const int32_t per_head = lo < hi ? (hi - lo + BQ - 1) / BQ : 0, steps = per_head * G;      // head by head, row tile by row tile
     auto load_stats = [&](char* buf, int h, int32_t i0) {
-        // 64 numbers each: (lse_1, lse_2) and (t_1, t_2) of the rows
-        {
-            const int32_t i = min(i0 + (lane >> 1), last);
-            const float* src = (wave ? g.delta : a.lse) + ((int64_t)i * a.Hq + h) * 2 + (lane & 1);
+        if (wave < 2) {
+            const int32_t i = min(i0 + (lane & 31), last);
+            const float* src = (wave ? g.delta : a.lse) + ((int64_t)i * a.Hq + h) * 2 + (lane >> 5);
             const int at0 = __builtin_amdgcn_readfirstlane(wave * 256);
             __builtin_amdgcn_global_load_lds((SGL_GLOBAL void*)src, (SGL_LDS void*)(buf + TILE + at0), 4, 0, 0);
         }
@@ -806,62 +793,48 @@ __device__ __forceinline__ void roles_body(const AttnArgs& g, int32_t tiles, cha
     auto step = [&](const char* buf, int h, int32_t i0) {
         if (i0 >= reach.hi || i0 + BQ <= reach.lo) return;
         const float lam = a.lam[h];
-        const float* stat = reinterpret_cast<const float*>(buf + TILE);
+        const float* stat = reinterpret_cast<const float*>(buf + TILE) + 4 * half;
+        const char* go = buf + BQ * RB;
         f32x16 s[2], dp;
-        s[0] = s[1] = zero16();
-        if constexpr (DK) dp = zero16();
-        // fragments of the walked rows: the two halves of the queries, then (for dK) d_out; owned ones from LDS ride along
-        auto load_row = [&](int n) {
-            return n < 2 * S::QS ? row_frag<T, RB>(buf, 0, col, n, half) : row_frag<T, RB>(buf + BQ * RB, 0, col, n - 2 * S::QS, half);
+        s[0] = s[1] = dp = zero16();
+        // fragments of the walked rows: a half of the queries and d_out, or both halves; those of the owned rows ride along
+        auto load = [&](const char* rows2, int n) {
+            if (n >= S::QS && DK) return row_frag<T, RB>(rows2 + BQ * RB, 0, col, n - S::QS, half);
+            return map_frag<T, RB>(rows2, 0, col, DK ? part : n / S::QS, n % S::QS, half);
         };
-        auto load_own = [&](int n) {
-            return n < 2 * S::QS ? row_frag<T, RB>(s_own, 0, col, n, half) : row_frag<T, RB>(s_own + ROWS * RB, 0, col, n - 2 * S::QS, half);
-        };
-        constexpr int FRAGS = 2 * S::QS + (DK ? S::VS : 0);
+        auto load_row = [&](int n) { return load(buf, n); };
+        auto load_own = [&](int n) { return load(s_own, n); };
+        constexpr int FRAGS = S::QS + (DK ? S::VS : S::QS);
         Pipe<T, FRAGS, AHEAD> ahead, own;
         own.fill(load_own);
         ahead.fill(load_row);
         ahead.drain(load_row, [&](int n, const typename M::Frag& f) {
-            f32x16& to = n < S::QS ? s[0] : n < 2 * S::QS ? s[1] : dp;
+            f32x16& to = n < S::QS ? s[0] : DK ? dp : s[1];
             to = M::mma(f, own.f[n % AHEAD], to);
             if (n + AHEAD < FRAGS) own.f[n % AHEAD] = load_own(n + AHEAD);
         });
-        f32x16 x;               // P_1 - lam P_2
+        // dS of the map (the second's times -lam), or P_1 - lam P_2
+        const float weight = DK && part == 0 ? 1.f : -lam;
 #pragma unroll
         for (int r4 = 0; r4 < 4; ++r4) {
-            const int r0 = 8 * r4 + 4 * half;
-            f32x4 l[2], t[2];
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                l[u] = *reinterpret_cast<const f32x4*>(stat + 2 * (r0 + 2 * u));
-                if (DK) t[u] = *reinterpret_cast<const f32x4*>(stat + 64 + 2 * (r0 + 2 * u));
-            }
+            const f32x4 l = *reinterpret_cast<const f32x4*>(stat + (DK ? 32 * part : 0) + 8 * r4);
+            const f32x4 u = *reinterpret_cast<const f32x4*>(stat + (DK ? 64 + 32 * part : 32) + 8 * r4);      // t, or the second map's lse
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                const int r = 4 * r4 + e, u = 2 * (e % 2);
-                const float p0 = exp2_hw(__builtin_fmaf(s[0][r], c2, -l[e / 2][u])), p1 = -lam * exp2_hw(__builtin_fmaf(s[1][r], c2, -l[e / 2][u + 1]));
-                if constexpr (DK) {
-                    s[0][r] = p0 * (dp[r] - t[e / 2][u]);
-                    s[1][r] = p1 * (dp[r] - t[e / 2][u + 1]);
-                }
-                if constexpr (DV) x[r] = p0 + p1;
+                const int r = 4 * r4 + e;
+                const float p = exp2_hw(__builtin_fmaf(s[0][r], c2, -l[e]));
+                if constexpr (DK) s[0][r] = weight * p * (dp[r] - u[e]);
+                else s[0][r] = __builtin_fmaf(weight, exp2_hw(__builtin_fmaf(s[1][r], c2, -u[e])), p);
             }
         }
         if (!(i0 >= reach.from && i0 + BQ <= reach.to)) {
             const uint32_t see = span_bits(i0, rows) >> (4 * half);
 #pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                if constexpr (DK) s[0][r] = row_bit(see, r) ? s[0][r] : 0.f, s[1][r] = row_bit(see, r) ? s[1][r] : 0.f;
-                if constexpr (DV) x[r] = row_bit(see, r) ? x[r] : 0.f;
-            }
+            for (int r = 0; r < 16; ++r) s[0][r] = row_bit(see, r) ? s[0][r] : 0.f;
         }
-        if constexpr (DV) add_product<T, RB, S::VT, AHEAD>(dv, buf + BQ * RB, 0, 0, operand<T>(x), lane);
-        if constexpr (DK) {
-            add_map<T, RB, S::DT, AHEAD>(dk[0], buf, 0, 0, operand<T>(s[0]), lane);
-            add_map<T, RB, S::DT, AHEAD>(dk[1], buf, 0, 1, operand<T>(s[1]), lane);
-        }
+        add_product<T, RB, N, AHEAD>(acc, (DK ? buf : go) + part * N * 1024, 0, 0, operand<T>(s[0]), lane);
     };
-    bool spoilt[2] = {false, false};        // a row with something not finite sees the key: NaN
+    bool spoilt = false;                    // (dK) a row with something not finite sees the key: NaN
     if (steps > 0) {
         int hn;                             // head and first row of the tile
         int32_t in;
@@ -883,10 +856,7 @@ __device__ __forceinline__ void roles_body(const AttnArgs& g, int32_t tiles, cha
                 staged();
             }
             if (finite) break;
-            bool bad = false;
-            if constexpr (DK) bad = any_nan(dk[0]) || any_nan(dk[1]);
-            if constexpr (DV) bad = bad || any_nan(dv);
-            if (bad && shown) s_bad = 1;
+            if (any_nan(acc) && shown) s_bad = 1;
             __syncthreads();
             if (!s_bad) break;
             finite = true;
@@ -906,11 +876,8 @@ __device__ __forceinline__ void roles_body(const AttnArgs& g, int32_t tiles, cha
                     if (in + r < rows.lo || in + r >= rows.hi) continue;
                     const uint8_t* of_out = s_marks + BQ * (RB / 16);
                     const bool o = marked_any<RB>(of_out, r, 0, RB / 16);
-                    spoilt[0] = spoilt[0] || o || marked_any<RB>(s_marks, r, 0, RB / 32);
-                    spoilt[1] = spoilt[1] || o || marked_any<RB>(s_marks, r, RB / 32, RB / 16);
-                    if constexpr (DV) {
-                        if (o) spoil<T, RB, S::VT>(dv, of_out, r, half);
-                    }
+                    if constexpr (DK) spoilt = spoilt || o || marked_any<RB>(s_marks, r, part * (RB / 32), (part + 1) * (RB / 32));
+                    else if (o) spoil<T, RB, N>(acc, of_out + part * N * 8, r, half);
                 }
                 next();
             }
@@ -921,14 +888,12 @@ __device__ __forceinline__ void roles_body(const AttnArgs& g, int32_t tiles, cha
     // the walked side's tiles are free: the last barrier is behind every wave's last look at them
     char* box = s_a + wave * (TILE / P::WAVES);
     constexpr int PIECE = TILE / P::WAVES / 32;               // bytes of a row at a time
-    if constexpr (DK) {
-        store_rows<T, PIECE, S::DT, DMA>([&](int t, int r) { return spoilt[0] ? NAN : shown ? dk[0][t][r] * g.scale : 0.f; }, box, lane, a.D, g.grain,
-                                         row_out<T>(a.d_k, j0, 2 * hk), a.d_k.row_stride, keep);
-        store_rows<T, PIECE, S::DT, DMA>([&](int t, int r) { return spoilt[1] ? NAN : shown ? dk[1][t][r] * g.scale : 0.f; }, box, lane, a.D, g.grain,
-                                         row_out<T>(a.d_k, j0, 2 * hk + 1), a.d_k.row_stride, keep);
-    }
-    if constexpr (DV)
-        store_rows<T, PIECE, S::VT, DMA>([&](int t, int r) { return shown ? dv[t][r] : 0.f; }, box, lane, a.Dv, g.grain, row_out<T>(a.d_v, j0, hk), a.d_v.row_stride, keep);
+    if constexpr (DK)
+        store_rows<T, PIECE, N, DMA>([&](int d, int r) { return spoilt ? NAN : shown ? acc[d][r] * g.scale : 0.f; }, box, lane, a.D, g.grain,
+                                     row_out<T>(a.d_k, j0, 2 * hk + part), a.d_k.row_stride, keep);
+    else
+        store_rows<T, PIECE, N, DMA>([&](int d, int r) { return shown ? acc[d][r] : 0.f; }, box, lane, a.Dv - part * N * 32, g.grain,
+                                     row_out<T>(a.d_v, j0, hk) + part * N * 32, a.d_v.row_stride, keep);
 }
 
 template <typename T, int DP, bool DMA>
@@ -940,9 +905,9 @@ __global__ __launch_bounds__((Roles<T, DP>::WAVES * 64), 1) void bwd_roles_kerne
     __shared__ int s_bad;
     const int64_t blocks = ceil_div<int64_t>((int64_t)tiles * g.a.Hk, 8) * 8;
     if ((int64_t)blockIdx.x >= blocks) return sum_lam<P::WAVES * 64>(g, (int)(blockIdx.x - blocks), row_tiles, s_a);
-    // (the waves of a SIMD take both roles: waves go to the four SIMDs in turn)
-    if (((int)(threadIdx.x >> 6) == 0) == ((blockIdx.x >> 3) % 2 == 0)) roles_body<T, DP, DMA, true, false>(g, tiles, s_a, s_own, s_marks, s_bad);
-    else roles_body<T, DP, DMA, false, true>(g, tiles, s_a, s_own, s_marks, s_bad);
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    if (wave < 2) roles_body<T, DP, DMA, true>(g, tiles, s_a, s_own, s_marks, s_bad, wave);
+    else roles_body<T, DP, DMA, false>(g, tiles, s_a, s_own, s_marks, s_bad, wave - 2);
 }
 
 template <typename T, int DP>
