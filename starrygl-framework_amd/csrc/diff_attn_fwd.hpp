@@ -81,7 +81,7 @@ __device__ __forceinline__ void step(State<T, DP, MAPS>& st, const typename Mat<
     typedef Mat<T> M;
     constexpr int RB = S::RB;
     const int half = lane >> 5, col = lane & 31;
-    constexpr int AHEAD = MAPS == 2 ? 2 : 4;                    // (each feeds MAPS products of the values)
+    constexpr int AHEAD = MAPS == 2 || RB > 512 ? 2 : 4;        // (each feeds MAPS products of the values)
     f32x16 s[MAPS];
 #pragma unroll
     for (int c = 0; c < MAPS; ++c) s[c] = zero16();
