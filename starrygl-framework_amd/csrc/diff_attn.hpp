@@ -4,6 +4,8 @@
 
 #include <math.h>
 
+#include <initializer_list>
+
 #include "common.hpp"
 
 namespace sgl {
@@ -14,6 +16,9 @@ constexpr float NEG_INF = -INFINITY;
 constexpr float LOG2E = 1.44269504088896340736f;
 
 constexpr int QUERY_ROWS = 128;     // query rows of a block of the backward pass (a sum of t_2 in the workspace each)
+
+// How rows come into LDS: through registers, whole (as wide as the image), or padded (narrower, in whole 16-byte chunks)
+enum { BY_REGISTERS, WHOLE_ROWS, PADDED };
 
 struct AttnArgs {
     sgl_diff_attn_args a;
@@ -392,9 +397,11 @@ __device__ __forceinline__ bool row_bit(uint32_t bits, int r) { return (bits >> 
 // Staging of ROWS rows from row0 (rows beyond `last` repeat it: their columns are hidden) into the image of RB-byte rows by NT
 // threads.  DMA: every chunk is whole and aligned, and goes from memory to LDS without passing through registers (a
 // wave's 64 chunks land side by side, a piece, so the exchange is applied to what each lane fetches); complete after
-// staged().  Otherwise through registers, with zeros behind a row's valid elements.
-template <typename T, int DP, int ROWS, int NT, bool DMA, bool TWO>
+// staged().  PADDED: lanes whose chunk lies behind a row's valid elements bring nothing, and what they would write has been zero
+// since the caller cleared the image.  Otherwise through registers, with zeros behind a row's valid elements.
+template <typename T, int DP, int ROWS, int NT, int MODE, bool TWO>
 struct Stager {
+    static constexpr bool DMA = MODE != BY_REGISTERS, PAD = MODE == PADDED;
     static constexpr int RB = 2 * DP * (int)sizeof(T), CH = RB / 16, EP = 16 / (int)sizeof(T);
     static constexpr int NW = NT / 64, PG = CH / 8;             // waves; pieces side by side
     static_assert(NW % PG == 0 || PG % NW == 0, "a wave covers whole columns or walks whole rows of pieces");
@@ -402,6 +409,7 @@ struct Stager {
     static constexpr int COLS = PG > NW ? PG / NW : 1;          // columns of pieces that a wave walks through
     static constexpr int KINDS = PG >= NW ? 2 : 1;              // rows of pieces of both parities, or of the wave's own
     int32_t off[COLS][KINDS];
+    bool on[COLS][KINDS];
 
     // row in its tile and chunk of what lane `lane` of piece `piece` brings
     static __device__ __forceinline__ void of_piece(int piece, int lane, int& r, int& c) {
@@ -412,6 +420,7 @@ struct Stager {
     static __device__ __forceinline__ int64_t element(const Source& s, int r, int c) {
         return r * s.row_stride + (TWO ? c / (CH / 2) * s.half_stride + c % (CH / 2) * EP : c * EP);
     }
+    static __device__ __forceinline__ bool valid(const Source& s, int c) { return (TWO ? c % (CH / 2) : c) * EP < s.len; }
     __device__ __forceinline__ void plan(const Source& s) {
         if constexpr (DMA) {
             const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -422,6 +431,7 @@ struct Stager {
                     int r, c;
                     of_piece(q * PG + p * NW + wave, lane, r, c);           // (PG > NW: wave < NW; else p = 0)
                     off[p][q] = (int32_t)((element(s, r, c) - q * 8 * s.row_stride) * (int64_t)sizeof(T));
+                    on[p][q] = !PAD || valid(s, c);
                 }
         }
     }
@@ -437,7 +447,7 @@ struct Stager {
 #pragma unroll
                 for (int k = 0; k < ROWS * CH / NT; ++k) {
                     const int at0 = __builtin_amdgcn_readfirstlane((k * NW + wave) * 1024);
-                    __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (SGL_LDS void*)(tile + at0), 16, off[k % COLS][KINDS == 2 ? k / COLS & 1 : 0], k / COLS * step, 0, 0);
+                    if (!PAD || on[k % COLS][KINDS == 2 ? k / COLS & 1 : 0]) __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (SGL_LDS void*)(tile + at0), 16, off[k % COLS][KINDS == 2 ? k / COLS & 1 : 0], k / COLS * step, 0, 0);
                 }
 #endif
             } else {
@@ -450,7 +460,7 @@ struct Stager {
                     const int32_t n = row0 + r < last ? row0 + r : last;
                     const T* src = static_cast<const T*>(s.data) + (int64_t)n * s.row_stride + element(s, 0, c);
                     const int at0 = __builtin_amdgcn_readfirstlane(piece * 1024);
-                    __builtin_amdgcn_global_load_lds((SGL_GLOBAL void*)src, (SGL_LDS void*)(tile + at0), 16, 0, 0);
+                    if (!PAD || valid(s, c)) __builtin_amdgcn_global_load_lds((SGL_GLOBAL void*)src, (SGL_LDS void*)(tile + at0), 16, 0, 0);
                 }
             }
         } else {
@@ -529,6 +539,14 @@ __device__ __forceinline__ void spoil(f32x16 (&x)[N], const uint8_t* marks, int 
 __device__ __forceinline__ void staged() {
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
+}
+
+// clears an image whose padding no load will write
+template <int MODE, int BYTES, int NT>
+__device__ __forceinline__ void clear_image(char* tile) {
+    if constexpr (MODE == PADDED) {
+        for (int i = threadIdx.x * 16; i < BYTES; i += NT * 16) *reinterpret_cast<uint4*>(tile + i) = uint4{0, 0, 0, 0};
+    }
 }
 
 // EP elements from element e of a row, kept in registers; zero beyond len.  WHOLE: every chunk is whole and aligned.
@@ -644,6 +662,13 @@ void seg_forward(const AttnArgs& g, hipStream_t st);
 void seg_backward(const AttnArgs& g, hipStream_t st);
 // rows whose offsets inside a tile of 64 fit 31 bits: up to 2^21 elements from row to row, 2^24 from half to half
 inline bool dma_rows(const sgl_rows& r) { return r.row_stride >= 0 && r.row_stride <= (1 << 21) && r.head_stride >= 0 && r.head_stride <= (1 << 24); }
+// How the matrix kernels of head width DP bring their rows in.  Training step of 8 sequences of 1024, 8 heads of 100 in fp32, causal:
+// padded rows 3170 us, the same through registers 4230.
+inline int stage_mode(const AttnArgs& g, int DP, std::initializer_list<const sgl_rows*> staged) {
+    bool direct = g.grain == 16;
+    for (const sgl_rows* r : staged) direct = direct && dma_rows(*r);
+    return !direct ? BY_REGISTERS : g.a.D == DP && g.a.Dv == 2 * DP ? WHOLE_ROWS : PADDED;
+}
 template <typename T>
 void forward_type(const AttnArgs& g, hipStream_t st);
 template <typename T>

@@ -94,7 +94,7 @@ struct Rows {
     static_assert(ROWS == WAVES * 32, "the row tiles of the workspace");
 };
 
-template <typename T, int DP, bool DMA>
+template <typename T, int DP, int MODE>
 __global__ __launch_bounds__((Rows<T, DP>::WAVES * 64), (Rows<T, DP>::OCC)) void bwd_rows_kernel(AttnArgs g, int32_t tiles) {
     typedef Shape<T, DP> S;
     typedef Rows<T, DP> P;
@@ -127,6 +127,8 @@ __global__ __launch_bounds__((Rows<T, DP>::WAVES * 64), (Rows<T, DP>::OCC)) void
     if (a.key_mask) reach.to = 0;
     if (lane == 0) s_lo[wave] = reach.lo, s_hi[wave] = reach.hi;
     if (threadIdx.x == 0) s_bad = 0;
+    clear_image<MODE, P::TILE, NT>(s_a);
+    clear_image<MODE, P::TILE, NT>(s_b);
     __syncthreads();
     int32_t lo = s_lo[0], hi = s_hi[0];
 #pragma unroll
@@ -140,13 +142,13 @@ __global__ __launch_bounds__((Rows<T, DP>::WAVES * 64), (Rows<T, DP>::OCC)) void
 #pragma unroll
     for (int m = 0; m < 2; ++m)
 #pragma unroll
-        for (int k = 0; k < S::QS; ++k) q[m][k] = global_frag<T, DMA>(row<T>(a.q, ii, 2 * h + m), (2 * k + half) * S::EP, a.D, g.grain);
+        for (int k = 0; k < S::QS; ++k) q[m][k] = global_frag<T, MODE == WHOLE_ROWS>(row<T>(a.q, ii, 2 * h + m), (2 * k + half) * S::EP, a.D, g.grain);
 #pragma unroll
     for (int k = 0; k < S::VS; ++k) {
         const int e = (2 * k + half) * S::EP;
-        go[k] = global_frag<T, DMA>(row<T>(a.d_out, ii, h), e, a.Dv, g.grain);
-        const typename M::Frag y2 = global_frag<T, DMA>(row<T>(a.o2, ii, h), e, a.Dv, g.grain);
-        const typename M::Frag y = global_frag<T, DMA>(row<T>(a.out, ii, h), e, a.Dv, g.grain);
+        go[k] = global_frag<T, MODE == WHOLE_ROWS>(row<T>(a.d_out, ii, h), e, a.Dv, g.grain);
+        const typename M::Frag y2 = global_frag<T, MODE == WHOLE_ROWS>(row<T>(a.o2, ii, h), e, a.Dv, g.grain);
+        const typename M::Frag y = global_frag<T, MODE == WHOLE_ROWS>(row<T>(a.out, ii, h), e, a.Dv, g.grain);
 #pragma unroll
         for (int j = 0; j < S::EP; ++j) {
             t[0] = __builtin_fmaf((float)go[k][j], __builtin_fmaf(lam, (float)y2[j], (float)y[j]), t[0]);
@@ -174,8 +176,8 @@ __global__ __launch_bounds__((Rows<T, DP>::WAVES * 64), (Rows<T, DP>::OCC)) void
     };
     clear();
     const float c2 = __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(signed_c2(g))));
-    Stager<T, DP, BN, NT, DMA, true> stage_k;
-    Stager<T, DP, BN, NT, DMA, false> stage_v;
+    Stager<T, DP, BN, NT, MODE, true> stage_k;
+    Stager<T, DP, BN, NT, MODE, false> stage_v;
     stage_k.plan(ks);
     stage_v.plan(vs);
     bool finite = false;        // the pass without what is not finite
@@ -323,9 +325,9 @@ __global__ __launch_bounds__((Rows<T, DP>::WAVES * 64), (Rows<T, DP>::OCC)) void
     char* box = (wave & 1 ? s_b : s_a) + (wave >> 1) * (P::TILE / 2);
     constexpr int PIECE = RB / 2;                               // bytes of a row at a time
     const float f0 = g.scale, f1 = -lam * g.scale;
-    store_rows<T, PIECE, S::DT, DMA>([&](int d, int r) { return spoilt[0] ? NAN : live ? dq[0][d][r] * f0 : 0.f; }, box, lane, a.D, g.grain, row_out<T>(a.d_q, i0, 2 * h),
+    store_rows<T, PIECE, S::DT, MODE == WHOLE_ROWS>([&](int d, int r) { return spoilt[0] ? NAN : live ? dq[0][d][r] * f0 : 0.f; }, box, lane, a.D, g.grain, row_out<T>(a.d_q, i0, 2 * h),
                                      a.d_q.row_stride, keep);
-    store_rows<T, PIECE, S::DT, DMA>([&](int d, int r) { return spoilt[1] ? NAN : live ? dq[1][d][r] * f1 : 0.f; }, box, lane, a.D, g.grain, row_out<T>(a.d_q, i0, 2 * h + 1),
+    store_rows<T, PIECE, S::DT, MODE == WHOLE_ROWS>([&](int d, int r) { return spoilt[1] ? NAN : live ? dq[1][d][r] * f1 : 0.f; }, box, lane, a.D, g.grain, row_out<T>(a.d_q, i0, 2 * h + 1),
                                      a.d_q.row_stride, keep);
 }
 
@@ -383,7 +385,7 @@ struct Keys {
     static constexpr int VAL = VAL_LDS ? VAL_LDS * GROUPS * 1024 : 16;
 };
 
-template <typename T, int DP, bool DMA>
+template <typename T, int DP, int MODE>
 __device__ __forceinline__ void keys_body(const AttnArgs& g, int32_t tiles, char* s_a, char* s_b, char* s_own, char* s_val, uint8_t* s_marks, int* s_lo, int* s_hi, int& s_bad) {
     typedef Shape<T, DP> S;
     typedef Keys<T, DP> P;
@@ -408,6 +410,8 @@ __device__ __forceinline__ void keys_body(const AttnArgs& g, int32_t tiles, char
     if (!__all(shown)) reach.to = 0;
     if (lane == 0) s_lo[wave] = reach.lo, s_hi[wave] = reach.hi;
     if (threadIdx.x == 0) s_bad = 0;
+    clear_image<MODE, TILE, NT>(s_a);
+    clear_image<MODE, TILE, NT>(s_b);
     __syncthreads();
     int32_t lo = s_lo[0], hi = s_hi[0];
 #pragma unroll
@@ -420,15 +424,15 @@ __device__ __forceinline__ void keys_body(const AttnArgs& g, int32_t tiles, char
 #pragma unroll
         for (int m = P::KEY_LDS; m < 2; ++m)
 #pragma unroll
-            for (int e = 0; e < S::QS; ++e) k[m][e] = global_frag<T, DMA>(row<T>(a.k, jj, 2 * hk + m), (2 * e + half) * S::EP, a.D, g.grain);
-        if constexpr (P::KEY_LDS == 2) Stager<T, DP, ROWS, NT, false, true>().load(s_own, halves<T>(a.k, hk, a.D), tile * ROWS, (int32_t)a.Tk - 1, g.grain);
-        if constexpr (P::KEY_LDS == 1) Stager<T, DP / 2, ROWS, NT, false, false>().load(s_own, run<T>(a.k, 2 * hk, a.D), tile * ROWS, (int32_t)a.Tk - 1, g.grain);
+            for (int e = 0; e < S::QS; ++e) k[m][e] = global_frag<T, MODE == WHOLE_ROWS>(row<T>(a.k, jj, 2 * hk + m), (2 * e + half) * S::EP, a.D, g.grain);
+        if constexpr (P::KEY_LDS == 2) Stager<T, DP, ROWS, NT, BY_REGISTERS, true>().load(s_own, halves<T>(a.k, hk, a.D), tile * ROWS, (int32_t)a.Tk - 1, g.grain);
+        if constexpr (P::KEY_LDS == 1) Stager<T, DP / 2, ROWS, NT, BY_REGISTERS, false>().load(s_own, run<T>(a.k, 2 * hk, a.D), tile * ROWS, (int32_t)a.Tk - 1, g.grain);
 #pragma unroll
-        for (int e = 0; e < V_REGS; ++e) v[e] = global_frag<T, DMA>(row<T>(a.v, jj, hk), (2 * e + half) * S::EP, a.Dv, g.grain);
+        for (int e = 0; e < V_REGS; ++e) v[e] = global_frag<T, MODE == WHOLE_ROWS>(row<T>(a.v, jj, hk), (2 * e + half) * S::EP, a.Dv, g.grain);
         if (P::VAL_LDS && share == 0) {
 #pragma unroll
             for (int e = 0; e < P::VAL_LDS; ++e)
-                *reinterpret_cast<typename M::Frag*>(s_val + e * GROUPS * 1024 + by_val) = global_frag<T, DMA>(row<T>(a.v, jj, hk), (2 * (V_REGS + e) + half) * S::EP, a.Dv, g.grain);
+                *reinterpret_cast<typename M::Frag*>(s_val + e * GROUPS * 1024 + by_val) = global_frag<T, MODE == WHOLE_ROWS>(row<T>(a.v, jj, hk), (2 * (V_REGS + e) + half) * S::EP, a.Dv, g.grain);
         }
     }
     f32x16 dk[2][S::DT], dv[S::VT];
@@ -444,8 +448,8 @@ __device__ __forceinline__ void keys_body(const AttnArgs& g, int32_t tiles, char
     const float c2 = __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(signed_c2(g))));
     const int32_t last = (int32_t)a.Tq - 1;
     const int32_t per_head = lo < hi ? (hi - lo + BQ - 1) / BQ : 0, steps = per_head * G;      // head by head, row tile by row tile
-    Stager<T, DP, BQ, NT, DMA, true> stage_q;
-    Stager<T, DP, BQ, NT, DMA, false> stage_go;
+    Stager<T, DP, BQ, NT, MODE, true> stage_q;
+    Stager<T, DP, BQ, NT, MODE, false> stage_go;
     stage_q.plan(halves<T>(a.q, 0, a.D));
     stage_go.plan(run<T>(a.d_out, 0, a.Dv));
     bool finite = false;        // the pass without what is not finite
@@ -695,16 +699,16 @@ __device__ __forceinline__ void keys_body(const AttnArgs& g, int32_t tiles, char
     constexpr int PIECE = TILE / P::WAVES / 32;                 // bytes of a row at a time
     char* box = s_a + wave * (TILE / P::WAVES);
     if (P::SPLIT == 1 || !share) {
-        store_rows<T, PIECE, S::DT, DMA>([&](int t, int r) { return spoilt[0] ? NAN : shown ? dk[0][t][r] * g.scale : 0.f; }, box, lane, a.D, g.grain,
+        store_rows<T, PIECE, S::DT, MODE == WHOLE_ROWS>([&](int t, int r) { return spoilt[0] ? NAN : shown ? dk[0][t][r] * g.scale : 0.f; }, box, lane, a.D, g.grain,
                                          row_out<T>(a.d_k, j0, 2 * hk), a.d_k.row_stride, keep);
-        store_rows<T, PIECE, S::DT, DMA>([&](int t, int r) { return spoilt[1] ? NAN : shown ? dk[1][t][r] * g.scale : 0.f; }, box, lane, a.D, g.grain,
+        store_rows<T, PIECE, S::DT, MODE == WHOLE_ROWS>([&](int t, int r) { return spoilt[1] ? NAN : shown ? dk[1][t][r] * g.scale : 0.f; }, box, lane, a.D, g.grain,
                                          row_out<T>(a.d_k, j0, 2 * hk + 1), a.d_k.row_stride, keep);
     }
     if (P::SPLIT == 1 || share)
-        store_rows<T, PIECE, S::VT, DMA>([&](int t, int r) { return shown ? dv[t][r] : 0.f; }, box, lane, a.Dv, g.grain, row_out<T>(a.d_v, j0, hk), a.d_v.row_stride, keep);
+        store_rows<T, PIECE, S::VT, MODE == WHOLE_ROWS>([&](int t, int r) { return shown ? dv[t][r] : 0.f; }, box, lane, a.Dv, g.grain, row_out<T>(a.d_v, j0, hk), a.d_v.row_stride, keep);
 }
 
-template <typename T, int DP, bool DMA>
+template <typename T, int DP, int MODE>
 __global__ __launch_bounds__((Keys<T, DP>::WAVES * 64), (Keys<T, DP>::OCC)) void bwd_keys_kernel(AttnArgs g, int32_t tiles, int32_t row_tiles) {
     typedef Keys<T, DP> P;
     __shared__ __align__(16) char s_a[P::BUF];
@@ -715,7 +719,7 @@ __global__ __launch_bounds__((Keys<T, DP>::WAVES * 64), (Keys<T, DP>::OCC)) void
     __shared__ int s_lo[P::WAVES], s_hi[P::WAVES], s_bad;
     const int64_t blocks = ceil_div<int64_t>((int64_t)tiles * g.a.Hk, 8) * 8;
     if ((int64_t)blockIdx.x >= blocks) sum_lam<P::WAVES * 64>(g, (int)(blockIdx.x - blocks), row_tiles, s_a);
-    else keys_body<T, DP, DMA>(g, tiles, s_a, s_b, s_own, s_val, s_marks, s_lo, s_hi, s_bad);
+    else keys_body<T, DP, MODE>(g, tiles, s_a, s_b, s_own, s_val, s_marks, s_lo, s_hi, s_bad);
 }
 
 // -------------------------------------------------------------------- owned: keys, rows of 1024 bytes (fp32, heads over 64)
@@ -731,7 +735,7 @@ struct Roles {
 };
 
 // DK: this wave sums dK of map `part`; else half `part` of dV's columns
-template <typename T, int DP, bool DMA, bool DK>
+template <typename T, int DP, int MODE, bool DK>
 __device__ __forceinline__ void roles_body(const AttnArgs& g, int32_t tiles, char* s_a, char* s_own, uint8_t* s_marks, int& s_bad, int part) {
     typedef Shape<T, DP> S;
     typedef Roles<T, DP> P;
@@ -754,9 +758,11 @@ __device__ __forceinline__ void roles_body(const AttnArgs& g, int32_t tiles, cha
     Reach reach = reach_of(rows);
     if (!__all(shown)) reach.to = 0;
     if (threadIdx.x == 0) s_bad = 0;
+    clear_image<MODE, TILE, NT>(s_a);
+    if (MODE == PADDED) __syncthreads();
     const int32_t lo = reach.lo, hi = reach.hi;                 // (the waves have the same keys)
-    Stager<T, DP, ROWS, NT, false, true>().load(s_own, halves<T>(a.k, hk, a.D), j0, (int32_t)a.Tk - 1, g.grain);
-    Stager<T, DP, ROWS, NT, false, false>().load(s_own + ROWS * RB, run<T>(a.v, hk, a.Dv), j0, (int32_t)a.Tk - 1, g.grain);
+    Stager<T, DP, ROWS, NT, BY_REGISTERS, true>().load(s_own, halves<T>(a.k, hk, a.D), j0, (int32_t)a.Tk - 1, g.grain);
+    Stager<T, DP, ROWS, NT, BY_REGISTERS, false>().load(s_own + ROWS * RB, run<T>(a.v, hk, a.Dv), j0, (int32_t)a.Tk - 1, g.grain);
     constexpr int N = DK ? S::DT : S::VT / 2;                   // 32-wide tiles of the sum
     f32x16 acc[N];
     auto clear = [&]() {
@@ -775,8 +781,8 @@ __device__ __forceinline__ void roles_body(const AttnArgs& g, int32_t tiles, cha
             __builtin_amdgcn_global_load_lds((SGL_GLOBAL void*)src, (SGL_LDS void*)(buf + TILE + at0), 4, 0, 0);
         }
     };
-    Stager<T, DP, BQ, NT, DMA, true> stage_q;
-    Stager<T, DP, BQ, NT, DMA, false> stage_go;
+    Stager<T, DP, BQ, NT, MODE, true> stage_q;
+    Stager<T, DP, BQ, NT, MODE, false> stage_go;
     stage_q.plan(halves<T>(a.q, 0, a.D));
     stage_go.plan(run<T>(a.d_out, 0, a.Dv));
     bool finite = false;        // the pass without what is not finite
@@ -889,14 +895,14 @@ __device__ __forceinline__ void roles_body(const AttnArgs& g, int32_t tiles, cha
     char* box = s_a + wave * (TILE / P::WAVES);
     constexpr int PIECE = TILE / P::WAVES / 32;               // bytes of a row at a time
     if constexpr (DK)
-        store_rows<T, PIECE, N, DMA>([&](int d, int r) { return spoilt ? NAN : shown ? acc[d][r] * g.scale : 0.f; }, box, lane, a.D, g.grain,
+        store_rows<T, PIECE, N, MODE == WHOLE_ROWS>([&](int d, int r) { return spoilt ? NAN : shown ? acc[d][r] * g.scale : 0.f; }, box, lane, a.D, g.grain,
                                      row_out<T>(a.d_k, j0, 2 * hk + part), a.d_k.row_stride, keep);
     else
-        store_rows<T, PIECE, N, DMA>([&](int d, int r) { return shown ? acc[d][r] : 0.f; }, box, lane, a.Dv - part * N * 32, g.grain,
+        store_rows<T, PIECE, N, MODE == WHOLE_ROWS>([&](int d, int r) { return shown ? acc[d][r] : 0.f; }, box, lane, a.Dv - part * N * 32, g.grain,
                                      row_out<T>(a.d_v, j0, hk) + part * N * 32, a.d_v.row_stride, keep);
 }
 
-template <typename T, int DP, bool DMA>
+template <typename T, int DP, int MODE>
 __global__ __launch_bounds__((Roles<T, DP>::WAVES * 64), 1) void bwd_roles_kernel(AttnArgs g, int32_t tiles, int32_t row_tiles) {
     typedef Roles<T, DP> P;
     __shared__ __align__(16) char s_a[P::BUF];
@@ -906,8 +912,8 @@ __global__ __launch_bounds__((Roles<T, DP>::WAVES * 64), 1) void bwd_roles_kerne
     const int64_t blocks = ceil_div<int64_t>((int64_t)tiles * g.a.Hk, 8) * 8;
     if ((int64_t)blockIdx.x >= blocks) return sum_lam<P::WAVES * 64>(g, (int)(blockIdx.x - blocks), row_tiles, s_a);
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    if (wave < 2) roles_body<T, DP, DMA, true>(g, tiles, s_a, s_own, s_marks, s_bad, wave);
-    else roles_body<T, DP, DMA, false>(g, tiles, s_a, s_own, s_marks, s_bad, wave - 2);
+    if (wave < 2) roles_body<T, DP, MODE, true>(g, tiles, s_a, s_own, s_marks, s_bad, wave);
+    else roles_body<T, DP, MODE, false>(g, tiles, s_a, s_own, s_marks, s_bad, wave - 2);
 }
 
 template <typename T, int DP>
@@ -915,25 +921,26 @@ void launch(const AttnArgs& g, hipStream_t st) {
     const sgl_diff_attn_args& a = g.a;
     typedef Shape<T, DP> S;
     const int32_t qt = (int32_t)ceil_div<int64_t>(a.Tq, QUERY_ROWS);
-    const bool dma = g.grain == 16 && a.D == DP && a.Dv == 2 * DP && dma_rows(a.k) && dma_rows(a.v) && dma_rows(a.q) && dma_rows(a.d_out);
-    if (qt > 0) {
-        const dim3 grid((unsigned)(ceil_div<int64_t>((int64_t)qt * a.Hq, 8) * 8)), block(Rows<T, DP>::WAVES * 64);
-        if (dma) hipLaunchKernelGGL((bwd_rows_kernel<T, DP, true>), grid, block, 0, st, g, qt);
-        else hipLaunchKernelGGL((bwd_rows_kernel<T, DP, false>), grid, block, 0, st, g, qt);
-    }
-    if constexpr (S::RB <= 512) {
-        typedef Keys<T, DP> P;
-        const int32_t kt = (int32_t)ceil_div<int64_t>(a.Tk, P::ROWS);
-        const dim3 grid((unsigned)(ceil_div<int64_t>((int64_t)kt * a.Hk, 8) * 8 + a.Hq)), block(P::WAVES * 64);
-        if (dma) hipLaunchKernelGGL((bwd_keys_kernel<T, DP, true>), grid, block, 0, st, g, kt, qt);
-        else hipLaunchKernelGGL((bwd_keys_kernel<T, DP, false>), grid, block, 0, st, g, kt, qt);
-    } else {
-        typedef Roles<T, DP> P;
-        const int32_t kt = (int32_t)ceil_div<int64_t>(a.Tk, P::ROWS);
-        const dim3 grid((unsigned)(ceil_div<int64_t>((int64_t)kt * a.Hk, 8) * 8 + a.Hq)), block(P::WAVES * 64);
-        if (dma) hipLaunchKernelGGL((bwd_roles_kernel<T, DP, true>), grid, block, 0, st, g, kt, qt);
-        else hipLaunchKernelGGL((bwd_roles_kernel<T, DP, false>), grid, block, 0, st, g, kt, qt);
-    }
+    auto go = [&](auto mode) {
+        constexpr int MODE = decltype(mode)::value;
+        if (qt > 0)
+            hipLaunchKernelGGL((bwd_rows_kernel<T, DP, MODE>), dim3((unsigned)(ceil_div<int64_t>((int64_t)qt * a.Hq, 8) * 8)), dim3(Rows<T, DP>::WAVES * 64), 0, st, g, qt);
+        if constexpr (S::RB <= 512) {
+            typedef Keys<T, DP> P;
+            const int32_t kt = (int32_t)ceil_div<int64_t>(a.Tk, P::ROWS);
+            const dim3 grid((unsigned)(ceil_div<int64_t>((int64_t)kt * a.Hk, 8) * 8 + a.Hq)), block(P::WAVES * 64);
+            hipLaunchKernelGGL((bwd_keys_kernel<T, DP, MODE>), grid, block, 0, st, g, kt, qt);
+        } else {
+            typedef Roles<T, DP> P;
+            const int32_t kt = (int32_t)ceil_div<int64_t>(a.Tk, P::ROWS);
+            const dim3 grid((unsigned)(ceil_div<int64_t>((int64_t)kt * a.Hk, 8) * 8 + a.Hq)), block(P::WAVES * 64);
+            hipLaunchKernelGGL((bwd_roles_kernel<T, DP, MODE>), grid, block, 0, st, g, kt, qt);
+        }
+    };
+    const int mode = stage_mode(g, DP, {&a.k, &a.v, &a.q, &a.d_out});
+    if (mode == WHOLE_ROWS) go(Int<WHOLE_ROWS>{});
+    else if (mode == PADDED) go(Int<PADDED>{});
+    else go(Int<BY_REGISTERS>{});
 }
 
 }  // namespace

@@ -146,11 +146,12 @@ __device__ __forceinline__ void step(State<T, DP, MAPS>& st, const typename Mat<
 }
 
 // HEADS: the columns are the query heads of one key head, all at query `seq`; otherwise 32 query rows of one head
-template <typename T, int DP, bool HEADS, bool DMA>
+template <typename T, int DP, bool HEADS, int MODE>
 __global__ __launch_bounds__((Shape<T, DP, HEADS>::NT), (HEADS && Shape<T, DP, HEADS>::RB > 512 ? 1 : 2)) void fwd_kernel(AttnArgs g, FwdWork w) {
     typedef Shape<T, DP, HEADS> S;
     typedef Mat<T> M;
     constexpr int RB = S::RB, BN = S::BN, MAPS = S::MAPS, VT = S::VT;
+    constexpr bool WHOLE = MODE == WHOLE_ROWS;
     __shared__ __align__(16) char s_a[S::TILE];
     __shared__ __align__(16) char s_b[S::TILE];
     __shared__ __align__(8) uint8_t s_marks[BN * (RB / 16)];
@@ -201,12 +202,14 @@ __global__ __launch_bounds__((Shape<T, DP, HEADS>::NT), (HEADS && Shape<T, DP, H
     for (int c = 0; c < MAPS; ++c)
 #pragma unroll
         for (int k = 0; k < S::QS; ++k)
-            q[c][k] = global_frag<T, DMA>(row<T>(a.q, mine ? i : 0, 2 * h + map0 + c), (2 * k + half) * S::EP, a.D, g.grain);
+            q[c][k] = global_frag<T, WHOLE>(row<T>(a.q, mine ? i : 0, 2 * h + map0 + c), (2 * k + half) * S::EP, a.D, g.grain);
     mine = mine && (seq >= 0 || (a.flags & SGL_ATTN_ZERO_REST));
     Reach reach = reach_of(span);
     if (a.key_mask) reach.to = 0;
     if (lane == 0 && (MAPS == 2 || map0 == 0)) s_lo[group] = reach.lo, s_hi[group] = reach.hi;
     if (threadIdx.x == 0) s_bad = 0;
+    clear_image<MODE, S::TILE, S::NT>(s_a);
+    clear_image<MODE, S::TILE, S::NT>(s_b);
     __syncthreads();
     int32_t lo = s_lo[0], hi = s_hi[0];
 #pragma unroll
@@ -223,8 +226,8 @@ __global__ __launch_bounds__((Shape<T, DP, HEADS>::NT), (HEADS && Shape<T, DP, H
     const int32_t last = (int32_t)a.Tk - 1;
     State<T, DP, MAPS> st;
     st.reset();
-    Stager<T, DP, BN, S::NT, DMA, true> stage_k;
-    Stager<T, DP, BN, S::NT, DMA, false> stage_v;
+    Stager<T, DP, BN, S::NT, MODE, true> stage_k;
+    Stager<T, DP, BN, S::NT, MODE, false> stage_v;
     stage_k.plan(ks);
     stage_v.plan(vs);
     bool finite = false;        // the pass without what is not finite
@@ -308,7 +311,7 @@ __global__ __launch_bounds__((Shape<T, DP, HEADS>::NT), (HEADS && Shape<T, DP, H
                 for (int r4 = 0; r4 < 4; ++r4) {
                     const int d = t * 32 + 8 * r4 + 4 * half;
                     const f32x4 x = {st.o[c][t][4 * r4], st.o[c][t][4 * r4 + 1], st.o[c][t][4 * r4 + 2], st.o[c][t][4 * r4 + 3]};
-                    if (DMA || a.Dv % 4 == 0) {
+                    if (WHOLE || a.Dv % 4 == 0) {
                         if (d < a.Dv) *reinterpret_cast<f32x4*>(o + d) = x;
                     } else {
 #pragma unroll
@@ -334,9 +337,9 @@ __global__ __launch_bounds__((Shape<T, DP, HEADS>::NT), (HEADS && Shape<T, DP, H
         const uint32_t keep = (uint32_t)__ballot(mine);
         if constexpr (MAPS == 2) {
             const auto second = [&](int t, int r) { return inv[1] == 0.f ? 0.f : st.o[1][t][r] * inv[1]; };
-            store_rows<T, SHARE / 32, VT, DMA>([&](int t, int r) { return __builtin_fmaf(-lam, second(t, r), inv[0] == 0.f ? 0.f : st.o[0][t][r] * inv[0]); }, own, lane, a.Dv,
+            store_rows<T, SHARE / 32, VT, WHOLE>([&](int t, int r) { return __builtin_fmaf(-lam, second(t, r), inv[0] == 0.f ? 0.f : st.o[0][t][r] * inv[0]); }, own, lane, a.Dv,
                                                g.grain, row_out<T>(a.out, i0, h), a.out.row_stride, keep);
-            if (a.o2.data) store_rows<T, SHARE / 32, VT, DMA>(second, own, lane, a.Dv, g.grain, row_out<T>(a.o2, i0, h), a.o2.row_stride, keep);
+            if (a.o2.data) store_rows<T, SHARE / 32, VT, WHOLE>(second, own, lane, a.Dv, g.grain, row_out<T>(a.o2, i0, h), a.o2.row_stride, keep);
         } else {
 #pragma unroll
             for (int t = 0; t < VT; ++t)
@@ -374,7 +377,7 @@ __global__ __launch_bounds__((Shape<T, DP, HEADS>::NT), (HEADS && Shape<T, DP, H
             __syncthreads();
             const sgl_rows& to = map0 ? a.o2 : a.out;
             if (to.data)
-                store_rows<T, SHARE / 32, VT, DMA>([&](int t, int r) { return st.o[0][t][r]; }, own, lane, a.Dv, g.grain, row_out<T>(to, i0, h), to.row_stride, keep);
+                store_rows<T, SHARE / 32, VT, WHOLE>([&](int t, int r) { return st.o[0][t][r]; }, own, lane, a.Dv, g.grain, row_out<T>(to, i0, h), to.row_stride, keep);
         }
     }
 }
@@ -467,14 +470,15 @@ void launch(const AttnArgs& g, hipStream_t st) {
     const FwdWork w = forward_work(g.a);
     const dim3 grid((unsigned)(ceil_div<int64_t>(w.items, 8) * 8));
     constexpr int ROW_NT = Shape<T, DP, false>::NT, HEAD_NT = Shape<T, DP, true>::NT;
-    const bool dma = g.grain == 16 && g.a.D == DP && g.a.Dv == 2 * DP && dma_rows(g.a.k) && dma_rows(g.a.v);
-    if (g.a.q_ptr) {
-        if (dma) hipLaunchKernelGGL((fwd_kernel<T, DP, false, true>), grid, dim3(ROW_NT), 0, st, g, w);
-        else hipLaunchKernelGGL((fwd_kernel<T, DP, false, false>), grid, dim3(ROW_NT), 0, st, g, w);
-    } else {
-        if (dma) hipLaunchKernelGGL((fwd_kernel<T, DP, true, true>), grid, dim3(HEAD_NT), 0, st, g, w);
-        else hipLaunchKernelGGL((fwd_kernel<T, DP, true, false>), grid, dim3(HEAD_NT), 0, st, g, w);
-    }
+    auto go = [&](auto mode) {
+        constexpr int MODE = decltype(mode)::value;
+        if (g.a.q_ptr) hipLaunchKernelGGL((fwd_kernel<T, DP, false, MODE>), grid, dim3(ROW_NT), 0, st, g, w);
+        else hipLaunchKernelGGL((fwd_kernel<T, DP, true, MODE>), grid, dim3(HEAD_NT), 0, st, g, w);
+    };
+    const int mode = stage_mode(g, DP, {&g.a.k, &g.a.v});
+    if (mode == WHOLE_ROWS) go(Int<WHOLE_ROWS>{});
+    else if (mode == PADDED) go(Int<PADDED>{});
+    else go(Int<BY_REGISTERS>{});
     if (g.parts > 1)
         hipLaunchKernelGGL(join_kernel<T>, dim3((unsigned)(g.a.Tq * g.a.Hq)), dim3(BLOCK), 0, st, g);
 }
