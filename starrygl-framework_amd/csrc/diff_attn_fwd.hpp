@@ -295,11 +295,12 @@ __global__ __launch_bounds__((Shape<T, DP, HEADS>::NT), (HEADS && Shape<T, DP, H
     }
 
     if (HEADS || g.parts > 1) {
-        // unnormalised results, to be joined with the other parts'
+        // unnormalised results, to be joined with the other parts'; a column without keys here has gathered what the others of its
+        // wave see, where they see all of a tile
         const int part = HEADS ? split * 2 + group : split;
 #pragma unroll
         for (int c = 0; c < MAPS; ++c) {
-            const float l = half_sum(st.l[c]);
+            const float gathered = half_sum(st.l[c]), l = span.lo < span.hi ? gathered : 0.f;
             if (!mine) continue;
             const int64_t at = (((int64_t)part * a.Tq + i) * a.Hq + h) * 2 + map0 + c;
             if (half == 0) g.part_ml[2 * at] = st.m[c], g.part_ml[2 * at + 1] = l;

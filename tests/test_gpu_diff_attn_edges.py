@@ -1,0 +1,44 @@
+"""Calls of differential attention at the edges of what it takes: rows without keys in split tiles, sizes past 32 bits, values
+that are not finite in every kernel, pointers behind the rows; bounds as derived in attn_plain."""
+import math
+
+import pytest
+import torch
+
+from test_gpu_diff_attn import BF16, F16, F32, _check, _inputs, _ptr, _within
+
+pytestmark = pytest.mark.gpu
+
+# D, Dv, dtype: both maps in a wave, and one (rows of 512 and of 1024 bytes)
+WIDTHS = [(32, 64, BF16), (32, 64, F32), (64, 128, BF16), (64, 128, F32), (128, 256, F16), (128, 256, F32), (100, 200, BF16), (7, 9, F16)]
+
+
+@pytest.mark.parametrize("D,Dv,dtype", WIDTHS)
+@pytest.mark.parametrize("causal", [False, True])
+def test_rows_without_keys_beside_a_split_sequence(hot, causal, D, Dv, dtype):
+    """a sequence with queries and no keys, queries that come before the first key (causal), and rows before and behind all
+    sequences share a row tile with a sequence long enough to be split over blocks: they give zeros, lse = inf"""
+    # (a wave that has a column of few keys looks at every mask: only causal calls have one here, beside the six rows that it hides)
+    more = 1 if causal else 0
+    q_ptr, k_ptr = _ptr([10, 12, 4] + [6] * more, 5), _ptr([0, 2048, 0] + [3] * more, 3)
+    Tq, Tk = 42, 2060
+    q, k, v, lam, go = _inputs(Tq, Tk, 2, 1, D, Dv, dtype, D)
+    _, ref = _check(q, k, v, lam, go, k_ptr, q_ptr, causal=causal)
+    dead = torch.ones(Tq, dtype=torch.bool)
+    dead[15:27] = False
+    if causal:
+        dead[34:37] = False                     # six queries over three keys
+    out, o2 = (torch.full((Tq, 2, Dv), 7.0, dtype=dtype, device="cuda") for _ in range(2))
+    lse = torch.full((Tq, 2, 2), 7.0, device="cuda")
+    flat = q.flatten(1, 2), k.flatten(1, 2), v
+    hot.diff_attn(*flat, lam, k_ptr, q_ptr, causal=causal, zero_rest=True, out=out, lse=lse, o2=o2)
+    _within(out, ref, "out")
+    dead = dead.cuda()
+    assert not o2[dead].any() and (lse[dead] == math.inf).all() and lse[~dead].isfinite().all()
+    # left as they were without zero_rest: rows of no sequence only
+    for t in (out, o2, lse):
+        t.fill_(7.0)
+    hot.diff_attn(*flat, lam, k_ptr, q_ptr, causal=causal, out=out, lse=lse, o2=o2)
+    for t in (out, o2):
+        assert (t[:5] == 7).all() and (t[37:] == 7).all() and not t[5:15].any() and not t[27:31].any()
+    assert (lse[:5] == 7).all() and (lse[37:] == 7).all()
