@@ -131,6 +131,9 @@ __device__ __forceinline__ T* row_out(const sgl_rows& r, int64_t n, int64_t h) {
     return static_cast<T*>(r.data) + n * r.row_stride + h * r.head_stride;
 }
 
+// where the two numbers of (row, head) lie in lse and delta: rows times heads may need all of 31 bits
+__device__ __forceinline__ int64_t pair_at(const sgl_diff_attn_args& a, int64_t i, int h) { return (i * a.Hq + h) * 2; }
+
 __device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }     // below 2^-126: 0
 
 // the other half's value of a reduction over lanes l and l ^ 32

@@ -159,9 +159,9 @@ __global__ __launch_bounds__((Rows<T, DP>::WAVES * 64), (Rows<T, DP>::OCC)) void
 #pragma unroll
     for (int m = 0; m < 2; ++m) {
         t[m] = half_sum(t[m]);
-        lse[m] = live ? a.lse[(i * a.Hq + h) * 2 + m] : INFINITY;
+        lse[m] = live ? a.lse[pair_at(a, i, h) + m] : INFINITY;
     }
-    if (i < a.Tq && half == 0) g.delta[(i * a.Hq + h) * 2] = t[0], g.delta[(i * a.Hq + h) * 2 + 1] = t[1];
+    if (i < a.Tq && half == 0) g.delta[pair_at(a, i, h)] = t[0], g.delta[pair_at(a, i, h) + 1] = t[1];
 
     const Source ks = halves<T>(a.k, hk, a.D), vs = run<T>(a.v, hk, a.Dv);
     const int32_t last = (int32_t)a.Tk - 1;
@@ -467,7 +467,7 @@ __device__ __forceinline__ void keys_body(const AttnArgs& g, int32_t tiles, char
 #pragma unroll
             for (int u = 0; u < P::SUBS; ++u) {
                 const int32_t i = min(i0 + 32 * u + (lane & 31), last);
-                const float* src = wave == 2 ? a.lam + h : (wave ? g.delta : a.lse) + ((int64_t)i * a.Hq + h) * 2 + (lane >> 5);
+                const float* src = wave == 2 ? a.lam + h : (wave ? g.delta : a.lse) + pair_at(a, i, h) + (lane >> 5);
                 const int at0 = __builtin_amdgcn_readfirstlane(u * P::STAT + wave * 256);
                 __builtin_amdgcn_global_load_lds((SGL_GLOBAL void*)src, (SGL_LDS void*)(buf + TILE + at0), 4, 0, 0);
             }
@@ -776,7 +776,7 @@ __device__ __forceinline__ void roles_body(const AttnArgs& g, int32_t tiles, cha
     auto load_stats = [&](char* buf, int h, int32_t i0) {
         if (wave < 2) {
             const int32_t i = min(i0 + (lane & 31), last);
-            const float* src = (wave ? g.delta : a.lse) + ((int64_t)i * a.Hq + h) * 2 + (lane >> 5);
+            const float* src = (wave ? g.delta : a.lse) + pair_at(a, i, h) + (lane >> 5);
             const int at0 = __builtin_amdgcn_readfirstlane(wave * 256);
             __builtin_amdgcn_global_load_lds((SGL_GLOBAL void*)src, (SGL_LDS void*)(buf + TILE + at0), 4, 0, 0);
         }

@@ -330,7 +330,7 @@ __global__ __launch_bounds__((Shape<T, DP, HEADS>::NT), (HEADS && Shape<T, DP, H
             const float l = half_sum(st.l[c]);
             const bool none = !(span.lo < span.hi) || l == 0.f;
             inv[c] = none ? 0.f : 1.f / l;
-            if (a.lse && half == 0 && mine) a.lse[(i * a.Hq + h) * 2 + map0 + c] = none ? INFINITY : st.m[c] + __builtin_amdgcn_logf(l);
+            if (a.lse && half == 0 && mine) a.lse[pair_at(a, i, h) + map0 + c] = none ? INFINITY : st.m[c] + __builtin_amdgcn_logf(l);
         }
         const float lam = a.lam[h];
         constexpr int SHARE = S::TILE / (S::WAVES / 2);                     // a wave's part of the two buffers

@@ -184,8 +184,8 @@ __global__ __launch_bounds__(BLOCK) void seg_bwd_kernel(AttnArgs g) {
             }
             t[0] = lanes_sum<L>(t[0]);
             t[1] = lanes_sum<L>(t[1]);
-            lse[0] = a.lse[(i * a.Hq + h) * 2];
-            lse[1] = a.lse[(i * a.Hq + h) * 2 + 1];
+            lse[0] = a.lse[pair_at(a, i, h)];
+            lse[1] = a.lse[pair_at(a, i, h) + 1];
         };
 #pragma unroll
         for (int e = 0; e < EP; ++e) dq[e] = 0.f;

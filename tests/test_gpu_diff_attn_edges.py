@@ -5,6 +5,8 @@ import math
 import pytest
 import torch
 
+import attn_plain as plain
+from starrygl_amd.nn.model import diff_attention
 from test_gpu_diff_attn import BF16, F16, F32, _check, _inputs, _ptr, _within
 
 pytestmark = pytest.mark.gpu
@@ -42,3 +44,28 @@ def test_rows_without_keys_beside_a_split_sequence(hot, causal, D, Dv, dtype):
     for t in (out, o2):
         assert (t[:5] == 7).all() and (t[37:] == 7).all() and not t[5:15].any() and not t[27:31].any()
     assert (lse[:5] == 7).all() and (lse[37:] == 7).all()
+
+
+@pytest.mark.parametrize("Tq", [1 << 26])
+def test_rows_times_heads_past_30_bits(hot, Tq):
+    """2^26 rows of 16 heads: the numbers kept for (row, head, map) are 2^31 and more; only the last rows belong to sequences"""
+    if torch.cuda.mem_get_info()[0] < 100 << 30:
+        pytest.skip("needs 100 GB")
+    nq, nk = [200, 100], [70, 130]
+    q, k, v, lam, go = _inputs(300, 200, 16, 4, 1, 1, BF16, 13)
+    big = [torch.zeros(Tq, *t.shape[1:], dtype=BF16, device="cuda") for t in (q, go)]
+    for b, t in zip(big, (q, go)):
+        b[-300:] = t
+        b[:64] = 1.0                            # (rows of no sequence)
+    k_ptr, q_ptr = _ptr(nk), _ptr(nq, Tq - 300)
+    ref = plain.diff_attention(q, k, v, lam, k_ptr, _ptr(nq), grad=go)
+    out, lse = torch.empty(Tq, 16, 1, dtype=BF16, device="cuda"), torch.empty(Tq, 16, 2, device="cuda")
+    o2 = torch.empty_like(out)
+    flat = big[0].view(Tq, 32, 1), k.view(200, 8, 1), v
+    hot.diff_attn(*flat, lam, k_ptr, q_ptr, zero_rest=True, out=out, lse=lse, o2=o2)
+    _within(out[-300:], ref, "out")
+    assert not out[:-300].any() and not o2[:-300].any() and lse[-300:].isfinite().all() and (lse[:-300] == math.inf).all()
+    got = hot.diff_attn_backward(big[1], *flat, lam, out, lse, o2, k_ptr, q_ptr, zero_rest=True)
+    assert not got[0][:-300].any()
+    for name, t in zip(("dq", "dk", "dv", "dlam"), (got[0][-300:].view(q.shape), got[1].view(k.shape), *got[2:])):
+        _within(t, ref, name)
