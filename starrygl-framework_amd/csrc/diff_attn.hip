@@ -39,7 +39,7 @@ FwdWork forward_work(const sgl_diff_attn_args& a) {
 
 namespace {
 
-constexpr int64_t GRID_MAX = 0x7FFFFFFF, COUNT_MAX = 0x7FFFFF00;
+constexpr int64_t PAIRS_MAX = 0x7FFFFFFF, COUNT_MAX = 0x7FFFFF00;
 
 int32_t check_args(const char* what, const sgl_diff_attn_args* a, bool backward) {
     if (!a) return fail(SGL_EINVAL, "%s: args is NULL", what);
@@ -60,8 +60,8 @@ int32_t check_args(const char* what, const sgl_diff_attn_args* a, bool backward)
         if (!a->d_lam || (a->Tq > 0 && (!a->lse || !a->d_out.data || !a->d_q.data)) || (a->Tk > 0 && (!a->d_k.data || !a->d_v.data)))
             return fail(SGL_EINVAL, "%s: lse, o2 or a gradient is NULL", what);
     }
-    if (a->Tq * a->Hq > GRID_MAX || a->Tk * a->Hk > GRID_MAX)
-        return fail(SGL_ENOTSUP, "%s: too many rows times heads", what);
+    // (blocks are counted in 32 bits)
+    if (a->Tq * a->Hq > PAIRS_MAX || a->Tk * a->Hk > PAIRS_MAX) return fail(SGL_ENOTSUP, "%s: Tq * Hq and Tk * Hk must stay below 2^31", what);
     return SGL_OK;
 }
 

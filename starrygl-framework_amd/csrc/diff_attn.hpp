@@ -15,6 +15,7 @@ constexpr int BLOCK = 256;
 constexpr float NEG_INF = -INFINITY;
 constexpr float LOG2E = 1.44269504088896340736f;
 
+constexpr int64_t GRID_PART = 1 << 22;      // blocks of a launch, a multiple of 8 (a launch takes less than 2^32 threads)
 constexpr int QUERY_ROWS = 128;     // query rows of a block of the backward pass (a sum of t_2 in the workspace each)
 
 // How rows come into LDS: through registers, whole (as wide as the image), or padded (narrower, in whole 16-byte chunks)
@@ -27,6 +28,7 @@ struct AttnArgs {
     int32_t negate;             // scale < 0: the operand that stays in registers changes its sign (exact)
     int32_t grain;              // bytes, 16 at most, that divide the address of every row and the length of every row's head
     int32_t parts;              // forward: partial results per (row, head, map), joined by a second kernel; 1: none
+    int64_t first;              // first block of a launch: large grids go out in parts
     float* part_ml;             // [parts, Tq * Hq, 2, 2]: running maximum (in powers of two) and sum
     float* part_o;              // [parts, Tq * Hq, 2, Dv]
     float* delta;               // backward [Tq, Hq, 2]: t_1, t_2
@@ -612,7 +614,10 @@ __device__ __forceinline__ void store_rows(Val val, char* box, int lane, int len
 
 // Work item of a block: consecutive items of one XCD (blocks go to the 8 of them in turn) are neighbours, so that what they
 // share lies in one L2.  The grid is a multiple of 8; items >= n do nothing.
-__device__ __forceinline__ uint32_t xcd_item(uint32_t n) { return (blockIdx.x % 8) * ((n + 7) / 8) + blockIdx.x / 8; }
+__device__ __forceinline__ uint32_t xcd_item(const AttnArgs& g, uint32_t n) {
+    const uint32_t first = (uint32_t)g.first, here = min(n - first, (uint32_t)GRID_PART);
+    return first + (blockIdx.x % 8) * ((here + 7) / 8) + blockIdx.x / 8;
+}
 
 // The spans of 32 columns (lanes l and l + 32 hold the same one): their union, and what all of them see.  Spans of ascending rows
 // ascend, so the first and the last that are not empty say it.
@@ -645,7 +650,13 @@ __device__ __forceinline__ bool sees(int32_t j, Span span, const uint8_t* __rest
 
 #endif  // __HIPCC__
 
-// Host side.  Forward on the matrix units: tiles of query rows, or (without q_ptr) of the heads of a group.
+// Host side.  A launch of any number of blocks, in parts (one, but for calls of millions of row tiles or rows).
+template <typename Launch>
+void in_parts(AttnArgs g, int64_t blocks, Launch launch) {
+    for (g.first = 0; g.first < blocks; g.first += GRID_PART) launch(g, dim3((unsigned)(blocks - g.first < GRID_PART ? blocks - g.first : GRID_PART)));
+}
+
+// Forward on the matrix units: tiles of query rows, or (without q_ptr) of the heads of a group.
 struct FwdWork {
     int64_t items;              // blocks with work
     int32_t tiles;              // row tiles, or sequences

@@ -107,7 +107,7 @@ __global__ __launch_bounds__((Rows<T, DP>::WAVES * 64), (Rows<T, DP>::OCC)) void
     __shared__ float s_lam[P::WAVES];
     const sgl_diff_attn_args& a = g.a;
     const int G = a.Hq / a.Hk;
-    const uint32_t n = (uint32_t)tiles * (uint32_t)a.Hq, item = xcd_item(n);
+    const uint32_t n = (uint32_t)tiles * (uint32_t)a.Hq, item = xcd_item(g, n);
     if (item >= n) return;
     const int hg = (int)(item % (uint32_t)G);
     const uint32_t rest = item / (uint32_t)G;
@@ -393,7 +393,7 @@ __device__ __forceinline__ void keys_body(const AttnArgs& g, int32_t tiles, char
     constexpr int RB = S::RB, NT = P::WAVES * 64, ROWS = P::ROWS, GROUPS = P::GROUPS, BQ = P::BQ, TILE = P::TILE, AHEAD = P::AHEAD;
     const sgl_diff_attn_args& a = g.a;
     const int G = a.Hq / a.Hk;
-    const uint32_t n = (uint32_t)tiles * (uint32_t)a.Hk, item = xcd_item(n);
+    const uint32_t n = (uint32_t)tiles * (uint32_t)a.Hk, item = xcd_item(g, n);
     if (item >= n) return;
     // key heads side by side; of a causal call the early keys, which most rows see, come first
     const int hk = (int)(item % (uint32_t)a.Hk);
@@ -717,8 +717,8 @@ __global__ __launch_bounds__((Keys<T, DP>::WAVES * 64), (Keys<T, DP>::OCC)) void
     __shared__ __align__(16) char s_val[P::VAL];
     __shared__ __align__(8) uint8_t s_marks[2 * P::BQ * (P::RB / 16)];
     __shared__ int s_lo[P::WAVES], s_hi[P::WAVES], s_bad;
-    const int64_t blocks = ceil_div<int64_t>((int64_t)tiles * g.a.Hk, 8) * 8;
-    if ((int64_t)blockIdx.x >= blocks) sum_lam<P::WAVES * 64>(g, (int)(blockIdx.x - blocks), row_tiles, s_a);
+    const int64_t blocks = ceil_div<int64_t>((int64_t)tiles * g.a.Hk, 8) * 8, block = g.first + blockIdx.x;
+    if (block >= blocks) sum_lam<P::WAVES * 64>(g, (int)(block - blocks), row_tiles, s_a);
     else keys_body<T, DP, MODE>(g, tiles, s_a, s_b, s_own, s_val, s_marks, s_lo, s_hi, s_bad);
 }
 
@@ -743,7 +743,7 @@ __device__ __forceinline__ void roles_body(const AttnArgs& g, int32_t tiles, cha
     constexpr int RB = S::RB, NT = P::WAVES * 64, ROWS = P::ROWS, BQ = P::BQ, TILE = P::TILE, AHEAD = 2;
     const sgl_diff_attn_args& a = g.a;
     const int G = a.Hq / a.Hk;
-    const uint32_t n = (uint32_t)tiles * (uint32_t)a.Hk, item = xcd_item(n);
+    const uint32_t n = (uint32_t)tiles * (uint32_t)a.Hk, item = xcd_item(g, n);
     if (item >= n) return;
     // key heads side by side; of a causal call the early keys, which most rows see, come first
     const int hk = (int)(item % (uint32_t)a.Hk);
@@ -909,8 +909,8 @@ __global__ __launch_bounds__((Roles<T, DP>::WAVES * 64), 1) void bwd_roles_kerne
     __shared__ __align__(16) char s_own[P::OWN];
     __shared__ __align__(8) uint8_t s_marks[2 * P::BQ * (P::RB / 16)];
     __shared__ int s_bad;
-    const int64_t blocks = ceil_div<int64_t>((int64_t)tiles * g.a.Hk, 8) * 8;
-    if ((int64_t)blockIdx.x >= blocks) return sum_lam<P::WAVES * 64>(g, (int)(blockIdx.x - blocks), row_tiles, s_a);
+    const int64_t blocks = ceil_div<int64_t>((int64_t)tiles * g.a.Hk, 8) * 8, block = g.first + blockIdx.x;
+    if (block >= blocks) return sum_lam<P::WAVES * 64>(g, (int)(block - blocks), row_tiles, s_a);
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     if (wave < 2) roles_body<T, DP, MODE, true>(g, tiles, s_a, s_own, s_marks, s_bad, wave);
     else roles_body<T, DP, MODE, false>(g, tiles, s_a, s_own, s_marks, s_bad, wave - 2);
@@ -924,17 +924,21 @@ void launch(const AttnArgs& g, hipStream_t st) {
     auto go = [&](auto mode) {
         constexpr int MODE = decltype(mode)::value;
         if (qt > 0)
-            hipLaunchKernelGGL((bwd_rows_kernel<T, DP, MODE>), dim3((unsigned)(ceil_div<int64_t>((int64_t)qt * a.Hq, 8) * 8)), dim3(Rows<T, DP>::WAVES * 64), 0, st, g, qt);
+            in_parts(g, ceil_div<int64_t>((int64_t)qt * a.Hq, 8) * 8, [&](const AttnArgs& part, dim3 grid) {
+                hipLaunchKernelGGL((bwd_rows_kernel<T, DP, MODE>), grid, dim3(Rows<T, DP>::WAVES * 64), 0, st, part, qt);
+            });
         if constexpr (S::RB <= 512) {
             typedef Keys<T, DP> P;
             const int32_t kt = (int32_t)ceil_div<int64_t>(a.Tk, P::ROWS);
-            const dim3 grid((unsigned)(ceil_div<int64_t>((int64_t)kt * a.Hk, 8) * 8 + a.Hq)), block(P::WAVES * 64);
-            hipLaunchKernelGGL((bwd_keys_kernel<T, DP, MODE>), grid, block, 0, st, g, kt, qt);
+            in_parts(g, ceil_div<int64_t>((int64_t)kt * a.Hk, 8) * 8 + a.Hq, [&](const AttnArgs& part, dim3 grid) {
+                hipLaunchKernelGGL((bwd_keys_kernel<T, DP, MODE>), grid, dim3(P::WAVES * 64), 0, st, part, kt, qt);
+            });
         } else {
             typedef Roles<T, DP> P;
             const int32_t kt = (int32_t)ceil_div<int64_t>(a.Tk, P::ROWS);
-            const dim3 grid((unsigned)(ceil_div<int64_t>((int64_t)kt * a.Hk, 8) * 8 + a.Hq)), block(P::WAVES * 64);
-            hipLaunchKernelGGL((bwd_roles_kernel<T, DP, MODE>), grid, block, 0, st, g, kt, qt);
+            in_parts(g, ceil_div<int64_t>((int64_t)kt * a.Hk, 8) * 8 + a.Hq, [&](const AttnArgs& part, dim3 grid) {
+                hipLaunchKernelGGL((bwd_roles_kernel<T, DP, MODE>), grid, dim3(P::WAVES * 64), 0, st, part, kt, qt);
+            });
         }
     };
     const int mode = stage_mode(g, DP, {&a.k, &a.v, &a.q, &a.d_out});

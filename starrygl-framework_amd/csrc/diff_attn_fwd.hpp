@@ -160,7 +160,7 @@ __global__ __launch_bounds__((Shape<T, DP, HEADS>::NT), (HEADS && Shape<T, DP, H
     const int G = a.Hq / a.Hk;
     // parts of a history in turn over the 8 XCDs: nothing is shared between them, and histories differ in length (as neighbours on one
     // XCD, 16 of up to 32768 keys took 140 us instead of 117)
-    const uint32_t item = HEADS ? blockIdx.x : xcd_item((uint32_t)w.items);
+    const uint32_t item = HEADS ? (uint32_t)g.first + blockIdx.x : xcd_item(g, (uint32_t)w.items);
     if (item >= w.items) return;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5, col = lane & 31;
     const int map0 = MAPS == 2 ? 0 : wave & 1, group = MAPS == 2 ? wave : wave >> 1;
@@ -391,7 +391,7 @@ __global__ __launch_bounds__(BLOCK) void join_kernel(AttnArgs g) {
     __shared__ float s_f[2][MOST], s_lse[2];
     __shared__ __align__(16) float s_o[2][8][256];
     const sgl_diff_attn_args& a = g.a;
-    const int64_t n = a.Tq * a.Hq, at = blockIdx.x;
+    const int64_t n = a.Tq * a.Hq, at = g.first + blockIdx.x;
     const int64_t i = at / a.Hq;
     const int h = (int)(at - i * a.Hq), wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
     const int32_t B = (int32_t)live_count(a.B_dev, a.B);
@@ -469,19 +469,21 @@ __global__ __launch_bounds__(BLOCK) void join_kernel(AttnArgs g) {
 template <typename T, int DP>
 void launch(const AttnArgs& g, hipStream_t st) {
     const FwdWork w = forward_work(g.a);
-    const dim3 grid((unsigned)(ceil_div<int64_t>(w.items, 8) * 8));
+    const int64_t blocks = ceil_div<int64_t>(w.items, 8) * 8;
     constexpr int ROW_NT = Shape<T, DP, false>::NT, HEAD_NT = Shape<T, DP, true>::NT;
     auto go = [&](auto mode) {
         constexpr int MODE = decltype(mode)::value;
-        if (g.a.q_ptr) hipLaunchKernelGGL((fwd_kernel<T, DP, false, MODE>), grid, dim3(ROW_NT), 0, st, g, w);
-        else hipLaunchKernelGGL((fwd_kernel<T, DP, true, MODE>), grid, dim3(HEAD_NT), 0, st, g, w);
+        in_parts(g, blocks, [&](const AttnArgs& part, dim3 grid) {
+            if (g.a.q_ptr) hipLaunchKernelGGL((fwd_kernel<T, DP, false, MODE>), grid, dim3(ROW_NT), 0, st, part, w);
+            else hipLaunchKernelGGL((fwd_kernel<T, DP, true, MODE>), grid, dim3(HEAD_NT), 0, st, part, w);
+        });
     };
     const int mode = stage_mode(g, DP, {&g.a.k, &g.a.v});
     if (mode == WHOLE_ROWS) go(Int<WHOLE_ROWS>{});
     else if (mode == PADDED) go(Int<PADDED>{});
     else go(Int<BY_REGISTERS>{});
     if (g.parts > 1)
-        hipLaunchKernelGGL(join_kernel<T>, dim3((unsigned)(g.a.Tq * g.a.Hq)), dim3(BLOCK), 0, st, g);
+        in_parts(g, g.a.Tq * g.a.Hq, [&](const AttnArgs& part, dim3 grid) { hipLaunchKernelGGL(join_kernel<T>, grid, dim3(BLOCK), 0, st, part); });
 }
 
 }  // namespace

@@ -82,7 +82,7 @@ __global__ __launch_bounds__(BLOCK) void seg_fwd_kernel(AttnArgs g) {
     constexpr int EP = Mat<T>::EP, SLOTS = 64 / L;
     const sgl_diff_attn_args& a = g.a;
     const int lane = threadIdx.x & 63;
-    const int64_t w = (int64_t)blockIdx.x * WAVES + (threadIdx.x >> 6);
+    const int64_t w = (g.first + blockIdx.x) * WAVES + (threadIdx.x >> 6);
     if (w >= a.B * a.Hq) return;
     const int64_t i = w / a.Hq;
     const int h = (int)(w - i * a.Hq), hk = h / (a.Hq / a.Hk);
@@ -282,7 +282,8 @@ __global__ __launch_bounds__(BLOCK) void lam_kernel(const float* __restrict__ pa
 
 template <typename T, int L>
 void launch_fwd(const AttnArgs& g, hipStream_t st) {
-    hipLaunchKernelGGL((seg_fwd_kernel<T, L>), dim3((unsigned)ceil_div<int64_t>(g.a.B * g.a.Hq, WAVES)), dim3(BLOCK), 0, st, g);
+    in_parts(g, ceil_div<int64_t>(g.a.B * g.a.Hq, WAVES),
+             [&](const AttnArgs& part, dim3 grid) { hipLaunchKernelGGL((seg_fwd_kernel<T, L>), grid, dim3(BLOCK), 0, st, part); });
 }
 
 template <typename T, int L>

@@ -46,9 +46,10 @@ def test_rows_without_keys_beside_a_split_sequence(hot, causal, D, Dv, dtype):
     assert (lse[:5] == 7).all() and (lse[37:] == 7).all()
 
 
-@pytest.mark.parametrize("Tq", [1 << 26])
+@pytest.mark.parametrize("Tq", [1 << 26, (1 << 27) - 16])
 def test_rows_times_heads_past_30_bits(hot, Tq):
-    """2^26 rows of 16 heads: the numbers kept for (row, head, map) are 2^31 and more; only the last rows belong to sequences"""
+    """2^26 rows of 16 heads and more: the numbers kept for (row, head, map) are 2^31 and more, the row tiles of the second call are
+    2^24 (one launch takes fewer than 2^24 blocks of 256); only the last rows belong to sequences"""
     if torch.cuda.mem_get_info()[0] < 100 << 30:
         pytest.skip("needs 100 GB")
     nq, nk = [200, 100], [70, 130]
@@ -69,3 +70,35 @@ def test_rows_times_heads_past_30_bits(hot, Tq):
     assert not got[0][:-300].any()
     for name, t in zip(("dq", "dk", "dv", "dlam"), (got[0][-300:].view(q.shape), got[1].view(k.shape), *got[2:])):
         _within(t, ref, name)
+
+
+def test_more_single_queries_over_few_keys_than_a_launch_has_waves(hot):
+    """2^26 roots with one neighbour each: P = 1, out = (1 - lam) v"""
+    if torch.cuda.mem_get_info()[0] < 30 << 30:
+        pytest.skip("needs 30 GB")
+    B = (1 << 26) + 5
+    g = torch.Generator("cuda").manual_seed(1)
+    q, k, v, go = (torch.randn(B, 1, n, generator=g, device="cuda").to(BF16) for n in (2, 2, 1, 1))
+    lam, k_ptr = torch.tensor([0.375], device="cuda"), torch.arange(B + 1, device="cuda")
+    v.requires_grad_()
+    y = diff_attention(q.view(B, 1, 2, 1), k.view(B, 1, 2, 1), v, lam, k_ptr)
+    dv, = torch.autograd.grad(y, v, go)
+    for got, x in ((y.detach(), v.detach()), (dv, go)):
+        want = x.double() * 0.625
+        assert ((got.double() - want).abs() <= (plain.h(BF16) + 16 * plain.U) * want.abs()).all()
+
+
+def test_more_single_queries_over_long_histories_than_a_launch_has_blocks(hot):
+    """2^24 sequences of 64 keys, three query heads over one: some of them, the last among them, against the plain form"""
+    if torch.cuda.mem_get_info()[0] < 60 << 30:
+        pytest.skip("needs 60 GB")
+    B, n = (1 << 24) + 3, 64
+    g = torch.Generator("cuda").manual_seed(2)
+    q = torch.randn(B, 3, 2, 1, generator=g, device="cuda").to(BF16)
+    k, v = torch.empty(B * n, 1, 2, 1, dtype=BF16, device="cuda").normal_(generator=g), torch.empty(B * n, 1, 1, dtype=BF16, device="cuda").normal_(generator=g)
+    lam = torch.tensor([0.2, 0.5, 0.7], device="cuda")
+    y = diff_attention(q, k, v, lam, torch.arange(B + 1, device="cuda") * n)
+    some = torch.cat([torch.arange(0, B, B // 40), torch.arange((1 << 22) - 3, (1 << 22) + 3), torch.arange((1 << 24) - 2, B)]).cuda()
+    keys = (some[:, None] * n + torch.arange(n, device="cuda")).flatten()
+    ref = plain.diff_attention(q[some], k[keys], v[keys], lam, torch.arange(some.numel() + 1) * n)
+    _within(y[some], ref, "out")
