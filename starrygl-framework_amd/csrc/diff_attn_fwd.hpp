@@ -295,16 +295,17 @@ __global__ __launch_bounds__((Shape<T, DP, HEADS>::NT), (HEADS && Shape<T, DP, H
     }
 
     if (HEADS || g.parts > 1) {
-        // unnormalised results, to be joined with the other parts'; a column without keys here has gathered what the others of its
-        // wave see, where they see all of a tile
+        // unnormalised results, to be joined with the other parts'; a column without keys here (sum -1, no result) has gathered what
+        // the others of its wave see, where they see all of a tile
         const int part = HEADS ? split * 2 + group : split;
 #pragma unroll
         for (int c = 0; c < MAPS; ++c) {
-            const float gathered = half_sum(st.l[c]), l = span.lo < span.hi ? gathered : 0.f;
+            const float l = half_sum(st.l[c]);
+            const bool none = !(span.lo < span.hi);
             if (!mine) continue;
             const int64_t at = (((int64_t)part * a.Tq + i) * a.Hq + h) * 2 + map0 + c;
-            if (half == 0) g.part_ml[2 * at] = st.m[c], g.part_ml[2 * at + 1] = l;
-            if (l == 0.f) continue;
+            if (half == 0) g.part_ml[2 * at] = st.m[c], g.part_ml[2 * at + 1] = none ? -1.f : l;
+            if (none) continue;
             float* o = g.part_o + at * a.Dv;
 #pragma unroll
             for (int t = 0; t < VT; ++t)
@@ -384,7 +385,8 @@ __global__ __launch_bounds__((Shape<T, DP, HEADS>::NT), (HEADS && Shape<T, DP, H
 }
 
 // Joins the parts of a (row, head), a block each: the weights of the parts first, then 8 groups of 32 lanes add up every eighth
-// part and are themselves added in order.
+// part and are themselves added in order.  A part whose weight vanishes beside the others' is added all the same, so that what
+// is not finite in it counts.
 template <typename T>
 __global__ __launch_bounds__(BLOCK) void join_kernel(AttnArgs g) {
     constexpr int MOST = 2 * 64;
@@ -405,22 +407,22 @@ __global__ __launch_bounds__(BLOCK) void join_kernel(AttnArgs g) {
             const int p = lane + 64 * u;
             const float* ml = g.part_ml + 2 * (((int64_t)p * n + at) * 2 + wave);
             m[u] = p < g.parts ? ml[0] : NEG_INF;
-            l[u] = p < g.parts ? ml[1] : 0.f;
-            if (l[u] != 0.f) top = fmaxf(top, m[u]);
+            l[u] = p < g.parts ? ml[1] : -1.f;
+            if (!(l[u] <= 0.f)) top = fmaxf(top, m[u]);
         }
 #pragma unroll
         for (int k = 1; k < 64; k <<= 1) top = fmaxf(top, __shfl_xor(top, k));
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
-            const float f = l[u] == 0.f ? 0.f : m[u] == top ? 1.f : exp2_hw(m[u] - top);
+            const float f = l[u] <= 0.f ? 0.f : m[u] == top ? 1.f : exp2_hw(m[u] - top);
             s_f[wave][lane + 64 * u] = f;
-            sum += l[u] == 0.f ? 0.f : l[u] * f;
+            sum += l[u] <= 0.f ? 0.f : l[u] * f;
         }
 #pragma unroll
         for (int k = 1; k < 64; k <<= 1) sum += __shfl_xor(sum, k);
         const float inv = sum == 0.f ? 0.f : 1.f / sum;
 #pragma unroll
-        for (int u = 0; u < 2; ++u) s_f[wave][lane + 64 * u] *= inv;
+        for (int u = 0; u < 2; ++u) s_f[wave][lane + 64 * u] = l[u] < 0.f ? -1.f : s_f[wave][lane + 64 * u] * inv;
         if (lane == 0) {
             s_lse[wave] = sum == 0.f ? INFINITY : top + __builtin_amdgcn_logf(sum);
             if (a.lse) a.lse[at * 2 + wave] = s_lse[wave];
@@ -434,7 +436,7 @@ __global__ __launch_bounds__(BLOCK) void join_kernel(AttnArgs g) {
         f32x4 acc[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
         for (int p = group; p < g.parts; p += 8) {
             const float f = s_f[m][p];
-            if (f == 0.f) continue;                     // (a part without keys wrote no result)
+            if (f < 0.f) continue;                      // (a part without keys wrote no result)
             const float* src = g.part_o + (((int64_t)p * n + at) * 2 + m) * a.Dv;
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
@@ -462,6 +464,7 @@ __global__ __launch_bounds__(BLOCK) void join_kernel(AttnArgs g) {
     for (int m = 0; m < 2; ++m)
 #pragma unroll
         for (int k = 0; k < 8; ++k) o[m] += s_o[m][k][d];
+    for (int m = 0; m < 2; ++m) o[m] = s_lse[m] == INFINITY ? 0.f : o[m];       // no key, or only scores of -inf
     row_out<T>(a.out, i, h)[d] = (T)__builtin_fmaf(-a.lam[h], o[1], o[0]);
     if (a.o2.data) row_out<T>(a.o2, i, h)[d] = (T)o[1];
 }

@@ -134,7 +134,7 @@ __global__ __launch_bounds__(BLOCK) void seg_fwd_kernel(AttnArgs g) {
         const float inv = none ? 0.f : 1.f / l[t];
 #pragma unroll
         for (int e = 0; e < EP; ++e) {
-            float x = f == 0.f ? 0.f : o[t][e] * f;
+            float x = o[t][e] * f;          // (NaN stays, whatever the slot's weight)
 #pragma unroll
             for (int k = L; k < 64; k <<= 1) x += __shfl_xor(x, k);
             o[t][e] = none ? 0.f : x * inv;

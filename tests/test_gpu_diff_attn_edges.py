@@ -102,3 +102,45 @@ def test_more_single_queries_over_long_histories_than_a_launch_has_blocks(hot):
     keys = (some[:, None] * n + torch.arange(n, device="cuda")).flatten()
     ref = plain.diff_attention(q[some], k[keys], v[keys], lam, torch.arange(some.numel() + 1) * n)
     _within(y[some], ref, "out")
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("form", ["few keys", "single queries", "split rows", "rows"])
+def test_a_seen_value_that_is_not_finite_counts_whatever_its_weight(hot, form, dtype):
+    """one key's score beats all others by hundreds of powers of two; a NaN value of another key that the query sees, wherever it
+    lies among the parts that a sequence is split into, makes its element NaN, and no other"""
+    n, nq = {"few keys": (12, 1), "single queries": (3000, 1), "split rows": (3000, 5), "rows": (400, 50)}[form]
+    q, k, v, lam, go = _inputs(nq, n, 4, 2, 32, 64, dtype, 17)
+    q[..., 0], k[..., 0] = 8.0, 0.0
+    k[n // 2, ..., 0] = 300.0
+    q_ptr = None if nq == 1 else _ptr([nq])
+    want = plain.diff_attention(q, k, v, lam, _ptr([n]), q_ptr)
+    for at in (0, 1, 2, 3, n // 2 - 1, n // 2 + 1, n - 1):
+        bad = v.clone()
+        bad[at, :, 3] = float("nan")
+        bad[at, :, 60] = float("inf")
+        y = diff_attention(q, k, bad, lam, _ptr([n]), q_ptr)
+        assert y[..., 3].isnan().all() and y[..., 60].isnan().all(), at
+        keep = [d for d in range(64) if d not in (3, 60)]
+        _within(y[..., keep], {"out": want["out"][..., keep], "out_tol": want["out_tol"][..., keep]}, "out")
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("form", ["few keys", "single queries", "split rows", "rows"])
+def test_scores_of_minus_infinity(hot, form, dtype):
+    """keys whose score overflows to -inf weigh nothing; a query with no others gets zeros, lse = inf and no gradient"""
+    n, nq = {"few keys": (12, 1), "single queries": (3000, 1), "split rows": (3000, 5), "rows": (400, 50)}[form]
+    q, k, v, lam, go = _inputs(2 * nq, 2 * n, 4, 2, 32, 64, dtype, 18)
+    q[..., 0], k[..., 0] = 2.0 ** 100, -(2.0 ** 100)
+    k[n // 2: n // 2 + 2, ..., 0] = k[:n // 3, ..., 0] = 0.0             # the first sequence has some others
+    k_ptr, q_ptr = _ptr([n, n]), None if nq == 1 else _ptr([nq, nq])
+    mask = torch.ones(2 * n, dtype=torch.bool, device="cuda")
+    mask[:n] = k[:n, 0, 0, 0] == 0
+    ref = plain.diff_attention(q[:nq], k[:n].clamp(min=-1e4), v[:n], lam, _ptr([n]), None if nq == 1 else _ptr([nq]), key_mask=mask[:n], grad=go[:nq])
+    leaves = [t.requires_grad_() for t in (q, k, v, lam)]
+    y = diff_attention(*leaves, k_ptr, q_ptr)
+    grads = torch.autograd.grad(y, leaves, go)
+    _within(y[:nq], ref, "out")
+    assert not y[nq:].any() and not grads[0][nq:].any() and not grads[1][n:].any() and not grads[2][n:].any()
+    for got, name, m in ((grads[1], "dk", n), (grads[2], "dv", n), (grads[3], "dlam", None)):
+        _within(got if m is None else got[:m], ref, name)
