@@ -65,6 +65,12 @@ bool is_vector(const Tensor& t, const Tensor& like, at::ScalarType type, int64_t
 bool wants_grad(const Tensor& t) { return t.requires_grad(); }
 bool wants_grad(const MaybeTensor& t) { return t.has_value() && t->requires_grad(); }
 
+// A dual tensor asks for no gradient: without this its tangent would be dropped without a word.
+void no_tangent(const char* what, std::initializer_list<MaybeTensor> inputs) {
+    for (const MaybeTensor& t : inputs)
+        TORCH_CHECK_NOT_IMPLEMENTED(!t.has_value() || !t->defined() || !t->_fw_grad(0).defined(), what, ": forward-mode derivatives are not implemented");
+}
+
 // The gradients below are formed outside of autograd.  Under create_graph=True they are tied to a node that refuses to be
 // differentiated, or a second derivative would silently miss them.
 variable_list once(const char* what, variable_list got) {
@@ -104,6 +110,7 @@ struct Rotary : public torch::autograd::Function<Rotary> {
         return rotary_call(x, pos, freq, interleaved, amplitude, false);
     }
     static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+        no_tangent("rotary_encode", {grads[0]});
         return once("rotary_encode", gradients(ctx, grads[0]));
     }
     static variable_list gradients(AutogradContext* ctx, const Tensor& grad) {
@@ -117,6 +124,7 @@ struct Rotary : public torch::autograd::Function<Rotary> {
 
 MaybeTensor rotary(const Tensor& x, const Tensor& pos, const Tensor& freq, bool interleaved, double amplitude) {
     if (!is_rows(x) || !params_fit(x, freq) || !is_vector(pos, x, at::kLong, x.size(0))) return std::nullopt;
+    no_tangent("rotary_encode", {x, freq});
     if (x.requires_grad() && at::GradMode::is_enabled()) return Rotary::apply(x, pos, freq, interleaved, amplitude);
     return rotary_call(x, pos, freq, interleaved, amplitude, false);
 }
@@ -164,6 +172,7 @@ struct Norm : public torch::autograd::Function<Norm> {
         return {yq, yk};
     }
     static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+        no_tangent("qk_norm_rotary", {grads[0], grads[1]});
         return once("qk_norm_rotary", gradients(ctx, grads));
     }
     static variable_list gradients(AutogradContext* ctx, const variable_list& grads) {
@@ -229,6 +238,7 @@ std::optional<std::tuple<Tensor, Tensor>> norm(const Tensor& q, const Tensor& k,
                                   ((w->dim() == 1 && w->size(0) == x.size(2)) || (w->dim() == 2 && w->size(0) == x.size(1) && w->size(1) == x.size(2))));
     };
     if (!fits(wq, q) || !fits(wk, k)) return std::nullopt;
+    no_tangent("qk_norm_rotary", {q, k, wq, wk, freq});
     const MaybeTensor pq = freq.has_value() ? pos_q : std::nullopt, pk = freq.has_value() ? pos_k : std::nullopt;
     if (at::GradMode::is_enabled() && (wants_grad(q) || wants_grad(k) || wants_grad(wq) || wants_grad(wk))) {
         const variable_list y = Norm::apply(q, k, pq, pk, wq, wk, freq, eps, interleaved, amplitude);
@@ -295,6 +305,7 @@ struct Attention : public torch::autograd::Function<Attention> {
         return out;
     }
     static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+        no_tangent("diff_attention", {grads[0]});
         return once("diff_attention", gradients(ctx, grads[0]));
     }
     static variable_list gradients(AutogradContext* ctx, const Tensor& grad) {
@@ -332,6 +343,7 @@ MaybeTensor attention(const Tensor& q, const Tensor& k, const Tensor& v, const T
         return std::nullopt;
     if (key_mask.has_value() && !is_vector(*key_mask, q, at::kBool, k.size(0)) && !is_vector(*key_mask, q, at::kByte, k.size(0))) return std::nullopt;
     if (window.has_value() && (!causal || *window < 1)) return std::nullopt;
+    no_tangent("diff_attention", {q, k, v, lam});
     const double c = scale.has_value() ? *scale : 1.0 / std::sqrt((double)q.size(3));
     if (at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || v.requires_grad() || lam.requires_grad()))
         return Attention::apply(q, k, v, lam, k_ptr, q_ptr, c, causal, window.value_or(0), key_mask);

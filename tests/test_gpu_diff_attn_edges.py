@@ -6,7 +6,7 @@ import pytest
 import torch
 
 import attn_plain as plain
-from starrygl_amd.nn.model import diff_attention
+from starrygl_amd.nn.model import diff_attention, qk_norm_rotary, rotary_encode, rotary_frequencies
 from test_gpu_diff_attn import BF16, F16, F32, _check, _inputs, _ptr, _within
 
 pytestmark = pytest.mark.gpu
@@ -144,3 +144,32 @@ def test_scores_of_minus_infinity(hot, form, dtype):
     assert not y[nq:].any() and not grads[0][nq:].any() and not grads[1][n:].any() and not grads[2][n:].any()
     for got, name, m in ((grads[1], "dk", n), (grads[2], "dv", n), (grads[3], "dlam", None)):
         _within(got if m is None else got[:m], ref, name)
+
+
+def test_forward_mode_derivatives_are_refused(hot):
+    """a tangent of any input is not dropped without a word"""
+    import torch.autograd.forward_ad as fwAD
+    q, k, v, lam, _ = _inputs(3, 9, 2, 1, 16, 32, F32, 1)
+    kp, pos, freq = _ptr([2, 4, 3]), torch.arange(3, device="cuda"), rotary_frequencies(16)[0].cuda()
+    w = torch.ones(16, device="cuda")
+    calls = [(lambda *t: diff_attention(*t, kp), (q, k, v, lam)),
+             (lambda x: rotary_encode(x, pos, freq), (q.flatten(1, 2),)),
+             (lambda a, b, c, d: qk_norm_rotary(a, b, pos, pos, c, d, freq), (q.flatten(1, 2), q[:, 0], w, w.clone()))]
+    for call, args in calls:
+        call(*args)
+        for i in range(len(args)):
+            for strided in (False, True):                  # brought into the plain form first, or not
+                with fwAD.dual_level():
+                    ins = list(args)
+                    t = ins[i]
+                    if strided and t.dim() > 1:
+                        t = t.repeat_interleave(2, -1)[..., ::2]
+                    ins[i] = fwAD.make_dual(t, torch.ones_like(t))
+                    with pytest.raises(NotImplementedError, match="forward"):
+                        call(*ins)
+        # nor that of a gradient on its way back
+        leaves = [t.detach().clone().requires_grad_() for t in args]
+        y = call(*leaves)
+        y = y[0] if isinstance(y, tuple) else y
+        with fwAD.dual_level(), pytest.raises(NotImplementedError, match="forward"):
+            torch.autograd.grad(y, leaves[0], fwAD.make_dual(torch.ones_like(y), torch.ones_like(y)))
