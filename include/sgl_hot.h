@@ -788,7 +788,8 @@ int32_t sgl_qk_norm_rotary_backward(const sgl_rotary_params* p, double eps, int3
  *   v   (key, Hk, Dv)                      out (row, Hq, Dv)
  * Sequence b has the queries [q_ptr[b], q_ptr[b+1]) (q_ptr NULL: the one query
  * b, Tq = B) and the keys [k_ptr[b], k_ptr[b+1]) (root_start_ptr of a sampled
- * hop, for one); both pointer arrays ascend.  Query i of nq sees key j of nk when
+ * hop, for one); both pointer arrays ascend, and entries outside the rows count
+ * as 0 or as Tq, Tk.  Query i of nq sees key j of nk when
  *   !causal, or i + nk - nq - window < j <= i + nk - nq  (window 0: no lower end),
  * and key_mask (NULL: all) is not 0 there.  A query that sees no key, or only keys
  * whose score is -inf, gives zeros and passes no gradient.  Values of keys that a

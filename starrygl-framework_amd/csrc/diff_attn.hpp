@@ -114,7 +114,7 @@ __device__ __forceinline__ Span keys_of(const sgl_diff_attn_args& a, int32_t seq
     const int32_t k0 = clamp_to(a.k_ptr[seq], a.Tk), k1 = clamp_to(a.k_ptr[seq + 1], a.Tk);
     int64_t lo = k0, hi = k1;
     if (a.causal) {
-        const int64_t last = k1 - (a.q_ptr ? a.q_ptr[seq + 1] - i : 1);       // the key that stands where the query does
+        const int64_t last = k1 - (a.q_ptr ? clamp_to(a.q_ptr[seq + 1], a.Tq) - i : 1);       // the key that stands where the query does
         if (last + 1 < hi) hi = last + 1;
         if (a.window > 0 && last + 1 - a.window > lo) lo = last + 1 - a.window;
     }

@@ -173,3 +173,19 @@ def test_forward_mode_derivatives_are_refused(hot):
         y = y[0] if isinstance(y, tuple) else y
         with fwAD.dual_level(), pytest.raises(NotImplementedError, match="forward"):
             torch.autograd.grad(y, leaves[0], fwAD.make_dual(torch.ones_like(y), torch.ones_like(y)))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("window", [None, 9])
+def test_pointers_behind_the_rows_count_as_the_last_row(hot, window, dtype):
+    """worst-case pointers may say more rows than there are: forward and gradients as with the pointers clamped"""
+    q, k, v, lam, go = _inputs(90, 100, 2, 1, 32, 64, dtype, 3)
+    q_ptr, k_ptr = torch.tensor([0, 40, 130], device="cuda"), torch.tensor([0, 40, 117], device="cuda")
+    got = _check(q, k, v, lam, go, k_ptr.clamp(max=100), q_ptr.clamp(max=90), causal=True, window=window)[0]
+    leaves = [t.detach().requires_grad_() for t in (q, k, v, lam)]
+    y = diff_attention(*leaves, k_ptr, q_ptr, causal=True, window=window)
+    assert torch.equal(y, got)
+    grads = torch.autograd.grad(y, leaves, go)
+    ref = plain.diff_attention(q, k, v, lam, k_ptr.clamp(max=100), q_ptr.clamp(max=90), causal=True, window=window, grad=go)
+    for n, t in zip(("dq", "dk", "dv", "dlam"), grads):
+        _within(t, ref, n)
