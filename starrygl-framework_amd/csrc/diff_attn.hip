@@ -52,7 +52,7 @@ int32_t check_args(const char* what, const sgl_diff_attn_args* a, bool backward)
     if (a->window > 0 && !a->causal) return fail(SGL_EINVAL, "%s: a window needs causal", what);
     if (!a->q_ptr && a->Tq != a->B) return fail(SGL_EINVAL, "%s: without q_ptr there is one query per sequence (Tq = B)", what);
     if (!a->k_ptr || !a->lam) return fail(SGL_EINVAL, "%s: k_ptr/lam is NULL", what);
-    if (!(a->scale > -INFINITY && a->scale < INFINITY)) return fail(SGL_EINVAL, "%s: scale is not finite", what);
+    if (!(fabs(a->scale) * LOG2E <= 3.4e38)) return fail(SGL_EINVAL, "%s: scale is not finite in 32 bits", what);
     if (a->Tq > 0 && (!a->q.data || !a->out.data)) return fail(SGL_EINVAL, "%s: q/out is NULL", what);
     if (a->Tk > 0 && (!a->k.data || !a->v.data)) return fail(SGL_EINVAL, "%s: k/v is NULL", what);
     if ((a->lse == nullptr) != (a->o2.data == nullptr)) return fail(SGL_EINVAL, "%s: lse and o2 come together", what);
