@@ -40,8 +40,8 @@ inline AttnArgs attn_args(const sgl_diff_attn_args& a) {
     g.a = a;
     if (a.window > 0x7FFFFFFF) g.a.window = 0;      // wider than any sequence
     g.scale = (float)a.scale;
-    // a scale of zero must not turn the -inf of a hidden score into a NaN: with 1e-30 every visible score vanishes too
-    g.c2 = fmaxf(fabsf(g.scale) * LOG2E, 1e-30f);
+    // a scale of zero must not turn the -inf of a hidden score into a NaN: with 2^-149 every visible score vanishes too
+    g.c2 = fmaxf(fabsf(g.scale) * LOG2E, 0x1p-149f);
     g.negate = g.scale < 0.f;
     g.parts = 1;
     return g;

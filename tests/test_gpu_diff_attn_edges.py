@@ -189,3 +189,21 @@ def test_pointers_behind_the_rows_count_as_the_last_row(hot, window, dtype):
     ref = plain.diff_attention(q, k, v, lam, k_ptr.clamp(max=100), q_ptr.clamp(max=90), causal=True, window=window, grad=go)
     for n, t in zip(("dq", "dk", "dv", "dlam"), grads):
         _within(t, ref, n)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("scale", [0.0, 1e-36, -1e-36])
+@pytest.mark.parametrize("form", ["few keys", "single queries", "rows"])
+def test_tiny_scales_of_huge_scores(hot, form, scale, dtype):
+    """products of 10^37 times a scale of 10^-36 are scores like any other; times zero they all are zero"""
+    n, nq = {"few keys": (12, 1), "single queries": (300, 1), "rows": (70, 50)}[form]
+    q, k, v, lam, go = _inputs(nq, n, 4, 2, 32, 64, dtype, 19)
+    mask = torch.arange(n, device="cuda") % 5 != 3
+    _check(q * 2.0 ** 60, k * 2.0 ** 60, v, lam, go, _ptr([n]), None if nq == 1 else _ptr([nq]), scale=scale, key_mask=mask)
+
+
+def test_scales_past_32_bits_are_refused(hot):
+    q, k, v, lam, _ = _inputs(1, 4, 2, 1, 16, 32, F32, 1)
+    for scale in (1e39, -1e39, 3e38, math.inf, math.nan):
+        with pytest.raises(ValueError, match="scale is not finite"):
+            diff_attention(q, k, v, lam, _ptr([4]), scale=scale)
