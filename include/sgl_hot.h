@@ -38,7 +38,7 @@
 extern "C" {
 #endif
 
-#define SGL_ABI_VERSION 9
+#define SGL_ABI_VERSION 10
 
 /* ------------------------------------------------------------------ status */
 #define SGL_OK        0
@@ -813,17 +813,24 @@ typedef struct {
     sgl_rows       q, k, v, out;
     float*         lse;                /* device [Tq, Hq, 2]: log2 of the sum of exp(S_m); NULL in a
                                         * forward call that no backward follows */
-    sgl_rows       o2;                 /* softmax(S_2) v, kept for the backward; data NULL likewise */
+    sgl_rows       o2;                 /* softmax(S_2) v, for the backward; data NULL: not kept */
     sgl_rows       d_out, d_q, d_k, d_v;  /* backward */
     float*         d_lam;              /* device [Hq] */
+    float*         maps;               /* device [Tq, Hq, 2, Dv], 16-byte aligned: softmax(S_m) v before any
+                                        * rounding, for the backward; NULL: not kept */
     int32_t        flags, reserved;
 } sgl_diff_attn_args;
 
 size_t  sgl_diff_attn_workspace_bytes(const sgl_diff_attn_args* a);
 int32_t sgl_diff_attn(const sgl_diff_attn_args* a, void* workspace,
                       size_t workspace_bytes, void* stream);
-/* Reads q, k, v, lam, out, lse, o2, d_out; writes d_q, d_k, d_v, d_lam.  No
- * atomics: the same inputs give the same bits. */
+/* Reads q, k, v, lam, lse, d_out, and maps, or (maps NULL) out and o2; writes
+ * d_q, d_k, d_v, d_lam.  The row sums t_m = d_out . softmax(S_m) v, which every
+ * score's gradient has subtracted, come from these: in 16 bits out and o2 have
+ * been rounded, and a query that sees one key, whose score has no gradient, gets
+ * one of the size of that rounding; from maps it does not.  A forward call before
+ * a backward one writes lse and maps, or lse and o2.  No atomics: the same inputs
+ * give the same bits. */
 size_t  sgl_diff_attn_backward_workspace_bytes(const sgl_diff_attn_args* a);
 int32_t sgl_diff_attn_backward(const sgl_diff_attn_args* a, void* workspace,
                                size_t workspace_bytes, void* stream);

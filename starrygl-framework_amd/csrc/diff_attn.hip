@@ -5,7 +5,12 @@
 // Backward: P_m = 2^(S_m - lse_m), dP = d_out v^T (one product for both maps), t_m = sum_j P_m dP = d_out o_m,
 //   dS_1 = P_1 (dP - t_1), dS_2 = -lam P_2 (dP - t_2), d_lam = -sum t_2,
 //   dV = (P_1 - lam P_2)^T d_out, dK_m = scale dS_m^T q_m, dQ_m = scale dS_m k_m.
-// d_lam sums P_2 dP in fp32 rather than d_out o_2, whose o_2 is rounded to the inputs' type.
+// t_m is taken from o_m, for which a call that a backward one follows keeps both maps' results as they are, in fp32 (`maps`): the
+// scores' gradients are differences P (dP - t) that mostly cancel where one key has all the weight, so a t that is off by a
+// rounding to 16 bits shows in dQ and dK whole (off by 0.005 to 0.007 in bf16 over rows of 10 to 200 keys with scores of a few
+// tens, 0.0024 from rounding dS alone; not zero where one key is seen).  It costs 6 bytes more an element written and 4 more
+// read: 8 sequences of 2048, 16 heads over 4, 64 wide, causal, bf16, forward 268 -> 318 us (50 us; through LDS 351, past the caches
+// 364), rows of the backward 297 -> 318.  In fp32 out and o_2 do (t_1 from out + lam o_2).  d_lam sums P_2 dP.
 #include "diff_attn.hpp"
 
 namespace sgl {
@@ -41,7 +46,10 @@ namespace {
 
 constexpr int64_t PAIRS_MAX = 0x7FFFFFFF, COUNT_MAX = 0x7FFFFF00;
 
-int32_t check_args(const char* what, const sgl_diff_attn_args* a, bool backward) {
+// SIZES: of a backward call whose gradients need not be there yet
+enum Call { FORWARD, SIZES, BACKWARD };
+
+int32_t check_args(const char* what, const sgl_diff_attn_args* a, Call call) {
     if (!a) return fail(SGL_EINVAL, "%s: args is NULL", what);
     if (a->dtype != SGL_DT_F32 && a->dtype != SGL_DT_BF16 && a->dtype != SGL_DT_F16) return fail(SGL_EINVAL, "%s: bad dtype", what);
     if (a->D < 1 || a->D > 128 || a->Dv < 1 || a->Dv > 256) return fail(SGL_ENOTSUP, "%s: D must lie in [1, 128] and Dv in [1, 256]", what);
@@ -53,12 +61,13 @@ int32_t check_args(const char* what, const sgl_diff_attn_args* a, bool backward)
     if (!a->q_ptr && a->Tq != a->B) return fail(SGL_EINVAL, "%s: without q_ptr there is one query per sequence (Tq = B)", what);
     if (!a->k_ptr || !a->lam) return fail(SGL_EINVAL, "%s: k_ptr/lam is NULL", what);
     if (!(fabs(a->scale) * LOG2E <= 3.4e38)) return fail(SGL_EINVAL, "%s: scale is not finite in 32 bits", what);
-    if (a->Tq > 0 && (!a->q.data || !a->out.data)) return fail(SGL_EINVAL, "%s: q/out is NULL", what);
+    if (a->Tq > 0 && (!a->q.data || (!a->out.data && !(call != FORWARD && a->maps)))) return fail(SGL_EINVAL, "%s: q/out is NULL", what);
     if (a->Tk > 0 && (!a->k.data || !a->v.data)) return fail(SGL_EINVAL, "%s: k/v is NULL", what);
-    if ((a->lse == nullptr) != (a->o2.data == nullptr)) return fail(SGL_EINVAL, "%s: lse and o2 come together", what);
-    if (backward) {
+    if ((a->lse == nullptr) != (a->o2.data == nullptr && a->maps == nullptr)) return fail(SGL_EINVAL, "%s: lse comes with o2 or maps", what);
+    if (reinterpret_cast<uintptr_t>(a->maps) % 16) return fail(SGL_EINVAL, "%s: maps is not aligned to 16 bytes", what);
+    if (call == BACKWARD) {
         if (!a->d_lam || (a->Tq > 0 && (!a->lse || !a->d_out.data || !a->d_q.data)) || (a->Tk > 0 && (!a->d_k.data || !a->d_v.data)))
-            return fail(SGL_EINVAL, "%s: lse, o2 or a gradient is NULL", what);
+            return fail(SGL_EINVAL, "%s: lse, o2 and maps, or a gradient is NULL", what);
     }
     // (blocks are counted in 32 bits)
     if (a->Tq * a->Hq > PAIRS_MAX || a->Tk * a->Hk > PAIRS_MAX) return fail(SGL_ENOTSUP, "%s: Tq * Hq and Tk * Hk must stay below 2^31", what);
@@ -101,9 +110,9 @@ size_t forward_need(const sgl_diff_attn_args& a, int32_t parts) {
 
 int64_t backward_row_tiles(const sgl_diff_attn_args& a) { return ceil_div<int64_t>(a.Tq, QUERY_ROWS); }
 size_t backward_need(const sgl_diff_attn_args& a) {
-    if (!a.q_ptr) return align_up((size_t)seg_blocks(a) * (size_t)a.Hq * sizeof(float));
-    return align_up((size_t)a.Tq * (size_t)a.Hq * 2 * sizeof(float)) +
-           align_up((size_t)backward_row_tiles(a) * (size_t)a.Hq * sizeof(float)) + 256;
+    const size_t sums = align_up((size_t)a.Tq * (size_t)a.Hq * 2 * sizeof(float));
+    if (!a.q_ptr) return align_up((size_t)seg_blocks(a) * (size_t)a.Hq * sizeof(float)) + (a.Hq == a.Hk ? 0 : sums);
+    return sums + align_up((size_t)backward_row_tiles(a) * (size_t)a.Hq * sizeof(float)) + 256;
 }
 
 }  // namespace
@@ -114,11 +123,11 @@ using namespace sgl;
 using namespace sgl::attn;
 
 extern "C" size_t sgl_diff_attn_workspace_bytes(const sgl_diff_attn_args* a) {
-    return check_args("diff_attn", a, false) ? 0 : forward_need(*a, forward_parts(*a));
+    return check_args("diff_attn", a, FORWARD) ? 0 : forward_need(*a, forward_parts(*a));
 }
 
 extern "C" int32_t sgl_diff_attn(const sgl_diff_attn_args* a, void* workspace, size_t workspace_bytes, void* stream) {
-    if (int32_t rc = check_args("diff_attn", a, false)) return rc;
+    if (int32_t rc = check_args("diff_attn", a, FORWARD)) return rc;
     if (a->Tq == 0) return SGL_OK;
     AttnArgs g = attn_args(*a);
     g.grain = grain_of(*a);
@@ -140,11 +149,11 @@ extern "C" int32_t sgl_diff_attn(const sgl_diff_attn_args* a, void* workspace, s
 }
 
 extern "C" size_t sgl_diff_attn_backward_workspace_bytes(const sgl_diff_attn_args* a) {
-    return check_args("diff_attn_backward", a, false) ? 0 : backward_need(*a);
+    return check_args("diff_attn_backward", a, SIZES) ? 0 : backward_need(*a);
 }
 
 extern "C" int32_t sgl_diff_attn_backward(const sgl_diff_attn_args* a, void* workspace, size_t workspace_bytes, void* stream) {
-    if (int32_t rc = check_args("diff_attn_backward", a, true)) return rc;
+    if (int32_t rc = check_args("diff_attn_backward", a, BACKWARD)) return rc;
     const size_t need = backward_need(*a);
     if (!workspace || workspace_bytes < need) return fail(SGL_ENOMEM, "diff_attn_backward: workspace of %zu bytes, %zu needed", workspace_bytes, need);
     AttnArgs g = attn_args(*a);
@@ -152,6 +161,7 @@ extern "C" int32_t sgl_diff_attn_backward(const sgl_diff_attn_args* a, void* wor
     Arena ws(workspace, workspace_bytes);
     if (!a->q_ptr) {
         g.lam_part = ws.take<float>((size_t)seg_blocks(*a) * (size_t)a->Hq);
+        if (a->Hq != a->Hk) g.delta = ws.take<float>((size_t)a->Tq * (size_t)a->Hq * 2);
         seg_backward(g, as_stream(stream));
     } else {
         g.delta = ws.take<float>((size_t)a->Tq * (size_t)a->Hq * 2);

@@ -27,6 +27,7 @@ struct AttnArgs {
     float c2;                   // |scale| log2(e): scores enter exponentials of base 2
     int32_t negate;             // scale < 0: the operand that stays in registers changes its sign (exact)
     int32_t grain;              // bytes, 16 at most, that divide the address of every row and the length of every row's head
+    int32_t map_grain;          // the same of the rows of `maps`
     int32_t parts;              // forward: partial results per (row, head, map), joined by a second kernel; 1: none
     int64_t first;              // first block of a launch: large grids go out in parts
     float* part_ml;             // [parts, Tq * Hq, 2, 2]: running maximum (in powers of two) and sum
@@ -43,6 +44,7 @@ inline AttnArgs attn_args(const sgl_diff_attn_args& a) {
     // a scale of zero must not turn the -inf of a hidden score into a NaN: with 2^-149 every visible score vanishes too
     g.c2 = fmaxf(fabsf(g.scale) * LOG2E, 0x1p-149f);
     g.negate = g.scale < 0.f;
+    g.map_grain = a.Dv % 4 == 0 ? 16 : a.Dv % 2 == 0 ? 8 : 4;
     g.parts = 1;
     return g;
 }
@@ -559,6 +561,20 @@ template <typename T, bool WHOLE>
 __device__ __forceinline__ typename Mat<T>::Frag global_frag(const T* src, int e, int len, int grain) {
     if constexpr (WHOLE) return *reinterpret_cast<const typename Mat<T>::Frag*>(src + e);
     else return load_chunk<T>(src + e, len - e, grain);
+}
+
+// of map m of (row i, head h)
+__device__ __forceinline__ float* map_row(const sgl_diff_attn_args& a, int64_t i, int h, int m) { return a.maps + (pair_at(a, i, h) + m) * a.Dv; }
+// sum += x . (the same elements of a row of `maps`, from element e)
+template <typename T, bool WHOLE>
+__device__ __forceinline__ float dot_map(const typename Mat<T>::Frag& x, const float* src, int e, int len, int grain, float sum) {
+#pragma unroll
+    for (int u = 0; u < Mat<T>::EP; u += 4) {
+        const f32x4 y = global_frag<float, WHOLE>(src, e + u, len, grain);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) sum = __builtin_fmaf((float)x[u + j], y[j], sum);
+    }
+    return sum;
 }
 
 __device__ __forceinline__ f32x16 zero16() {

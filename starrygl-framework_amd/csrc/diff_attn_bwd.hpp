@@ -134,7 +134,7 @@ __global__ __launch_bounds__((Rows<T, DP>::WAVES * 64), (Rows<T, DP>::OCC)) void
 #pragma unroll
     for (int w = 1; w < P::WAVES; ++w) lo = min(lo, s_lo[w]), hi = max(hi, s_hi[w]);
 
-    // t_m = sum over the values of d_out * o_m, with o_1 = out + lam o_2
+    // t_m = sum over the values of d_out * o_m: of the unrounded results if they were kept, or with o_1 = out + lam o_2
     const float lam = a.lam[h];
     typename M::Frag q[2][S::QS], go[S::VS];
     float t[2] = {0.f, 0.f};
@@ -144,15 +144,23 @@ __global__ __launch_bounds__((Rows<T, DP>::WAVES * 64), (Rows<T, DP>::OCC)) void
 #pragma unroll
         for (int k = 0; k < S::QS; ++k) q[m][k] = global_frag<T, MODE == WHOLE_ROWS>(row<T>(a.q, ii, 2 * h + m), (2 * k + half) * S::EP, a.D, g.grain);
 #pragma unroll
-    for (int k = 0; k < S::VS; ++k) {
-        const int e = (2 * k + half) * S::EP;
-        go[k] = global_frag<T, MODE == WHOLE_ROWS>(row<T>(a.d_out, ii, h), e, a.Dv, g.grain);
-        const typename M::Frag y2 = global_frag<T, MODE == WHOLE_ROWS>(row<T>(a.o2, ii, h), e, a.Dv, g.grain);
-        const typename M::Frag y = global_frag<T, MODE == WHOLE_ROWS>(row<T>(a.out, ii, h), e, a.Dv, g.grain);
+    for (int k = 0; k < S::VS; ++k) go[k] = global_frag<T, MODE == WHOLE_ROWS>(row<T>(a.d_out, ii, h), (2 * k + half) * S::EP, a.Dv, g.grain);
+    if (a.maps) {
 #pragma unroll
-        for (int j = 0; j < S::EP; ++j) {
-            t[0] = __builtin_fmaf((float)go[k][j], __builtin_fmaf(lam, (float)y2[j], (float)y[j]), t[0]);
-            t[1] = __builtin_fmaf((float)go[k][j], (float)y2[j], t[1]);
+        for (int k = 0; k < S::VS; ++k)
+#pragma unroll
+            for (int m = 0; m < 2; ++m) t[m] = dot_map<T, MODE == WHOLE_ROWS>(go[k], map_row(a, ii, h, m), (2 * k + half) * S::EP, a.Dv, g.map_grain, t[m]);
+    } else {
+#pragma unroll
+        for (int k = 0; k < S::VS; ++k) {
+            const int e = (2 * k + half) * S::EP;
+            const typename M::Frag y2 = global_frag<T, MODE == WHOLE_ROWS>(row<T>(a.o2, ii, h), e, a.Dv, g.grain);
+            const typename M::Frag y = global_frag<T, MODE == WHOLE_ROWS>(row<T>(a.out, ii, h), e, a.Dv, g.grain);
+#pragma unroll
+            for (int j = 0; j < S::EP; ++j) {
+                t[0] = __builtin_fmaf((float)go[k][j], __builtin_fmaf(lam, (float)y2[j], (float)y[j]), t[0]);
+                t[1] = __builtin_fmaf((float)go[k][j], (float)y2[j], t[1]);
+            }
         }
     }
     float lse[2];

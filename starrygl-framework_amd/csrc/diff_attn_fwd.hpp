@@ -12,7 +12,9 @@
 // groups of waves take every other sub-tile of keys.
 //
 // Probabilities are rounded to the inputs' type for their product with the values (the matrix units take no other): by at most
-// h = 2^-9 in bf16 (2^-12 in fp16) of each, once; their sum is taken before.  Sums, maxima and results are fp32.
+// h = 2^-8 in bf16 (2^-11 in fp16) of each, once; their sum is taken before.  Sums, maxima and results are fp32.  Over 4096 keys
+// each map is off by 0.0017 in bf16 (2-norm; by 0.0002 in fp16), out, a difference of two that have the values' mean in common, by
+// 0.0025 where rounding the exact result alone gives 0.0017.  P in two operands would take that away for half as many products again.
 //
 // Bound by the matrix and vector instructions, which overlap between the two waves of a SIMD only in part (a tile of 32 x 32: 768
 // cycles of products, about 720 of vector instructions, 2000 measured).  8 sequences of 2048, 16 heads over 4, 64 wide, causal,
@@ -145,8 +147,29 @@ __device__ __forceinline__ void step(State<T, DP, MAPS>& st, const typename Mat<
     });
 }
 
-// HEADS: the columns are the query heads of one key head, all at query `seq`; otherwise 32 query rows of one head
-template <typename T, int DP, bool HEADS, int MODE>
+// the results of a column as they are
+template <int VT, bool WHOLE>
+__device__ __forceinline__ void store_map(const f32x16 (&x)[VT], float* to, int Dv, int half) {
+#pragma unroll
+    for (int t = 0; t < VT; ++t)
+#pragma unroll
+        for (int r4 = 0; r4 < 4; ++r4) {
+            const int d = t * 32 + 8 * r4 + 4 * half;
+            const f32x4 y = {x[t][4 * r4], x[t][4 * r4 + 1], x[t][4 * r4 + 2], x[t][4 * r4 + 3]};
+            if (WHOLE || Dv % 4 == 0) {
+                if (d < Dv) *reinterpret_cast<f32x4*>(to + d) = y;
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (d + e < Dv) to[d + e] = y[e];
+            }
+        }
+}
+
+// HEADS: the columns are the query heads of one key head, all at query `seq`; otherwise 32 query rows of one head.  KEEP: the
+// results of both maps are kept as they are too (in kernels of their own: the stores cost a forward pass that keeps nothing
+// registers, 248 us instead of 226 for 32 ragged histories of up to 2048, 8 heads of 64, causal, fp16)
+template <typename T, int DP, bool HEADS, int MODE, bool KEEP>
 __global__ __launch_bounds__((Shape<T, DP, HEADS>::NT), (HEADS && Shape<T, DP, HEADS>::RB > 512 ? 1 : 2)) void fwd_kernel(AttnArgs g, FwdWork w) {
     typedef Shape<T, DP, HEADS> S;
     typedef Mat<T> M;
@@ -306,21 +329,7 @@ __global__ __launch_bounds__((Shape<T, DP, HEADS>::NT), (HEADS && Shape<T, DP, H
             const int64_t at = (((int64_t)part * a.Tq + i) * a.Hq + h) * 2 + map0 + c;
             if (half == 0) g.part_ml[2 * at] = st.m[c], g.part_ml[2 * at + 1] = none ? -1.f : l;
             if (none) continue;
-            float* o = g.part_o + at * a.Dv;
-#pragma unroll
-            for (int t = 0; t < VT; ++t)
-#pragma unroll
-                for (int r4 = 0; r4 < 4; ++r4) {
-                    const int d = t * 32 + 8 * r4 + 4 * half;
-                    const f32x4 x = {st.o[c][t][4 * r4], st.o[c][t][4 * r4 + 1], st.o[c][t][4 * r4 + 2], st.o[c][t][4 * r4 + 3]};
-                    if (WHOLE || a.Dv % 4 == 0) {
-                        if (d < a.Dv) *reinterpret_cast<f32x4*>(o + d) = x;
-                    } else {
-#pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            if (d + e < a.Dv) o[d + e] = x[e];
-                    }
-                }
+            store_map<VT, WHOLE>(st.o[c], g.part_o + at * a.Dv, a.Dv, half);
         }
         return;
     }
@@ -337,16 +346,24 @@ __global__ __launch_bounds__((Shape<T, DP, HEADS>::NT), (HEADS && Shape<T, DP, H
         constexpr int SHARE = S::TILE / (S::WAVES / 2);                     // a wave's part of the two buffers
         char* own = (wave < S::WAVES / 2 ? s_a : s_b) + wave % (S::WAVES / 2) * SHARE;
         const uint32_t keep = (uint32_t)__ballot(mine);
+        if constexpr (KEEP || MAPS == 1) {
+#pragma unroll
+            for (int c = 0; c < MAPS; ++c) {
+#pragma unroll
+                for (int t = 0; t < VT; ++t)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) st.o[c][t][r] = inv[c] == 0.f ? 0.f : st.o[c][t][r] * inv[c];
+                // (32 bytes of a row at a time, a cache line in four stores)
+                if (KEEP && mine) store_map<VT, WHOLE>(st.o[c], map_row(a, i, h, map0 + c), a.Dv, half);
+            }
+        }
         if constexpr (MAPS == 2) {
-            const auto second = [&](int t, int r) { return inv[1] == 0.f ? 0.f : st.o[1][t][r] * inv[1]; };
-            store_rows<T, SHARE / 32, VT, WHOLE>([&](int t, int r) { return __builtin_fmaf(-lam, second(t, r), inv[0] == 0.f ? 0.f : st.o[0][t][r] * inv[0]); }, own, lane, a.Dv,
-                                               g.grain, row_out<T>(a.out, i0, h), a.out.row_stride, keep);
-            if (a.o2.data) store_rows<T, SHARE / 32, VT, WHOLE>(second, own, lane, a.Dv, g.grain, row_out<T>(a.o2, i0, h), a.o2.row_stride, keep);
+            const auto value = [&](int c, int t, int r) { return KEEP ? st.o[c][t][r] : inv[c] == 0.f ? 0.f : st.o[c][t][r] * inv[c]; };
+            store_rows<T, SHARE / 32, VT, WHOLE>([&](int t, int r) { return __builtin_fmaf(-lam, value(1, t, r), value(0, t, r)); }, own, lane, a.Dv, g.grain, row_out<T>(a.out, i0, h),
+                                                 a.out.row_stride, keep);
+            if (a.o2.data)
+                store_rows<T, SHARE / 32, VT, WHOLE>([&](int t, int r) { return value(1, t, r); }, own, lane, a.Dv, g.grain, row_out<T>(a.o2, i0, h), a.o2.row_stride, keep);
         } else {
-#pragma unroll
-            for (int t = 0; t < VT; ++t)
-#pragma unroll
-                for (int r = 0; r < 16; ++r) st.o[0][t][r] = inv[0] == 0.f ? 0.f : st.o[0][t][r] * inv[0];
             // the second map's waves hand their results over, the first's subtract them; a 32 x 32 tile takes 4 KB, half the
             // groups use each buffer
             constexpr int SLOT = 4096, AT_ONCE = S::TILE / (S::GROUPS / 2 * SLOT);
@@ -467,6 +484,7 @@ __global__ __launch_bounds__(BLOCK) void join_kernel(AttnArgs g) {
     for (int m = 0; m < 2; ++m) o[m] = s_lse[m] == INFINITY ? 0.f : o[m];       // no key, or only scores of -inf
     row_out<T>(a.out, i, h)[d] = (T)__builtin_fmaf(-a.lam[h], o[1], o[0]);
     if (a.o2.data) row_out<T>(a.o2, i, h)[d] = (T)o[1];
+    if (a.maps) map_row(a, i, h, 0)[d] = o[0], map_row(a, i, h, 1)[d] = o[1];
 }
 
 template <typename T, int DP>
@@ -477,8 +495,9 @@ void launch(const AttnArgs& g, hipStream_t st) {
     auto go = [&](auto mode) {
         constexpr int MODE = decltype(mode)::value;
         in_parts(g, blocks, [&](const AttnArgs& part, dim3 grid) {
-            if (g.a.q_ptr) hipLaunchKernelGGL((fwd_kernel<T, DP, false, MODE>), grid, dim3(ROW_NT), 0, st, part, w);
-            else hipLaunchKernelGGL((fwd_kernel<T, DP, true, MODE>), grid, dim3(HEAD_NT), 0, st, part, w);
+            if (!g.a.q_ptr) hipLaunchKernelGGL((fwd_kernel<T, DP, true, MODE, false>), grid, dim3(HEAD_NT), 0, st, part, w);
+            else if (g.a.maps && g.parts == 1) hipLaunchKernelGGL((fwd_kernel<T, DP, false, MODE, true>), grid, dim3(ROW_NT), 0, st, part, w);
+            else hipLaunchKernelGGL((fwd_kernel<T, DP, false, MODE, false>), grid, dim3(ROW_NT), 0, st, part, w);
         });
     };
     const int mode = stage_mode(g, DP, {&g.a.k, &g.a.v});

@@ -143,6 +143,13 @@ __global__ __launch_bounds__(BLOCK) void seg_fwd_kernel(AttnArgs g) {
     }
     if (ln.slot != 0) return;
     const float lam = a.lam[h];
+    if (a.maps) {
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int u = 0; u < EP; u += 4)
+                store_chunk<float>(map_row(a, i, h, t) + ln.ev + u, f32x4{o[t][u], o[t][u + 1], o[t][u + 2], o[t][u + 3]}, a.Dv - ln.ev - u, g.map_grain);
+    }
     if (a.o2.data) store_part<T>(row_out<T>(a.o2, i, h), o[1], 1.f, ln.ev, a.Dv, g.grain);
 #pragma unroll
     for (int e = 0; e < EP; ++e) o[0][e] = __builtin_fmaf(-lam, o[1][e], o[0][e]);
@@ -150,7 +157,7 @@ __global__ __launch_bounds__(BLOCK) void seg_fwd_kernel(AttnArgs g) {
 }
 
 // DQ: a wave's unit is (sequence, query head), it sums dQ and d_lam's share.  DKV: (sequence, key head), it writes dK and dV,
-// summed over the heads of the group.  Groups of one head do both at once.
+// summed over the heads of the group; it reads the row sums t_m that the former leaves.  Groups of one head do both at once.
 template <typename T, int L, bool DQ, bool DKV>
 __global__ __launch_bounds__(BLOCK) void seg_bwd_kernel(AttnArgs g) {
     constexpr int EP = Mat<T>::EP, SLOTS = 64 / L;
@@ -170,22 +177,34 @@ __global__ __launch_bounds__(BLOCK) void seg_bwd_kernel(AttnArgs g) {
         const Span span = keys_of(a, i < B ? (int32_t)i : -1, i);
         float q[EP], go[EP], t[2], lse[2], dq[EP], lam = 0.f;
         auto of_head = [&](int h) {
-            float y[EP], y2[EP];
             lam = a.lam[h];
             load_part<T>(q, row<T>(a.q, i, 2 * h + ln.half), ln.e, a.D, true, g.grain);
-            load_part<T>(go, row<T>(a.d_out, i, h), ln.ev, a.Dv, true, g.grain);
-            load_part<T>(y, row<T>(a.out, i, h), ln.ev, a.Dv, true, g.grain);
-            load_part<T>(y2, row<T>(a.o2, i, h), ln.ev, a.Dv, true, g.grain);
+            const typename Mat<T>::Frag x = global_frag<T, false>(row<T>(a.d_out, i, h), ln.ev, a.Dv, g.grain);
+            widen<T>(go, x);
+            lse[0] = a.lse[pair_at(a, i, h)];
+            lse[1] = a.lse[pair_at(a, i, h) + 1];
+            if (!DQ) {
+                t[0] = g.delta[pair_at(a, i, h)];
+                t[1] = g.delta[pair_at(a, i, h) + 1];
+                return;
+            }
             t[0] = t[1] = 0.f;
+            if (a.maps) {
 #pragma unroll
-            for (int e = 0; e < EP; ++e) {
-                t[1] = __builtin_fmaf(go[e], y2[e], t[1]);
-                t[0] = __builtin_fmaf(go[e], __builtin_fmaf(lam, y2[e], y[e]), t[0]);
+                for (int m = 0; m < 2; ++m) t[m] = dot_map<T, false>(x, map_row(a, i, h, m), ln.ev, a.Dv, g.map_grain, 0.f);
+            } else {
+                float y[EP], y2[EP];
+                load_part<T>(y, row<T>(a.out, i, h), ln.ev, a.Dv, true, g.grain);
+                load_part<T>(y2, row<T>(a.o2, i, h), ln.ev, a.Dv, true, g.grain);
+#pragma unroll
+                for (int e = 0; e < EP; ++e) {
+                    t[1] = __builtin_fmaf(go[e], y2[e], t[1]);
+                    t[0] = __builtin_fmaf(go[e], __builtin_fmaf(lam, y2[e], y[e]), t[0]);
+                }
             }
             t[0] = lanes_sum<L>(t[0]);
             t[1] = lanes_sum<L>(t[1]);
-            lse[0] = a.lse[pair_at(a, i, h)];
-            lse[1] = a.lse[pair_at(a, i, h) + 1];
+            if (!DKV && lane == 0) g.delta[pair_at(a, i, h)] = t[0], g.delta[pair_at(a, i, h) + 1] = t[1];
         };
 #pragma unroll
         for (int e = 0; e < EP; ++e) dq[e] = 0.f;

@@ -273,15 +273,23 @@ sgl_diff_attn_args attn_args(const Tensor& q, const Tensor& k, const Tensor& v, 
     return a;
 }
 
-Tensor attn_forward(sgl_diff_attn_args& a, const Tensor& q, Tensor* lse, Tensor* o2) {
+// What the backward takes its row sums from: in fp32 out and o2, whose roundings are those of a sum; in 16 bits both maps'
+// results before they are rounded.
+void set_kept(sgl_diff_attn_args& a, const Tensor& lse, const Tensor& kept) {
+    if (a.Tq == 0) return;
+    a.lse = lse.data_ptr<float>();
+    if (kept.dim() == 3) a.o2 = rows(kept);
+    else a.maps = kept.data_ptr<float>();
+}
+
+Tensor attn_forward(sgl_diff_attn_args& a, const Tensor& q, Tensor* lse, Tensor* kept) {
     Tensor out = at::empty({a.Tq, a.Hq, a.Dv}, q.options());
     a.out = rows(out);
     if (lse) {
-        *lse = at::empty({a.Tq, a.Hq, 2}, q.options().dtype(at::kFloat));
-        *o2 = at::empty({a.Tq, a.Hq, a.Dv}, q.options());
-        a.lse = lse->data_ptr<float>();
-        a.o2 = rows(*o2);
-        if (a.Tq == 0) a.lse = nullptr, a.o2.data = nullptr;
+        const auto f32 = q.options().dtype(at::kFloat);
+        *lse = at::empty({a.Tq, a.Hq, 2}, f32);
+        *kept = a.dtype == SGL_DT_F32 ? at::empty({a.Tq, a.Hq, a.Dv}, f32) : at::empty({a.Tq, a.Hq, 2, a.Dv}, f32);
+        set_kept(a, *lse, *kept);
     }
     const c10::DeviceGuard guard(q.device());
     const size_t bytes = lib.attn_bytes(&a);
@@ -295,10 +303,10 @@ struct Attention : public torch::autograd::Function<Attention> {
     static Tensor forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& lam, const Tensor& k_ptr, const MaybeTensor& q_ptr,
                           double scale, bool causal, int64_t window, const MaybeTensor& key_mask) {
         sgl_diff_attn_args a = attn_args(q, k, v, lam, k_ptr, q_ptr, scale, causal, window, key_mask);
-        Tensor lse, o2;
-        Tensor out = attn_forward(a, q, &lse, &o2);
+        Tensor lse, kept;
+        Tensor out = attn_forward(a, q, &lse, &kept);
         const auto some = [](const MaybeTensor& t) { return t.has_value() ? *t : Tensor(); };
-        ctx->save_for_backward({q, k, v, lam, out, lse, o2, k_ptr, some(q_ptr), some(key_mask)});
+        ctx->save_for_backward({q, k, v, lam, kept.dim() == 3 ? out : Tensor(), lse, kept, k_ptr, some(q_ptr), some(key_mask)});
         ctx->saved_data["scale"] = scale;
         ctx->saved_data["causal"] = causal;
         ctx->saved_data["window"] = window;
@@ -312,15 +320,15 @@ struct Attention : public torch::autograd::Function<Attention> {
         const at::AutoGradMode off(false);
         const variable_list t = ctx->get_saved_variables();
         const auto some = [](const Tensor& x) { return x.defined() ? MaybeTensor(x) : std::nullopt; };
-        const Tensor &q = t[0], &k = t[1], &v = t[2], &lam = t[3], &out = t[4], &lse = t[5], &o2 = t[6];
+        const Tensor &q = t[0], &k = t[1], &v = t[2], &lam = t[3], &out = t[4];
         sgl_diff_attn_args a = attn_args(q, k, v, lam, t[7], some(t[8]), ctx->saved_data["scale"].toDouble(), ctx->saved_data["causal"].toBool(),
                                          ctx->saved_data["window"].toInt(), some(t[9]));
         const Tensor g = inner(grad);
         Tensor dq = at::empty(q.sizes(), q.options()), dk = at::empty(k.sizes(), k.options()), dv = at::empty(v.sizes(), v.options());
         Tensor dlam = at::empty({a.Hq}, lam.options());
-        a.out = rows(out), a.o2 = rows(o2), a.d_out = rows(g);
-        a.lse = lse.data_ptr<float>();
-        if (a.Tq == 0) a.lse = nullptr, a.o2.data = nullptr;
+        set_kept(a, t[5], t[6]);
+        if (out.defined()) a.out = rows(out);
+        a.d_out = rows(g);
         a.d_q = halves(dq), a.d_k = halves(dk), a.d_v = rows(dv);
         a.d_lam = dlam.data_ptr<float>();
         const c10::DeviceGuard guard(q.device());

@@ -5,7 +5,7 @@ header declares.  The product library exports them as ``sgl_*``.
 """
 import ctypes as C
 
-ABI_VERSION = 9
+ABI_VERSION = 10
 
 SGL_OK, SGL_EINVAL, SGL_ERANGE, SGL_ENOTSUP, SGL_EHIP, SGL_ENOMEM = 0, -1, -2, -3, -4, -5
 SAMPLE_RECENT, SAMPLE_UNIFORM = 0, 1
@@ -84,7 +84,7 @@ class DiffAttnArgs(C.Structure):
                 ("scale", f64), ("B", i64), ("Tq", i64), ("Tk", i64), ("B_dev", vp), ("q_ptr", vp), ("k_ptr", vp),
                 ("key_mask", vp), ("lam", vp), ("q", Rows), ("k", Rows), ("v", Rows), ("out", Rows), ("lse", vp),
                 ("o2", Rows), ("d_out", Rows), ("d_q", Rows), ("d_k", Rows), ("d_v", Rows), ("d_lam", vp),
-                ("flags", i32), ("reserved", i32)]
+                ("maps", vp), ("flags", i32), ("reserved", i32)]
 
 
 # in the order of sgl_struct_bytes(which)

@@ -216,21 +216,23 @@ class ModelOps:
         self._attn_args(q, k, v, lam, k_ptr, q_ptr, scale, causal, window, key_mask, None, True)
 
     def diff_attn(self, q, k, v, lam, k_ptr, q_ptr=None, scale=None, causal=False, window=None, key_mask=None, B_dev=None,
-                  zero_rest=False, out=None, lse=None, o2=None):
+                  zero_rest=False, out=None, lse=None, o2=None, maps=None):
         """out [Tq, Hq, Dv] = softmax(S_1) v - lam softmax(S_2) v over ragged sequences (sgl_diff_attn).  lse [Tq, Hq, 2]
-        float32 and o2 (like out) are written when given: diff_attn_backward reads them."""
+        float32 and maps [Tq, Hq, 2, Dv] float32, or o2 (like out), are written when given: diff_attn_backward reads them.
+        In 16 bits gradients from maps are free of the rounding of out and o2."""
         a = self._attn_args(q, k, v, lam, k_ptr, q_ptr, scale, causal, window, key_mask, B_dev, zero_rest)
         shape = (a.Tq, a.Hq, a.Dv)
         if out is None:
             out = self.be.torch.empty(shape, dtype=q.dtype, device=q.device)
-        if (lse is None) != (o2 is None):
-            raise ValueError("lse and o2 come together")
+        if (lse is None) != (o2 is None and maps is None):
+            raise ValueError("lse comes with o2 or maps")
         for name, t in (("out", out), ("o2", o2)):
             if t is not None:
                 self._written(name, self._rows_check(name, t, q.dtype, shape))
                 setattr(a, name, _rows(t))
         self._vec_check("lse", lse, "f32", (a.Tq, a.Hq, 2))
-        a.lse = self.be.ptr(lse)
+        self._vec_check("maps", maps, "f32", (a.Tq, a.Hq, 2, a.Dv))
+        a.lse, a.maps = self.be.ptr(lse), self.be.ptr(maps)
         n = self.lib.diff_attn_workspace_bytes(C.byref(a))
         ws = self._scratch(n) if n else None
         with self._on_device():
@@ -238,14 +240,19 @@ class ModelOps:
         return out
 
     def diff_attn_backward(self, d_out, q, k, v, lam, out, lse, o2, k_ptr, q_ptr=None, scale=None, causal=False, window=None,
-                           key_mask=None, B_dev=None, zero_rest=False, d_q=None, d_k=None, d_v=None):
-        """-> (d_q, d_k, d_v, d_lam) from what diff_attn was given, returned and kept."""
+                           key_mask=None, B_dev=None, zero_rest=False, d_q=None, d_k=None, d_v=None, maps=None):
+        """-> (d_q, d_k, d_v, d_lam) from what diff_attn was given, returned and kept; out and o2 may be None where maps
+        is given."""
         a = self._attn_args(q, k, v, lam, k_ptr, q_ptr, scale, causal, window, key_mask, B_dev, zero_rest)
         torch, shape = self.be.torch, (a.Tq, a.Hq, a.Dv)
+        if maps is None and (out is None or o2 is None):
+            raise ValueError("the backward call needs maps, or out and o2")
         for name, t in (("out", out), ("o2", o2), ("d_out", d_out)):
-            setattr(a, name, _rows(self._rows_check(name, t, q.dtype, shape)))
+            if t is not None or name == "d_out":
+                setattr(a, name, _rows(self._rows_check(name, t, q.dtype, shape)))
         self._vec_check("lse", lse, "f32", (a.Tq, a.Hq, 2))
-        a.lse = self.be.ptr(lse)
+        self._vec_check("maps", maps, "f32", (a.Tq, a.Hq, 2, a.Dv))
+        a.lse, a.maps = self.be.ptr(lse), self.be.ptr(maps)
         got = []
         for name, t, like in (("d_q", d_q, q), ("d_k", d_k, k), ("d_v", d_v, v)):
             if t is None:

@@ -207,3 +207,88 @@ def test_scales_past_32_bits_are_refused(hot):
     for scale in (1e39, -1e39, 3e38, math.inf, math.nan):
         with pytest.raises(ValueError, match="scale is not finite"):
             diff_attention(q, k, v, lam, _ptr([4]), scale=scale)
+
+
+def _one_key_bounds(q, k, v, lam, go, key):
+    """|dQ|, |dK| of rows i that see the one key key[i]: both are zero, a kernel with fp32 sums and states may be off by
+      e = 2 ((D + 4) U c sum |q k| + 4 U (|s| + 1))        the probability, from a score formed twice and an lse,
+      |dS| <= 1.01 (2 e + 2 (Dv + 8) U) sum |go v|,        two sums over the values (dP, t) and a result off by e + 4 U,
+    dS rounded to the type: in fp16 by up to 2^-25 absolutely"""
+    q, k, v, lam, go = (t.detach().cpu().double() for t in (q, k, v, lam, go))
+    Tq, Hq, _, D = q.shape
+    G, Dv, c = Hq // k.shape[1], v.shape[2], D ** -0.5
+    dq, dk = torch.zeros_like(q), torch.zeros_like(k)
+    for i, j in enumerate(key):
+        if j < 0:
+            continue
+        K, V = k[j].repeat_interleave(G, 0), v[j].repeat_interleave(G, 0)
+        for m in range(2):
+            mag, s = c * (q[i, :, m] * K[:, m]).abs().sum(-1), c * (q[i, :, m] * K[:, m]).sum(-1).abs()
+            e = 2 * ((D + 4) * plain.U * mag + 4 * plain.U * (s + 1))
+            dS = 1.01 * (2 * e + 2 * (Dv + 8) * plain.U) * (go[i] * V).abs().sum(-1) * (1 if m == 0 else lam.abs()) + 2.0 ** -24
+            dq[i, :, m] += c * dS[:, None] * K[:, m].abs() + 2.0 ** -24
+            dk[j, :, m] += (c * dS[:, None] * q[i, :, m].abs() + 2.0 ** -24).view(-1, G, D).sum(1)
+    return dq, dk
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("Hq,Hk,D,Dv", [(2, 2, 32, 64), (4, 1, 64, 128), (2, 1, 128, 256), (2, 2, 25, 50)])
+@pytest.mark.parametrize("form", ["roots", "rows", "split rows"])
+def test_a_single_visible_key_passes_no_gradient_to_queries_and_keys(hot, form, Hq, Hk, D, Dv, dtype):
+    """its probability is one whatever the score: the gradient's two terms cancel to what fp32 sums leave"""
+    n = 40
+    if form == "roots":
+        Tq, Tk, k_ptr, q_ptr, mask, key = n, n, _ptr([1] * n), None, None, list(range(n))
+    elif form == "rows":
+        Tq, Tk, k_ptr, q_ptr, mask = 3 * n, n, _ptr([1] * n), _ptr([3] * n), None
+        key = [i // 3 for i in range(Tq)]
+    else:
+        Tq, Tk, k_ptr, q_ptr = 6, 3000, _ptr([3000]), _ptr([6])
+        mask, key = torch.zeros(Tk, dtype=torch.bool, device="cuda"), [1500] * 6
+        mask[1500] = True
+    q, k, v, lam, go = _inputs(Tq, Tk, Hq, Hk, D, Dv, dtype, D)
+    leaves = [t.requires_grad_() for t in (q, k, v, lam)]
+    dq, dk, _, _ = torch.autograd.grad(diff_attention(*leaves, k_ptr, q_ptr, key_mask=mask), leaves, go)
+    tq, tk = _one_key_bounds(q, k, v, lam, go, key)
+    assert (dq.cpu().double().abs() <= tq).all() and (dk.cpu().double().abs() <= tk).all()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("D,Dv", [(32, 64), (64, 128), (128, 256), (25, 50), (7, 9)])
+@pytest.mark.parametrize("form", ["roots", "long", "rows", "split rows"])
+def test_unrounded_results_kept_for_the_backward_call(hot, form, D, Dv, dtype):
+    """maps, with and without o2 beside it: rows behind the live sequences stay as they were, gradients need no out and o2"""
+    nk = {"roots": [5, 0, 9, 4], "long": [700, 0, 900, 40], "rows": [40, 0, 70, 9], "split rows": [900, 0, 1100, 40]}[form]
+    nq = {"roots": [1] * 4, "long": [1] * 4, "rows": [20, 3, 50, 8], "split rows": [3, 2, 4, 1]}[form]
+    kp, q_ptr = _ptr(nk), None if nq[0] == 1 else _ptr(nq)
+    Tq, Tk, live = sum(nq), sum(nk), sum(nq[:3])
+    q, k, v, lam, go = _inputs(Tq, Tk, 4, 2, D, Dv, dtype, 23)
+    flat, B = (q.flatten(1, 2), k.flatten(1, 2), v), torch.tensor([3], device="cuda")
+    cut = None if q_ptr is None else q_ptr[:4]
+    ref = plain.diff_attention(q[:live], k, v, lam, kp[:4], cut, grad=go[:live])
+    got = []
+    for o2 in (None, torch.full((Tq, 4, Dv), 7.0, dtype=dtype, device="cuda")):
+        lse, maps = torch.full((Tq, 4, 2), 7.0, device="cuda"), torch.full((Tq, 4, 2, Dv), 7.0, device="cuda")
+        out = hot.diff_attn(*flat, lam, kp, q_ptr, B_dev=B, lse=lse, o2=o2, maps=maps)
+        _within(out[:live], ref, "out")
+        assert (maps[live:] == 7).all()
+        joined = maps[:live, :, 0] - lam[:, None] * maps[:live, :, 1]
+        _within(joined, ref, "out")
+        assert torch.equal(joined.to(dtype), out[:live]) or (joined - out[:live].float()).abs().max() <= 2 * plain.h(dtype) * joined.abs().max()
+        if o2 is not None:
+            assert torch.equal(o2[:live], maps[:live, :, 1].to(dtype)) and (o2[live:] == 7).all()
+        d = hot.diff_attn_backward(go, *flat, lam, None, lse, None, kp, q_ptr, B_dev=B, zero_rest=True, maps=maps)
+        for n, t, like in zip(("dq", "dk", "dv", "dlam"), d, (q, k, v, lam)):
+            r = t.view(like.shape)
+            if n == "dq":
+                assert not r[live:].any()
+                r = r[:live]
+            _within(r, ref, n)
+        got.append(d)
+    assert all(torch.equal(a, b) for a, b in zip(*got))
+    with pytest.raises(ValueError, match="maps, or out and o2"):
+        hot.diff_attn_backward(go, *flat, lam, out, lse, None, kp, q_ptr)
+    with pytest.raises(ValueError, match="lse comes with"):
+        hot.diff_attn(*flat, lam, kp, q_ptr, lse=lse)
+    with pytest.raises(ValueError, match="maps"):
+        hot.diff_attn(*flat, lam, kp, q_ptr, lse=lse, maps=maps[:, :, 0])
