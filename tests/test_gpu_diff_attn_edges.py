@@ -292,3 +292,101 @@ def test_unrounded_results_kept_for_the_backward_call(hot, form, D, Dv, dtype):
         hot.diff_attn(*flat, lam, kp, q_ptr, lse=lse)
     with pytest.raises(ValueError, match="maps"):
         hot.diff_attn(*flat, lam, kp, q_ptr, lse=lse, maps=maps[:, :, 0])
+
+
+# every kernel and way of staging: 16-byte chunks whole, padded, and through registers
+KERNELS = [(64, 128, BF16), (128, 256, BF16), (64, 128, F32), (128, 256, F32), (48, 96, BF16), (80, 160, F16), (100, 200, F32), (50, 100, BF16), (100, 200, F16), (25, 50, F32)]
+
+
+def _layout(form):
+    """-> lengths of the keys, of the queries (None: one each), causal"""
+    if form == "single queries":
+        return [300, 75, 0, 220, 1], None, False
+    if form == "split rows":
+        return [700, 1, 900, 600], [5, 1, 9, 3], True
+    return [40, 25, 70, 10], [40, 25, 70, 10], True
+
+
+def _visibility(nk, nq, causal):
+    nq = nq or [1] * len(nk)
+    see = torch.zeros(sum(nq), sum(nk), dtype=torch.bool)
+    q0 = k0 = 0
+    for a, b in zip(nq, nk):
+        see[q0:q0 + a, k0:k0 + b] = plain.visible(a, b, causal, None)
+        q0, k0 = q0 + a, k0 + b
+    return see
+
+
+def _held(got, ref, name, clean):
+    """within bounds where `clean` says that nothing of it got in"""
+    got, clean = got.detach().cpu().double(), clean.expand(got.shape)
+    off = (got - ref[name]).abs() - ref[name + "_tol"]
+    assert not ((off > 0) | got.isnan())[clean].any(), name
+
+
+@pytest.mark.parametrize("D,Dv,dtype", KERNELS)
+@pytest.mark.parametrize("form", ["rows", "split rows", "single queries"])
+@pytest.mark.parametrize("what", ["q", "k", "v", "go"])
+def test_a_nan_reaches_what_sees_it_and_nothing_else(hot, what, form, D, Dv, dtype):
+    nk, nq, causal = _layout(form)
+    see = _visibility(nk, nq, causal)
+    Tq, Tk = see.shape
+    q, k, v, lam, go = _inputs(Tq, Tk, 4, 1, D, Dv, dtype, 29)
+    k_ptr, q_ptr = _ptr(nk), None if nq is None else _ptr(nq)
+    ref = plain.diff_attention(q, k, v, lam, k_ptr, q_ptr, causal=causal, grad=go)
+    # in the middle of a long sequence: a row, a key, and an element of either's value
+    i, j = {"rows": (50, 100), "split rows": (8, 900), "single queries": (1, 310)}[form]
+    rows, keys = torch.zeros(Tq, dtype=torch.bool), torch.zeros(Tk, dtype=torch.bool)
+    bad = [t.clone() for t in (q, k, v, go)]
+    if what in "kv":
+        bad["qkv".index(what)][j, :, 5 if what == "v" else 1] = float("nan")           # (k: the second map)
+        rows = see[:, j]
+        keys = see[rows].any(0)
+    else:
+        bad[0 if what == "q" else 3][(i, slice(None), 0) if what == "q" else (i, slice(None), 5)] = float("nan")
+        rows[i] = True
+        keys = see[i]
+    leaves = [t.requires_grad_() for t in (*bad[:3], lam)]
+    y = diff_attention(*leaves, k_ptr, q_ptr, causal=causal)
+    dq, dk, dv, dlam = torch.autograd.grad(y, leaves, bad[3])
+    five = torch.arange(Dv) == 5
+    r3, k3, r4, k4 = rows[:, None, None], keys[:, None, None], rows[:, None, None, None], keys[:, None, None, None]
+    assert rows.any() and keys.any() and not rows.all() and not keys.all()
+    # what it enters
+    hit = {"q": (r3, r4, k4, k3), "k": (r3, r4, k4, k3), "v": (r3 & five, r4, k4, k3 & False), "go": (r3 & False, r4, k4, k3 & five)}[what]
+    for t, name, m in zip((y, dq, dk, dv), ("out", "dq", "dk", "dv"), hit):
+        _held(t, ref, name, ~m)
+        m = m.expand(t.shape).to(t.device)
+        if name in ("dq", "dk") and what in "qk":                   # (of one map for sure)
+            of = 0 if what == "q" else 1
+            assert t[:, :, of][m[:, :, of]].isnan().all(), name
+        else:
+            assert t[m].isnan().all(), name
+    assert dlam.isnan().any() or what == "q"
+
+
+@pytest.mark.parametrize("D,Dv,dtype", KERNELS)
+@pytest.mark.parametrize("form", ["rows", "split rows", "single queries"])
+def test_hidden_keys_may_hold_anything(hot, form, D, Dv, dtype):
+    """NaN and infinities in the keys and values that the mask hides, and in rows of no sequence"""
+    nk, nq, causal = _layout(form)
+    lead = 3
+    Tq, Tk = sum(nq) + 2 * lead if nq else len(nk), sum(nk) + 2 * lead
+    q, k, v, lam, go = _inputs(Tq, Tk, 4, 1, D, Dv, dtype, 31)
+    k_ptr, q_ptr = _ptr(nk, lead), None if nq is None else _ptr(nq, lead)
+    mask = torch.rand(Tk, generator=torch.Generator().manual_seed(5)).cuda() < 0.6
+    mask[lead:lead + 3] = False
+    clean = [torch.where(mask.view(-1, *[1] * (t.dim() - 1)), t, 0.0) for t in (k, v)]
+    ref = plain.diff_attention(q, *clean, lam, k_ptr, q_ptr, causal=causal, key_mask=mask, grad=go)
+    k[~mask], v[~mask] = float("nan"), float("-inf")
+    none = torch.ones(Tk, dtype=torch.bool, device="cuda")
+    none[lead:-lead] = False
+    k[none], v[none] = float("inf"), float("nan")
+    if nq is not None:
+        q[:lead], go[-lead:] = float("nan"), float("inf")
+    leaves = [t.requires_grad_() for t in (q, k, v, lam)]
+    y = diff_attention(*leaves, k_ptr, q_ptr, causal=causal, key_mask=mask)
+    grads = torch.autograd.grad(y, leaves, go)
+    for t, name in zip((y, *grads), ("out", "dq", "dk", "dv", "dlam")):
+        _within(t, ref, name)
+    assert not grads[1][~mask].any() and not grads[2][none].any()
