@@ -797,8 +797,8 @@ int32_t sgl_qk_norm_rotary_backward(const sgl_rotary_params* p, double eps, int3
  * is seen makes what it enters NaN.
  * Rows of no sequence: zeros with SGL_ATTN_ZERO_REST, else left as they were.
  * B_dev (when given) is the live number of sequences, <= B.
- * |scale| <= 2.3e38; 1 <= D <= 128, 1 <= Dv <= 256; Tq, Tk and B at most 2^31 - 256, Tq * Hq and
- * Tk * Hk below 2^31. */
+ * |scale| <= 2.3e38; 1 <= D <= 128, 1 <= Dv <= 256; Tq, Tk and B at most
+ * 2^31 - 256, Tq * Hq and Tk * Hk below 2^31. */
 #define SGL_ATTN_ZERO_REST 1
 typedef struct {
     int32_t        dtype, Hq, Hk, D, Dv, causal;

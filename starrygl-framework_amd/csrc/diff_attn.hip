@@ -79,7 +79,11 @@ int32_t check_args(const char* what, const sgl_diff_attn_args* a, Call call) {
 //   16 heads over 4, 64 wide, bf16   n = 32: 260, 148   48: 187, 130   64: 145, 122   96: 115, 120   128: 91, 119
 //    8 heads over 8, 64 wide, bf16   n = 64: 196, 110   128: 142, 102   256: 124, 93   512: 107, 137
 //    2 heads over 2, 32 wide, fp32   n = 64: 64, 25   128: 49, 28   256: 43, 48   512: 44, 84
-// so groups of one or two heads stay there longer, if there is a wave for every SIMD.
+//    2 heads over 1, 32 wide, fp32   n = 64: 37, 18    96: 39, 22   128: 29, 26   192: 33, 37   256: 25, 47
+//   16 heads over 8, 64 wide, bf16   n = 64: 228, 192  96: 185, 192 128: 157, 198 192: 141, 214
+// so groups of one or two heads stay there longer, if there is a wave for every SIMD (groups of two wide heads lose by it from about
+// 96 keys on).  The rule knows the average length only: one long sequence among short ones is walked by a wave a head (12000 roots of
+// 10 keys, 2 heads, 32 wide, fp32: 29 us; one of them with 1000 more 179, with 10000 more 1683).
 bool by_segments(const sgl_diff_attn_args& a) {
     const int64_t keys = a.Hq / a.Hk <= 2 && a.B * a.Hq >= 1024 ? 192 : 64;
     return !a.q_ptr && a.Tk < keys * a.B;

@@ -8,8 +8,8 @@
 // type for those products, once each; everything else is fp32.
 //
 // Bound by the matrix and vector instructions of a wave, which alternate in the order written here.  8 sequences of 2048, 16
-// heads over 4, 64 wide, causal, bf16: rows 295 us (0.70 PFLOP/s), keys 455 us (0.60 PFLOP/s); 2 of 4096, 8 over 2, 128 wide:
-// 460 us (0.90) and 757 us (0.73).  A map to a wave, dP formed twice: rows 367 and 507 us.  Keys with dK and dV in waves of their
+// heads over 4, 64 wide, causal, bf16: rows 315 us (0.66 PFLOP/s), keys 455 us (0.60 PFLOP/s); 2 of 4096, 8 over 2, 128 wide:
+// 480 us (0.86) and 757 us (0.73).  A map to a wave, dP formed twice: rows 367 and 507 us.  Keys with dK and dV in waves of their
 // own, scores formed twice: 525 and 1098 us; a map to a wave, dP twice: 517 and 981 us.
 #pragma once
 

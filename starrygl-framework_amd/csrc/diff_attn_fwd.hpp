@@ -18,9 +18,9 @@
 //
 // Bound by the matrix and vector instructions, which overlap between the two waves of a SIMD only in part (a tile of 32 x 32: 768
 // cycles of products, about 720 of vector instructions, 2000 measured).  8 sequences of 2048, 16 heads over 4, 64 wide, causal,
-// bf16: 270 us, 0.76 PFLOP/s; 2 of 4096, 8 over 2, 128 wide: 405 us, 1.02 PFLOP/s.  Tiles of 32 keys: 277 us for the former; the
-// exponentials of one map between the products of the other, which reads the values twice: 288 us.  Single queries are bound by
-// the keys' bytes: 16 histories of up to 32768 keys, 16 heads over 4, 117 us, 4.7 TB/s (a copy reaches 5.0).
+// bf16: 270 us, 0.76 PFLOP/s; 2 of 4096, 8 over 2, 128 wide: 405 us, 1.02 PFLOP/s; with both maps' results kept for a backward call
+// 315 and 440 us.  Tiles of 32 keys: 277 us for the first; the exponentials of one map between the products of the other, which
+// reads the values twice: 288 us.  Single queries are bound by the keys' bytes: 16 histories of up to 32768 keys, 16 heads over 4, 117 us, 4.7 TB/s (a copy reaches 5.0).
 #pragma once
 
 #include "diff_attn.hpp"
