@@ -253,6 +253,14 @@ __global__ __launch_bounds__(BLOCK) void seg_bwd_kernel(AttnArgs g) {
                 store_part<T>(row_out<T>(a.d_v, j, hk), dv, 1.f, ln.ev, a.Dv, g.grain);
             }
         }
+        if (DKV && a.window > 0) {
+            // keys of the sequence in front of the window
+            const float none[EP] = {};
+            for (int32_t j = clamp_to(a.k_ptr[i], a.Tk) + ln.slot; j < span.lo; j += SLOTS) {
+                store_part<T>(row_out<T>(a.d_k, j, 2 * hk + ln.half), none, 1.f, ln.e, a.D, g.grain);
+                store_part<T>(row_out<T>(a.d_v, j, hk), none, 1.f, ln.ev, a.Dv, g.grain);
+            }
+        }
         if (DQ) {
 #pragma unroll
             for (int e = 0; e < EP; ++e) {

@@ -390,3 +390,26 @@ def test_hidden_keys_may_hold_anything(hot, form, D, Dv, dtype):
     for t, name in zip((y, *grads), ("out", "dq", "dk", "dv", "dlam")):
         _within(t, ref, name)
     assert not grads[1][~mask].any() and not grads[2][none].any()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("Hq,Hk", [(2, 2), (4, 2)])
+@pytest.mark.parametrize("rest", [False, True])
+@pytest.mark.parametrize("window", [1, 3, 40])
+def test_window_of_single_queries(hot, window, rest, Hq, Hk, dtype):
+    """keys of a sequence in front of the window get gradients of zero, whatever the buffers held"""
+    nk, lead = [5, 0, 30, 1, 100], 3
+    k_ptr, Tk = _ptr(nk, lead), sum(nk) + 2 * lead
+    q, k, v, lam, go = _inputs(5, Tk, Hq, Hk, 32, 64, dtype, 37)
+    _, ref = _check(q, k, v, lam, go, k_ptr, causal=True, window=window)
+    flat, how = (q.flatten(1, 2), k.flatten(1, 2), v), dict(causal=True, window=window, zero_rest=rest)
+    lse, maps = torch.empty(5, Hq, 2, device="cuda"), torch.empty(5, Hq, 2, 64, device="cuda")
+    hot.diff_attn(*flat, lam, k_ptr, lse=lse, maps=maps, **how)
+    d_k, d_v = torch.full_like(flat[1], 7.0), torch.full_like(v, 7.0)
+    got = hot.diff_attn_backward(go, *flat, lam, None, lse, None, k_ptr, maps=maps, d_k=d_k, d_v=d_v, **how)
+    live = slice(lead, Tk - lead)
+    for n, t, like in zip(("dq", "dk", "dv", "dlam"), got, (q, k, v, lam)):
+        cut = live if n in ("dk", "dv") else slice(None)
+        _within(t.view(like.shape)[cut], {n: ref[n][cut], n + "_tol": ref[n + "_tol"][cut]}, n)
+    for t in (d_k, d_v):
+        assert (t[:lead] == (0 if rest else 7)).all() and (t[Tk - lead:] == (0 if rest else 7)).all()
